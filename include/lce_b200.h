@@ -282,6 +282,46 @@ int lce_read_status(void* workspace, void* stream);
 int lce_eval_loss_static(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
                          const int64_t* labels, float* out5, void* stream);
 
+/* ---- operators on given logits ------------------------------------------------------------------
+ * No counterpart in the reference. They need no workspace; logits: [rows, vocab] device memory of element type dtype, rows
+ * ld elements apart (ld >= 0, any alignment of the element type).
+ *
+ * lce_top_logits: the k largest logits of each row, descending, equal ones by ascending index (-0 equals +0, a NaN
+ * is larger than everything), and lse = log(sum_j exp(logit_j / temperature)).
+ * values: [rows, k] in dtype; indices: int64 [rows, k]; lse: float [rows]. 1 <= k <= min(vocab, LCE_TOP_MAX).
+ *
+ * lce_sample_logits: one token per row, drawn from given random numbers. With w_j = exp((l_j - max l) / temperature) and
+ * the order (logit descending, index ascending): the first top_k of the order stay (0: all); of those the shortest
+ * prefix whose mass reaches top_p of their mass (1: all); of those w_j >= min_p (0: all). The token is the first
+ * one in index order at which the kept weights, added up, exceed u * (their sum); logprobs = log(w / their sum).
+ * temperature 0: the largest logit with the lowest index. -inf and NaN logits are never drawn; +inf logits share all the
+ * mass. A row without any logit that may be drawn gives token -1 and logprob -inf.
+ * Weights and their sums are held in 64-bit integers: the answer does not depend on the order of summation. */
+#define LCE_TOP_MAX 1024
+int lce_top_logits(int32_t dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, int32_t k,
+                   float temperature, void* values, int64_t* indices, float* lse, void* stream);
+
+#define LCE_SAMPLING_U_F64 3 /* u_dtype: double (LCE_DTYPE_F32: float) */
+/* Each setting is one value for all rows, or -- where the pointer is not null -- one device value per row. Values
+ * out of range in device memory are taken as the nearest that means something: temperature <= 0 or NaN as 0, top_k <= 0 as all,
+ * top_p <= 0 as the first token alone, >= 1 or NaN as all, min_p <= 0 or NaN as none, > 1 as 1; u outside [0, 1) as
+ * the nearest inside. The values for all rows are checked (LCE_ERR_INVALID_ARGUMENT). */
+typedef struct lce_sampling {
+  const void* u;            /* [rows] random numbers in [0, 1) */
+  const float* temperature; /* [rows] or null */
+  const int32_t* top_k;     /* [rows] or null */
+  const float* top_p;       /* [rows] or null */
+  const float* min_p;       /* [rows] or null */
+  double temperature_all;
+  double top_p_all;
+  double min_p_all;
+  int64_t top_k_all;
+  int32_t u_dtype;
+  int32_t reserved;
+} lce_sampling;
+int lce_sample_logits(int32_t dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
+                      const lce_sampling* s, int64_t* tokens, float* logprobs, void* stream);
+
 /* ---- measurement ------------------------------------------------------------------------------
  * With profiling enabled, a CUDA event pair is recorded on the launching stream around each of the
  * three tensor-core contractions (0: logits z = x W, 1: dx = dZ W^T, 2: dW = x^T dZ).

@@ -1,7 +1,8 @@
 """B200-native fused linear + cross-entropy loss.
 
 Same public names as ``linear_cross_entropy`` (the reference package, __init__.py:1):
-``LinearCrossEntropyLoss``, ``linear_cross_entropy``, ``fwd_configs``, ``bwd_configs``.
+``LinearCrossEntropyLoss``, ``linear_cross_entropy``, ``fwd_configs``, ``bwd_configs``. Beside them, on the same heads:
+``top_logits`` and ``sample_logits``.
 """
 from .ops import (  # noqa: F401
     LinearCrossEntropyLoss,
@@ -12,4 +13,7 @@ from .ops import (  # noqa: F401
     set_autocast_policy,
 )
 
-__all__ = ["LinearCrossEntropyLoss", "linear_cross_entropy", "fwd_configs", "bwd_configs", "set_autocast_policy"]
+from .head import Sampled, TopLogits, sample_logits, top_logits  # noqa: F401
+
+__all__ = ["LinearCrossEntropyLoss", "linear_cross_entropy", "fwd_configs", "bwd_configs", "set_autocast_policy",
+           "top_logits", "TopLogits", "sample_logits", "Sampled"]

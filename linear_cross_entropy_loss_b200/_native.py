@@ -9,6 +9,7 @@ import ctypes
 import os
 import shutil
 import subprocess
+import tempfile
 import threading
 from pathlib import Path
 
@@ -57,7 +58,8 @@ class Problem(ctypes.Structure):
 
 
 def _sources():
-    return sorted(list(_CSRC.glob("*.cu")) + list(_CSRC.glob("*.cuh")) + list(_INCLUDE.glob("*.h")))
+    return sorted(list(_CSRC.glob("*.cu")) + list(_CSRC.glob("*.cuh")) + list(_CSRC.glob("*.h"))
+                  + list(_INCLUDE.glob("*.h")))
 
 
 def needs_build() -> bool:
@@ -92,23 +94,29 @@ def _build_locked(verbose: bool) -> Path:
     if not os.path.exists(nvcc):
         raise RuntimeError("nvcc not found: liblce_b200.so cannot be built")
     tmp = LIB_PATH.parent / f"{LIB_PATH.name}.{os.getpid()}.tmp"
-    cmd = [
-        nvcc,
+    flags = [
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-O3", "-lineinfo", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC",
+        "-Xcompiler", "-fPIC",
         "-I", str(_INCLUDE),
-        "-o", str(tmp),
-        str(_CSRC / "lce_api.cu"),
     ]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+        flags.append("-Xptxas=-v")
+    with tempfile.TemporaryDirectory() as objects:
+        # one compiler per translation unit, side by side
+        units = [(src, str(Path(objects) / f"{src.stem}.o")) for src in sorted(_CSRC.glob("*.cu"))]
+        procs = [subprocess.Popen([nvcc, *flags, "-c", str(src), "-o", obj], stdout=subprocess.PIPE,
+                                  stderr=subprocess.STDOUT, text=True) for src, obj in units]
+        logs = [proc.communicate()[0] for proc in procs]
+        if any(proc.returncode != 0 for proc in procs):
+            raise RuntimeError("nvcc failed:\n" + "\n".join(logs))
+        link = subprocess.run([nvcc, *flags, "-shared", "-o", str(tmp), *(obj for _, obj in units)],
+                              capture_output=True, text=True)
+        if link.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + link.stdout + link.stderr)
     os.replace(tmp, LIB_PATH)
     if verbose:
-        print(proc.stderr)
+        print("\n".join(logs))
     return LIB_PATH
 
 
@@ -126,6 +134,27 @@ class PeerTable(ctypes.Structure):
 
     _fields_ = [("world", ctypes.c_int32), ("rank", ctypes.c_int32), ("base", ctypes.c_void_p * MAX_PEERS)]
 
+
+class Sampling(ctypes.Structure):
+    """Mirror of ``lce_sampling``: each setting one value for all rows, or a device pointer to one per row."""
+
+    _fields_ = [
+        ("u", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("top_k", ctypes.c_void_p),
+        ("top_p", ctypes.c_void_p),
+        ("min_p", ctypes.c_void_p),
+        ("temperature_all", ctypes.c_double),
+        ("top_p_all", ctypes.c_double),
+        ("min_p_all", ctypes.c_double),
+        ("top_k_all", ctypes.c_int64),
+        ("u_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+SAMPLING_U_F64 = 3
+TOP_MAX = 1024
 
 # name -> (restype, argtypes); kept in one table so that a test can check it against the header.
 SIGNATURES = {
@@ -166,6 +195,10 @@ SIGNATURES = {
     "lce_read_status": (ctypes.c_int, [_vp, _vp]),
     "lce_rerun_stats_async": (ctypes.c_int, [_vp, _vp, _vp]),
     "lce_eval_loss_static": (ctypes.c_int, [ctypes.POINTER(Problem), _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "lce_top_logits": (
+        ctypes.c_int, [_i32, _vp, _i64, _i64, _i64, _i32, ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "lce_sample_logits": (
+        ctypes.c_int, [_i32, _vp, _i64, _i64, _i64, ctypes.POINTER(Sampling), _vp, _vp, _vp]),
     "lce_profile_enable": (ctypes.c_int, [_i32]),
     "lce_profile_read": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_longlong)]),
     "lce_debug_gemm": (

@@ -1,6 +1,6 @@
 // C ABI of the library (declared in include/lce_b200.h): argument validation, workspace layout,
 // TMA tensor-map construction and kernel launches. No device memory is allocated here.
-#include "../../include/lce_b200.h"
+#include "launch.h"
 
 #include "aux_kernels.cuh"
 #include "gemm_sm100.cuh"
@@ -15,11 +15,13 @@
 #include <mutex>
 #include <vector>
 
+namespace lce {
+std::atomic<long long> g_launches{0};
+}
+
 namespace {
 
 using namespace lce;
-
-std::atomic<long long> g_launches{0};
 
 // ------------------------------------------------------------------------------------------------
 // device bookkeeping
@@ -315,11 +317,6 @@ int choose_raster_group(int fast_tiles, int fast_tile_rows) {
 // ------------------------------------------------------------------------------------------------
 // launches
 // ------------------------------------------------------------------------------------------------
-int check_launch() {
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return cudaGetLastError() == cudaSuccess ? LCE_OK : LCE_ERR_CUDA;
-}
-
 // Optional per-launch timing of the three tensor-core contractions (lce_profile_enable): a CUDA event
 // pair is recorded on the launching stream around each GEMM kernel and read back by lce_profile_read.
 enum : int { PROF_FWD = 0, PROF_DX = 1, PROF_DW = 2, PROF_KINDS = 3 };

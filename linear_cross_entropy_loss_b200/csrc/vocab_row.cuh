@@ -1,0 +1,158 @@
+// Pieces shared by the kernels that work on one row of logits (top_logits.cuh, sample_logits.cuh): the order of the
+// logits, the exact weights of the sampler, block-wide reductions and sorting.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace lce {
+
+__device__ __forceinline__ float logit_to_float(float v) { return v; }
+__device__ __forceinline__ float logit_to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float logit_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Logits as unsigned keys in the same order: -inf = kKeyNegInf < finite < +inf < NaN (all NaN alike); -0 equals +0.
+constexpr uint32_t kKeyNegInf = 0x007fffffu;
+constexpr uint32_t kKeyPosInf = 0xff800000u;
+constexpr uint32_t kKeyNaN = 0xffffffffu;
+__device__ __forceinline__ uint32_t order_key(float f) {
+  const uint32_t b = __float_as_uint(f + 0.0f);
+  const uint32_t key = b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+  return f != f ? kKeyNaN : key;
+}
+__device__ __forceinline__ float key_to_float(uint32_t key) {
+  if (key == kKeyNaN) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);
+}
+
+// A logit and its place as one number: larger = larger logit, then lower index.
+__device__ __forceinline__ unsigned long long order_pair(uint32_t key, uint32_t index) {
+  return ((unsigned long long)key << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t pair_key(unsigned long long pair) { return uint32_t(pair >> 32); }
+__device__ __forceinline__ uint32_t pair_index(unsigned long long pair) { return 0xffffffffu - uint32_t(pair); }
+
+// ---------------------------------------------------------------------------------------------
+// block-wide steps; every thread of the block takes part, blockDim.x is a multiple of 32
+// ---------------------------------------------------------------------------------------------
+template <typename T, typename Op>
+__device__ __forceinline__ T block_reduce(T v, T* scratch /*[32]*/, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  __syncthreads();  // scratch may still be read from an earlier call
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  v = scratch[lane < warps ? lane : 0];
+  T r = v;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const T other = __shfl_xor_sync(0xffffffffu, r, o);
+    r = op(r, other);
+  }
+  return r;  // warps beyond the block repeat scratch[0]: fine for max / min; block_sum masks them itself
+}
+template <typename T>
+__device__ __forceinline__ T block_max(T v, T* scratch) {
+  return block_reduce(v, scratch, [](T a, T b) { return a > b ? a : b; });
+}
+template <typename T>
+__device__ __forceinline__ T block_sum(T v, T* scratch /*[32]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  __syncthreads();
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  T r = lane < warps ? scratch[lane] : T(0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+  return r;
+}
+// Sum of v over the threads before this one; the sum over all of them in *total.
+template <typename T>
+__device__ __forceinline__ T block_prefix(T v, T* scratch /*[32]*/, T* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  T inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T other = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += other;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = inc;
+  __syncthreads();
+  T w = lane < warps ? scratch[lane] : T(0);
+  T winc = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T other = __shfl_up_sync(0xffffffffu, winc, o);
+    if (lane >= o) winc += other;
+  }
+  *total = __shfl_sync(0xffffffffu, winc, 31);
+  const T before = __shfl_sync(0xffffffffu, winc - w, warp);
+  return before + inc - v;
+}
+
+// Sorts n (a power of two) numbers in shared memory, largest first.
+__device__ __forceinline__ void block_sort_descending(unsigned long long* a, int n) {
+  for (int size = 2; size <= n; size <<= 1) {
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < (n >> 1); i += blockDim.x) {
+        const int lo = ((i & ~(stride - 1)) << 1) | (i & (stride - 1));
+        const int hi = lo | stride;
+        const unsigned long long x = a[lo], y = a[hi];
+        const bool descending = (lo & size) == 0;
+        if ((x < y) == descending) {
+          a[lo] = y;
+          a[hi] = x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------
+// weights of the sampler
+// ---------------------------------------------------------------------------------------------
+// w = exp((l - max) / T) as an integer: w * 2^bits rounded to the nearest. Integers add up to the same sum in any
+// order, so the sums of a row do not depend on how it is split over threads and blocks, and a token's border is where
+// 64-bit arithmetic puts it: the rounding of one weight is 2^-(bits + 1) of the largest one (bits = 44 for up to
+// 2^18 columns), that of the exponential below 2^-47. A sum of 32-bit floats would be off by 1e-7 of the total, which is
+// as wide as the share of a token in the tail of a vocabulary.
+//   exp(d / T) = 2^(n / 32) (1 + x + x^2 / 2 + ...),  n = round(32 d log2(e) / T),  |x| <= ln(2) / 64
+struct RowWeights {
+  double largest;        // the row's largest logit
+  double steps;          // 32 log2(e) / T: logit difference -> n
+  double to_int;         // 2^(52 - bits): adding it leaves w * 2^bits in the low bits of the sum
+  const double* table;   // shared memory: 2^(j / 32), j = 0 .. 31
+  bool only_largest;     // the largest logit is +inf: it alone has weight
+};
+constexpr int kWeightBits = 44;
+constexpr double kStepLn2 = 0.021660849392498290;  // ln(2) / 32
+
+__device__ __forceinline__ double weight_steps(const RowWeights& w, float logit) {
+  return (double(logit) - w.largest) * w.steps;
+}
+__device__ __forceinline__ unsigned long long row_weight(const RowWeights& w, float logit) {
+  if (w.only_largest) return double(logit) == w.largest ? 1ull << 32 : 0ull;
+  const double t = weight_steps(w, logit);
+  if (!(t > -32.0 * (kWeightBits + 2))) return 0ull;  // rounds to nothing; also -inf and NaN
+  const double shifted = t + 6755399441055744.0;      // 1.5 * 2^52: the integer part ends up in the low word
+  const int n = __double2loint(shifted);
+  const double x = (t - (shifted - 6755399441055744.0)) * kStepLn2;
+  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(x, p, 1.0 / 6.0);
+  p = fma(x, p, 0.5);
+  p = fma(x, p, 1.0);
+  p = fma(x, p, 1.0);
+  p *= w.table[n & 31];
+  p = __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+  return (unsigned long long)(__double_as_longlong(p + w.to_int) - __double_as_longlong(w.to_int));
+}
+
+}  // namespace lce

@@ -1,0 +1,130 @@
+"""What a vocabulary head answers with: the largest logits of a row, and tokens drawn from it.
+
+``top_logits`` lists the k largest logits of each row with the row's log-sum-exp -- the form in which a teacher's
+distribution is kept for :func:`linear_distillation`. ``sample_logits`` draws one token per row from given random
+numbers. Both read each logit once and run as one kernel launch in ``liblce_b200.so``, on the current stream of the
+logits' device; like the loss they have no CPU fallback. The reference project has no counterpart of either.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Union
+
+import torch
+
+from . import _native
+from .ops import _DTYPE_CODE, _device_guard, get_backend
+
+
+class TopLogits(NamedTuple):
+    values: torch.Tensor   # (..., k) in the type of the logits, descending
+    indices: torch.Tensor  # (..., k) int64
+    lse: torch.Tensor      # (...) float32: logsumexp(logits / temperature) over the whole row
+
+
+class Sampled(NamedTuple):
+    tokens: torch.Tensor    # (...) int64
+    logprobs: torch.Tensor  # (...) float32: of the token, in the distribution that was drawn from
+
+
+def _rows_of(logits: torch.Tensor) -> torch.Tensor:
+    """(rows, V) with unit inner stride; leading dimensions merged (a copy only where the strides do not allow it)."""
+    assert logits.dim() >= 1 and logits.shape[-1] >= 1, "logits must have at least one column"
+    assert logits.dtype in _DTYPE_CODE, f"unsupported dtype {logits.dtype}"
+    rows = logits.detach().reshape(-1, logits.shape[-1])
+    return rows if rows.stride(1) == 1 or rows.shape[1] == 1 else rows.contiguous()
+
+
+def _require_cuda(backend, *tensors) -> None:
+    if getattr(backend, "requires_cuda", True) and not all(t.is_cuda for t in tensors):
+        raise RuntimeError("linear_cross_entropy_loss_b200 runs on CUDA tensors only; there is no CPU fallback")
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The k largest logits of each row, descending, equal ones by ascending index, and the row's log-sum-exp.
+
+    logits: (..., V) in float16, bfloat16 or float32; rows may start anywhere and lie any distance apart.
+    1 <= k <= min(V, 1024). NaN counts as larger than everything, as in ``torch.topk``; ``lse`` is NaN then.
+    ``temperature`` only enters ``lse`` = logsumexp(logits / temperature). Not differentiable.
+    """
+    k = int(k)
+    rows = _rows_of(logits)
+    assert 1 <= k <= rows.shape[1], "k must lie between 1 and the number of columns"
+    assert k <= _native.TOP_MAX, f"k must be at most {_native.TOP_MAX}"
+    assert temperature > 0, "temperature must be positive"
+    backend = get_backend()
+    _require_cuda(backend, rows)
+    lead = logits.shape[:-1]
+    n, dev = rows.shape[0], rows.device
+    values = torch.empty((n, k), dtype=rows.dtype, device=dev)
+    indices = torch.empty((n, k), dtype=torch.int64, device=dev)
+    lse = torch.empty(n, dtype=torch.float32, device=dev)
+    with _device_guard(rows):
+        backend.top_logits(rows, k, float(temperature), values, indices, lse)
+    return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
+
+
+def _setting(value, name: str, dtype, n: int, device):
+    """(value for all rows, None) or (None, one value per row on the device)."""
+    if not isinstance(value, torch.Tensor):
+        return value, None
+    assert value.numel() in (1, n), f"{name} must be a number or have one entry per row"
+    assert value.device == device, f"{name} must be on the device of the logits"
+    value = value.detach().reshape(-1)
+    if dtype == torch.int32:
+        assert not value.is_floating_point(), f"{name} must hold whole numbers"
+        if value.dtype != torch.int32:
+            value = value.clamp(0, 2**31 - 1)
+    return None, value.to(dtype).expand(n).contiguous()
+
+
+def sample_logits(
+    logits: torch.Tensor,
+    u: torch.Tensor,
+    temperature: Union[float, torch.Tensor] = 1.0,
+    top_k: Union[int, torch.Tensor] = 0,
+    top_p: Union[float, torch.Tensor] = 1.0,
+    min_p: Union[float, torch.Tensor] = 0.0,
+) -> Sampled:
+    """One token of each row, drawn with the random number that is given for it.
+
+    logits: (..., V) in float16, bfloat16 or float32. u: (...) float32 or float64 in [0, 1).
+    With w_j = exp((l_j - max l) / temperature) and the order (logit descending, index ascending): the first ``top_k`` of
+    the order stay (0: all); of those the shortest prefix whose mass reaches ``top_p`` of their mass; of those
+    w_j >= ``min_p``. The token is the first one in INDEX order at which the kept weights, added up, exceed u times their
+    sum; ``logprobs`` is log(w / sum). temperature 0 gives the largest logit (the lowest index among equals).
+
+    Each setting is a number, which is checked, or a tensor with one entry per row (float32; ``top_k`` int32), which is not: out-of-range
+    entries are taken as the nearest value that means something. -inf and NaN logits are never drawn; +inf logits share
+    all the mass. A row without any logit to draw gives token -1 and logprob -inf.
+
+    Weights and sums are kept in 64-bit integers, so the answer for a row depends on its inputs alone.
+    """
+    rows = _rows_of(logits)
+    n, dev = rows.shape[0], rows.device
+    assert u.numel() == n, "u must have one entry per row of the logits"
+    assert u.dtype in (torch.float32, torch.float64), "u must be float32 or float64"
+    assert u.device == dev, "u must be on the device of the logits"
+    s = _native.Sampling(u_dtype=_native.DTYPE_F32 if u.dtype == torch.float32 else _native.SAMPLING_U_F64)
+    u = u.detach().reshape(-1).contiguous()
+    s.u = u.data_ptr()
+    alive = []  # what the pointers in `s` refer to, until the kernel has been enqueued
+    for name, dtype, value in (("temperature", torch.float32, temperature), ("top_k", torch.int32, top_k),
+                               ("top_p", torch.float32, top_p), ("min_p", torch.float32, min_p)):
+        number, tensor = _setting(value, name, dtype, n, dev)
+        if tensor is None:
+            setattr(s, f"{name}_all", int(number) if name == "top_k" else float(number))
+        else:
+            alive.append(tensor)
+            setattr(s, name, tensor.data_ptr())
+    assert s.temperature or s.temperature_all >= 0, "temperature must not be negative"
+    assert s.top_k or s.top_k_all >= 0, "top_k must not be negative"
+    assert s.top_p or 0 < s.top_p_all <= 1, "top_p must lie in (0, 1]"
+    assert s.min_p or 0 <= s.min_p_all <= 1, "min_p must lie in [0, 1]"
+    backend = get_backend()
+    _require_cuda(backend, rows, u)
+    tokens = torch.empty(n, dtype=torch.int64, device=dev)
+    logprobs = torch.empty(n, dtype=torch.float32, device=dev)
+    with _device_guard(rows):
+        backend.sample_logits(rows, s, tokens, logprobs)
+    lead = logits.shape[:-1]
+    return Sampled(tokens.view(lead), logprobs.view(lead))

@@ -185,6 +185,24 @@ class NativeBackend:
             "lce_grad_scale_cast",
         )
 
+    def top_logits(self, logits, k, temperature, values, indices, lse):
+        _native.check(
+            self.lib.lce_top_logits(
+                _DTYPE_CODE[logits.dtype], _ptr(logits), logits.stride(0), logits.shape[0], logits.shape[1], k,
+                temperature, _ptr(values), _ptr(indices), _ptr(lse), self._stream(logits),
+            ),
+            "lce_top_logits",
+        )
+
+    def sample_logits(self, logits, sampling, tokens, logprobs):
+        _native.check(
+            self.lib.lce_sample_logits(
+                _DTYPE_CODE[logits.dtype], _ptr(logits), logits.stride(0), logits.shape[0], logits.shape[1],
+                ctypes.byref(sampling), _ptr(tokens), _ptr(logprobs), self._stream(logits),
+            ),
+            "lce_sample_logits",
+        )
+
     def rerun_stats_async(self, workspace, host_int32x2) -> None:
         _native.check(self.lib.lce_rerun_stats_async(_ptr(workspace), host_int32x2.data_ptr(),
                                                      self._stream(workspace)), "lce_rerun_stats_async")

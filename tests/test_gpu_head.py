@@ -1,0 +1,299 @@
+"""top_logits and sample_logits against their definitions in 64 bits. Indices and tokens have to be equal."""
+import numpy as np
+import pytest
+import torch
+
+from head_util import sample_reference, top_reference
+from linear_cross_entropy_loss_b200 import sample_logits, top_logits
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+INF, NAN = float("inf"), float("nan")
+
+
+def normal(n, V, dtype, seed=0, std=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (std * torch.randn(n, V, generator=g)).to(dtype)
+
+
+# Row sums run over V terms of relative error (|d| + 3) 2^-23 each (the exponential and its argument; the terms weigh
+# exp(d), so |d| counts 1/e at most), added in fewer than 64 + log2 steps of 2^-24; the logarithm turns the relative error of
+# the sum into an absolute one, and max / T + log(sum) and 1 / T are rounded once each.
+def lse_tolerance(lse, largest, T):
+    return 2.0 ** -17 + 2.0 ** -22 * (abs(lse) + abs(largest / T))
+
+
+def check_top(logits, k, T=1.0):
+    got = top_logits(logits, k, temperature=T)
+    flat = logits.reshape(-1, logits.shape[-1])
+    host = flat.double().cpu().numpy()
+    indices, lse = top_reference(host, k, T)
+    assert got.values.shape == (*logits.shape[:-1], k) and got.values.dtype == logits.dtype
+    assert got.indices.shape == (*logits.shape[:-1], k) and got.indices.dtype == torch.int64
+    assert got.lse.shape == logits.shape[:-1] and got.lse.dtype == torch.float32
+    assert np.array_equal(got.indices.reshape(-1, k).cpu().numpy(), indices)
+    values = got.values.reshape(-1, k).double().cpu().numpy()
+    want = np.take_along_axis(host, indices, 1)
+    assert np.array_equal(values, want, equal_nan=True)
+    for r, (a, b) in enumerate(zip(got.lse.reshape(-1).double().cpu().numpy(), lse)):
+        if np.isfinite(b):
+            assert abs(a - b) <= lse_tolerance(b, host[r].max(), T), (r, a, b)
+        else:
+            assert a == b or (np.isnan(a) and np.isnan(b)), (r, a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(1, 1), (2, 1), (2, 2), (7, 3), (31, 31), (33, 8), (256, 64), (1000, 1000), (1025, 1024),
+                                 (4099, 100), (8192, 1), (20000, 513), (50257, 64), (131072, 50), (262147, 128)])
+def test_top_logits(dtype, V, k):
+    check_top(normal(5, V, dtype, seed=V + k).cuda(), k)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 64, 149, 700])
+def test_top_logits_row_counts(n):
+    check_top(normal(n, 3001, torch.bfloat16, seed=n).cuda(), 20, T=0.7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 5000, 70001])
+def test_top_logits_orders(dtype, V):
+    up = torch.linspace(-8, 8, V).to(dtype)
+    few = torch.randint(0, 3, (V,), generator=torch.Generator().manual_seed(V)).to(dtype)
+    zeros = torch.zeros(V, dtype=dtype)
+    zeros[1::2] = -0.0
+    last = torch.zeros(V, dtype=dtype)
+    last[-1] = 1.0
+    lowest = torch.full((V,), torch.finfo(dtype).min, dtype=dtype)
+    lowest[V // 2] = 0.5
+    rows = torch.stack([up, up.flip(0), few, zeros, last, lowest, torch.full((V,), 2.0, dtype=dtype)])
+    check_top(rows.cuda(), 33)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [50, 9001])
+def test_top_logits_infinities_and_nan(dtype, V):
+    rows = normal(7, V, dtype, seed=3)
+    rows[0] = -INF
+    rows[1, :] = -INF
+    rows[1, [3, V - 1]] = torch.tensor([1.0, 2.0], dtype=dtype)
+    rows[2, [0, V - 2]] = INF
+    rows[3, [5, 6, V - 1]] = NAN
+    rows[4, 7] = NAN
+    rows[4, 8] = INF
+    rows[4, 9] = -INF
+    rows[5] = NAN
+    rows[6] = INF
+    check_top(rows.cuda(), 20)
+
+
+def test_top_logits_layouts():
+    base = normal(24, 1200, torch.bfloat16).cuda()
+    check_top(base[:, 1:-2], 17)                       # rows off the 16-byte grid
+    check_top(base[::3, 5:1000], 17)
+    check_top(base.view(2, 3, 4, 1200), 9)
+    check_top(base.t().contiguous().t(), 9)             # inner stride 24
+    check_top(base[:1].expand(6, 1200), 9)              # one row, six times
+    check_top(base[3], 9)
+    empty = top_logits(base[:0], 4)
+    assert empty.values.shape == (0, 4) and empty.indices.shape == (0, 4) and empty.lse.shape == (0,)
+    f32 = normal(9, 1501, torch.float32).cuda()
+    check_top(f32[:, 3:], 100)
+    check_top(f32[:, :1], 1)
+
+
+# ---------------------------------------------------------------------------------------------------- sampling
+# The logarithm is taken in 64 bits of weights that are rounded to 2^-45 of the largest one, then rounded to float32.
+def check_sample(logits, u, T=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    got = sample_logits(logits, u, temperature=T, top_k=top_k, top_p=top_p, min_p=min_p)
+    assert got.tokens.shape == logits.shape[:-1] and got.tokens.dtype == torch.int64
+    assert got.logprobs.shape == logits.shape[:-1] and got.logprobs.dtype == torch.float32
+    host = logits.reshape(-1, logits.shape[-1]).double().cpu().numpy()
+    uu = u.reshape(-1).double().cpu().numpy()
+
+    def of(v, r):
+        return float(v.reshape(-1)[r if v.numel() > 1 else 0]) if isinstance(v, torch.Tensor) else v
+
+    want = [sample_reference(host[r], uu[r], of(T, r), int(of(top_k, r)), of(top_p, r), of(min_p, r)) for r in range(len(host))]
+    assert got.tokens.reshape(-1).tolist() == [w[0] for w in want]
+    lp = got.logprobs.reshape(-1).double().cpu().numpy()
+    for a, (_, b) in zip(lp, want):
+        assert a == b or abs(a - b) <= 2.0 ** -24 * abs(b) + 1e-8, (a, b)
+    return got
+
+
+def uniform(n, seed=0, dtype=torch.float32):
+    return torch.rand(n, generator=torch.Generator().manual_seed(1000 + seed), dtype=dtype).cuda()
+
+
+SETTINGS = [dict(), dict(T=0.6), dict(T=2.5), dict(top_k=1), dict(top_k=5), dict(top_k=50, T=0.8), dict(top_p=0.9),
+            dict(top_p=0.3, T=1.5), dict(min_p=0.05), dict(min_p=1.0), dict(top_k=40, top_p=0.8), dict(top_k=300, top_p=0.95, min_p=0.01),
+            dict(top_k=3000, top_p=0.7), dict(top_p=0.999, min_p=0.002), dict(T=0.0), dict(top_k=10**6), dict(top_p=1e-6),
+            dict(T=1e-6), dict(T=1e4, top_p=0.5)]
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 5000), (torch.bfloat16, 32768), (torch.float16, 50257)])
+def test_sample_logits(dtype, V, settings):
+    check_sample(normal(7, V, dtype, seed=V).cuda(), uniform(7, V), **settings)
+
+
+@pytest.mark.parametrize("V", [1, 2, 3, 31, 32, 33, 257, 1023, 8193, 131072, 300001])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.9)], ids=str)
+def test_sample_logits_vocabularies(V, settings):
+    check_sample(normal(3, V, torch.bfloat16, seed=V).cuda(), uniform(3, V), **settings)
+    check_sample(normal(2, V, torch.float32, seed=V).cuda(), uniform(2, V + 1), **settings)
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 63, 150, 600])
+def test_sample_logits_row_counts(n):
+    check_sample(normal(n, 2000, torch.bfloat16, seed=n).cuda(), uniform(n, n), top_k=50, top_p=0.9)
+    check_sample(normal(n, 2000, torch.float16, seed=n).cuda(), uniform(n, n), top_p=0.9)
+
+
+def test_sample_logits_settings_per_row():
+    n, V = 96, 6000
+    g = torch.Generator().manual_seed(5)
+    logits = normal(n, V, torch.bfloat16, seed=9)
+    logits[::4, ::2] = -INF
+    T = torch.where(torch.rand(n, generator=g) < 0.2, torch.zeros(n), 0.3 + torch.rand(n, generator=g)).cuda()
+    top_k = torch.randint(-1, 2500, (n,), generator=g).cuda()
+    top_k[::5] = 0
+    top_p = torch.rand(n, generator=g).cuda()
+    top_p[::3] = 1.0
+    min_p = (0.2 * torch.rand(n, generator=g)).cuda()
+    min_p[1::3] = 0.0
+    u = uniform(n)
+    check_sample(logits.cuda(), u, T, top_k, top_p, min_p)
+    check_sample(logits.cuda(), u, T, top_k.to(torch.int32), 0.9, min_p)
+    check_sample(logits.cuda(), u, T[:1], top_k, top_p, 0.0)
+    check_sample(logits.cuda().view(8, 12, V), u.view(8, 12), T, top_k, top_p, min_p)
+
+
+def test_sample_logits_takes_settings_out_of_range_as_the_nearest():
+    logits, u = normal(6, 300, torch.float32).cuda(), uniform(6)
+    same = sample_logits(logits, u)
+    off = sample_logits(logits, u, top_p=torch.tensor([1.5, NAN, 2.0, 1.0, INF, 1.1]).cuda(),
+                        min_p=torch.tensor([-1.0, NAN, 0.0, -INF, -0.5, 0.0]).cuda(),
+                        top_k=torch.tensor([-5, 0, -1, 300, 10**9, 301]).cuda())
+    assert torch.equal(same.tokens, off.tokens)
+    first = logits.argmax(1)
+    assert torch.equal(sample_logits(logits, u, temperature=torch.tensor([0.0, -1.0, NAN, 0.0, -INF, 0.0]).cuda()).tokens, first)
+    assert torch.equal(sample_logits(logits, u, top_p=torch.zeros(6).cuda() - 1).tokens, first)
+    assert torch.equal(sample_logits(logits, u, min_p=torch.full((6,), 3.0).cuda()).tokens, first)
+    lo = sample_logits(logits, torch.zeros(6).cuda()).tokens
+    hi = sample_logits(logits, torch.full((6,), 1 - 2.0 ** -24).cuda()).tokens
+    assert torch.equal(sample_logits(logits, torch.tensor([-1.0, NAN, -INF, 0.0, -0.0, -3.0]).cuda()).tokens, lo)
+    assert torch.equal(sample_logits(logits, torch.tensor([1.0, 2.0, INF, 1.0, 7.0, 1.0]).cuda()).tokens, hi)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_logits_ties(dtype):
+    """Equal logits everywhere: counts and masses end inside a run of equal values."""
+    V = 40000
+    flat = torch.zeros(5, V, dtype=dtype)
+    flat[1, 1::2] = -0.0
+    flat[2] = torch.randint(0, 3, (V,), generator=torch.Generator().manual_seed(1)).to(dtype)
+    flat[3] = torch.finfo(dtype).min
+    flat[3, 100:30000] = 1.0
+    flat[4] = -7.5
+    flat = flat.cuda()
+    for settings in [dict(), dict(top_k=100), dict(top_k=12345), dict(top_p=0.37), dict(top_k=2000, top_p=0.5),
+                     dict(top_k=20000, top_p=0.5), dict(top_p=0.9, min_p=0.5, T=1e3)]:
+        check_sample(flat, uniform(5), **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=7), dict(top_p=0.8), dict(min_p=0.3), dict(T=0.0), dict(top_k=2000, top_p=0.6)], ids=str)
+def test_sample_logits_masks_infinities_and_nan(dtype, settings):
+    V = 3000
+    rows = normal(8, V, dtype, seed=4)
+    rows[0] = -INF
+    rows[1] = NAN
+    rows[2] = -INF
+    rows[2, V - 1] = -3.0
+    rows[3, [4, 77, 2999]] = INF
+    rows[4, ::3] = NAN
+    rows[5, 10:] = torch.finfo(dtype).min
+    rows[6, :2999] = -INF
+    rows[6, 5] = NAN
+    rows[7] = torch.finfo(dtype).min
+    check_sample(rows.cuda(), uniform(8), **settings)
+
+
+def test_sample_logits_borders():
+    """u on the borders between tokens of equal weight: the token above the border is drawn."""
+    logits = torch.zeros(9, 8).cuda()
+    u = torch.tensor([0, 1 / 8, 2 / 8, 3 / 8, 4 / 8, 5 / 8, 6 / 8, 7 / 8, 1 - 2.0 ** -53], dtype=torch.float64).cuda()
+    assert sample_logits(logits, u).tokens.tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 7]
+    # one token outweighs the rest by more than the weights resolve
+    logits = torch.full((1, 64), -60.0).cuda()
+    logits[0, 20] = 0.0
+    for v in (0.0, 0.5, 1 - 2.0 ** -24):
+        assert sample_logits(logits, torch.tensor([v]).cuda()).tokens.item() == 20
+
+
+def test_sample_logits_layouts():
+    base = normal(24, 1200, torch.bfloat16).cuda()
+    for settings in (dict(top_k=30, top_p=0.9), dict(top_p=0.9)):
+        check_sample(base[:, 1:-2], uniform(24), **settings)
+        check_sample(base[::3, 5:1000], uniform(8), **settings)
+        check_sample(base.t().contiguous().t(), uniform(24), **settings)
+        check_sample(base[:1].expand(6, 1200), uniform(12)[::2], **settings)
+        check_sample(base[2], uniform(1).view(()), **settings)
+        check_sample(base.view(4, 6, 1200), uniform(24, dtype=torch.float64).view(4, 6), **settings)
+    none = sample_logits(base[:0], uniform(24)[:0])
+    assert none.tokens.shape == (0,) and none.logprobs.shape == (0,)
+
+
+def test_sample_logits_draws_the_distribution():
+    """Tokens of a grid of random numbers: their shares are the probabilities, to one grid step each."""
+    n = 4096
+    row = normal(1, 200, torch.float32, std=1.0)
+    p = torch.softmax(row[0].double(), 0)
+    u = ((torch.arange(n, dtype=torch.float64) + 0.5) / n).cuda()
+    tokens = sample_logits(row.expand(n, 200).cuda(), u).tokens.cpu()
+    counts = torch.bincount(tokens, minlength=200).double()
+    assert (counts - n * p).abs().max() <= 1.0
+
+
+@pytest.mark.parametrize("what", ["top", "sample", "nucleus"])
+def test_other_streams_and_captured_graphs(what):
+    logits, u = normal(40, 5001, torch.bfloat16).cuda(), uniform(40)
+    call = {"top": lambda: top_logits(logits, 30), "sample": lambda: sample_logits(logits, u, top_k=30, top_p=0.9),
+            "nucleus": lambda: sample_logits(logits, u, top_p=0.9)}[what]
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    old = logits.clone()
+    logits.copy_(normal(40, 5001, torch.bfloat16, seed=8).cuda())
+    graph.replay()
+    torch.cuda.synchronize()
+    new = call()
+    assert all(torch.equal(a, b) for a, b in zip(got, new))
+    logits.copy_(old)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_side_by_side_on_two_streams():
+    a, b = normal(64, 20000, torch.float32, seed=1).cuda(), normal(64, 20000, torch.float32, seed=2).cuda()
+    u = uniform(64)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((*top_logits(x, 100), *sample_logits(x, u, top_p=0.9), *sample_logits(x, u, top_k=50)))
+    torch.cuda.synchronize()
+    for runs in got:
+        for run in runs[1:]:
+            assert all(torch.equal(p, q) for p, q in zip(run, runs[0]))
