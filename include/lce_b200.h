@@ -282,6 +282,35 @@ int lce_read_status(void* workspace, void* stream);
 int lce_eval_loss_static(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
                          const int64_t* labels, float* out5, void* stream);
 
+/* ---- distillation from a teacher's top logits --------------------------------------------------
+ * No counterpart in the reference. One pass of
+ *     z = logit_scale * (x @ W)
+ *     q_ik = softmax over the row's entries of teacher logit / T   (or exp(teacher logit / T - lse_i), lse given)
+ *     loss = T^2 / n * sum_i sum_k q_ik (log q_ik - z[i, idx_ik] / T + logsumexp_j(z_ij / T))
+ * with both gradients, over the same chunks, slab and contractions as lce_fused_pass.
+ * An entry whose index lies outside [0, vocab) is not there, whatever its logit; one with logit -inf has no weight. Rows
+ * without weight do not count (n = rows that do; none: the loss is NaN). NaN or +inf in an entry that is there makes
+ * the loss NaN. The same index twice in a row: both count.
+ * p: as for lce_fused_pass; ignore_index is not used; z_regularization and monitoring must be 0, chunk_buffers 0 or 1.
+ * workspace: lce_distill_workspace_bytes() bytes. dx (element type of x), dweight, dweight_residual: as for lce_fused_pass.
+ * loss: one float. Nothing synchronises, nothing is allocated. */
+#define LCE_TEACHER_MAX 1024
+typedef struct lce_teacher {
+  const void* logits;   /* [n_rows_total, k], rows logits_ld elements apart */
+  const void* indices;  /* [n_rows_total, k], rows indices_ld elements apart */
+  const float* lse;     /* [n_rows_total] logsumexp of ALL teacher logits / T, or null: the listed ones are everything */
+  int64_t logits_ld;
+  int64_t indices_ld;
+  int32_t k;            /* 1 .. LCE_TEACHER_MAX */
+  int32_t logits_dtype; /* LCE_DTYPE_* */
+  int32_t indices_bits; /* 32 or 64 */
+  float temperature;    /* T > 0 */
+} lce_teacher;
+int lce_distill_workspace_bytes(const lce_problem* p, int32_t k, size_t* bytes);
+int lce_distill_pass(const lce_problem* p, const lce_teacher* teacher, const void* x, int64_t x_ld,
+                     const void* weight, int64_t w_ld, void* workspace, void* dx, int64_t dx_ld, void* dweight,
+                     int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, float* loss, void* stream);
+
 /* ---- operators on given logits ------------------------------------------------------------------
  * No counterpart in the reference. They need no workspace; logits: [rows, vocab] device memory of element type dtype, rows
  * ld elements apart (ld >= 0, any alignment of the element type).

@@ -2,7 +2,7 @@
 
 Same public names as ``linear_cross_entropy`` (the reference package, __init__.py:1):
 ``LinearCrossEntropyLoss``, ``linear_cross_entropy``, ``fwd_configs``, ``bwd_configs``. Beside them, on the same heads:
-``top_logits`` and ``sample_logits``.
+``LinearDistillationLoss``, ``linear_distillation``, ``top_logits`` and ``sample_logits``.
 """
 from .ops import (  # noqa: F401
     LinearCrossEntropyLoss,
@@ -13,7 +13,8 @@ from .ops import (  # noqa: F401
     set_autocast_policy,
 )
 
+from .distill import LinearDistillationLoss, linear_distillation  # noqa: F401
 from .head import Sampled, TopLogits, sample_logits, top_logits  # noqa: F401
 
 __all__ = ["LinearCrossEntropyLoss", "linear_cross_entropy", "fwd_configs", "bwd_configs", "set_autocast_policy",
-           "top_logits", "TopLogits", "sample_logits", "Sampled"]
+           "LinearDistillationLoss", "linear_distillation", "top_logits", "TopLogits", "sample_logits", "Sampled"]

@@ -135,6 +135,25 @@ class PeerTable(ctypes.Structure):
     _fields_ = [("world", ctypes.c_int32), ("rank", ctypes.c_int32), ("base", ctypes.c_void_p * MAX_PEERS)]
 
 
+class Teacher(ctypes.Structure):
+    """Mirror of ``lce_teacher``: a teacher's top logits for every row."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("indices", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("logits_ld", ctypes.c_int64),
+        ("indices_ld", ctypes.c_int64),
+        ("k", ctypes.c_int32),
+        ("logits_dtype", ctypes.c_int32),
+        ("indices_bits", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+    ]
+
+
+TEACHER_MAX = 1024
+
+
 class Sampling(ctypes.Structure):
     """Mirror of ``lce_sampling``: each setting one value for all rows, or a device pointer to one per row."""
 
@@ -195,6 +214,12 @@ SIGNATURES = {
     "lce_read_status": (ctypes.c_int, [_vp, _vp]),
     "lce_rerun_stats_async": (ctypes.c_int, [_vp, _vp, _vp]),
     "lce_eval_loss_static": (ctypes.c_int, [ctypes.POINTER(Problem), _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "lce_distill_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(Problem), _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "lce_distill_pass": (
+        ctypes.c_int,
+        [ctypes.POINTER(Problem), ctypes.POINTER(Teacher), _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64,
+         _vp, _vp],
+    ),
     "lce_top_logits": (
         ctypes.c_int, [_i32, _vp, _i64, _i64, _i64, _i32, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "lce_sample_logits": (

@@ -113,6 +113,34 @@ __device__ __forceinline__ void lse_merge(float& m, float& s, float& u, float m2
   }
 }
 
+// A teacher's lists for the rows of a call (distillation): row r has n = start[n_tiles * start_ld + r] entries, columns
+// idx[r * k + e] in ascending order with weights q and student logits z. All null for the cross-entropy loss.
+struct TeacherRows {
+  const int* idx;
+  const float* q;
+  const float* z;
+  const float* plogp;  // [rows] sum_e q log q before equal columns were merged
+  const unsigned short* start;
+  long long start_ld;
+  int k;
+  int n_tiles;
+};
+
+// What takes the place of the label's logit: sum_e q z - sum_e q log q, for the block's 32 rows r0 + 0 .. 31 (8 warps, four rows
+// each; dots is complete after the caller's next __syncthreads).
+__device__ __forceinline__ void listed_dots(const TeacherRows& t, int r0, int rows, float* dots /*[32]*/) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = 4 * warp; i < 4 * warp + 4; ++i) {
+    const int r = r0 + i;
+    if (r >= rows) break;
+    const int n = t.start[(long long)t.n_tiles * t.start_ld + r];
+    float d = 0.f;
+    for (int e = lane; e < n; e += 32) d = fmaf(t.q[(long long)r * t.k + e], t.z[(long long)r * t.k + e], d);
+    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (lane == 0) dots[i] = d - t.plogp[r];
+  }
+}
+
 // Block = 32 rows x 8 warps; warp w walks V tiles w, w+8, ...; lane = row. Per-tile statistics are
 // stored [tile][row], so each warp load is 128 contiguous bytes.
 // parts layout: [ROW_PARTS][stat_ld].
@@ -122,8 +150,9 @@ row_stats_kernel(const float* __restrict__ tile_max, const float* __restrict__ t
                  const float* __restrict__ tile_ez, const float* __restrict__ tile_sq,
                  const float* __restrict__ target_logit, const long long* __restrict__ labels, int rows,
                  int n_tiles, long long stat_ld, long long ignore_index, long long vocab_offset,
-                 long long vocab_local, float* __restrict__ parts) {
+                 long long vocab_local, const TeacherRows teacher, float* __restrict__ parts) {
   __shared__ float sm[8][4][32];
+  __shared__ float dots[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f, u = 0.f, q = 0.f;
@@ -140,6 +169,7 @@ row_stats_kernel(const float* __restrict__ tile_max, const float* __restrict__ t
   sm[warp][1][lane] = s;
   sm[warp][2][lane] = u;
   sm[warp][3][lane] = q;
+  if (teacher.idx != nullptr) listed_dots(teacher, blockIdx.x * 32, rows, dots);
   __syncthreads();
   if (warp == 0 && r < rows) {
     for (int w = 1; w < 8; ++w) {
@@ -151,7 +181,7 @@ row_stats_kernel(const float* __restrict__ tile_max, const float* __restrict__ t
     const bool own = (yv != ignore_index) && yl >= 0 && yl < vocab_local;
     parts[0 * stat_ld + r] = m;
     parts[1 * stat_ld + r] = s;
-    parts[2 * stat_ld + r] = own ? target_logit[r] : 0.f;
+    parts[2 * stat_ld + r] = teacher.idx != nullptr ? dots[lane] : (own ? target_logit[r] : 0.f);
     parts[3 * stat_ld + r] = u;
     parts[4 * stat_ld + r] = q;
     parts[5 * stat_ld + r] = m;
@@ -171,11 +201,12 @@ row_stats_rowref_kernel(const float* __restrict__ tile_max, const float* __restr
                         int n_tiles, long long stat_ld, long long ignore_index, long long vocab_offset,
                         long long vocab_local, const float* row_ref_in, float* row_ref_out, float* row_base_out,
                         int* rescue, int* rescue_groups, int group_row0, const int* run_if,
-                        float* __restrict__ parts) {
+                        const TeacherRows teacher, float* __restrict__ parts) {
   // rescue_groups[g]: set when a row of the 256-row group g (rows counted from -group_row0) needs the re-run.
   // In the re-run itself (run_if given) only the flagged groups were recomputed, so only they are re-read.
   if (run_if != nullptr && (*run_if == 0 || rescue_groups[(group_row0 + blockIdx.x * 32) >> 8] == 0)) return;
   __shared__ float sm[8][4][32];
+  __shared__ float dots[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f, u = 0.f, q = 0.f;
@@ -194,6 +225,7 @@ row_stats_rowref_kernel(const float* __restrict__ tile_max, const float* __restr
   sm[warp][1][lane] = s;
   sm[warp][2][lane] = u;
   sm[warp][3][lane] = q;
+  if (teacher.idx != nullptr) listed_dots(teacher, blockIdx.x * 32, rows, dots);
   __syncthreads();
   if (warp == 0 && r < rows) {
     for (int w = 1; w < 8; ++w) {
@@ -208,7 +240,7 @@ row_stats_rowref_kernel(const float* __restrict__ tile_max, const float* __restr
     const bool own = (yv != ignore_index) && yl >= 0 && yl < vocab_local;
     parts[0 * stat_ld + r] = ref;
     parts[1 * stat_ld + r] = s;
-    parts[2 * stat_ld + r] = own ? target_logit[r] : 0.f;
+    parts[2 * stat_ld + r] = teacher.idx != nullptr ? dots[lane] : (own ? target_logit[r] : 0.f);
     parts[3 * stat_ld + r] = u;
     parts[4 * stat_ld + r] = q;
     parts[5 * stat_ld + r] = m;
@@ -242,11 +274,12 @@ __device__ __forceinline__ float ld_coherent(const float* p) {
 
 // Body of the combine step, for one block of 1024 threads per chunk. parts_all: [world][ROW_PARTS][stat_ld].
 // rescue_groups: n_groups ints of this chunk's buffers; the last one is the chunk's "any group flagged" word.
+// row_mass: distillation, the sum of the row's teacher weights (null: 1, a label).
 template <bool kCoherent>
 __device__ __forceinline__ void combine_rows(const float* parts_all, int world, const long long* __restrict__ labels,
                                              int rows, long long stat_ld, long long ignore_index, int monitoring,
                                              float* __restrict__ lse_out, PassScalars* sc, int* rescue_groups,
-                                             int n_groups) {
+                                             int n_groups, const float* row_mass = nullptr) {
   __shared__ double scratch_d[32];
   __shared__ float scratch_f[32];
   double a_nll = 0.0, a_lse2 = 0.0, a_ent = 0.0, a_norm = 0.0;
@@ -265,7 +298,7 @@ __device__ __forceinline__ void combine_rows(const float* parts_all, int world, 
     lse_out[r] = lse;
     const bool valid = labels[r] != ignore_index;
     if (valid) {
-      a_nll += (double)lse - (double)t;
+      a_nll += (row_mass != nullptr ? (double)row_mass[r] * (double)lse : (double)lse) - (double)t;
       a_lse2 += (double)lse * (double)lse;
       if (monitoring) a_ent += (double)lse - (double)u / (double)s;
     }
@@ -298,9 +331,9 @@ __device__ __forceinline__ void combine_rows(const float* parts_all, int world, 
 __global__ void __launch_bounds__(1024)
 combine_kernel(const float* __restrict__ parts_all, int world, const long long* __restrict__ labels, int rows,
                long long stat_ld, long long ignore_index, int monitoring, float* __restrict__ lse_out,
-               PassScalars* sc, int* rescue_groups, int n_groups) {
+               PassScalars* sc, int* rescue_groups, int n_groups, const float* __restrict__ row_mass) {
   combine_rows<false>(parts_all, world, labels, rows, stat_ld, ignore_index, monitoring, lse_out, sc, rescue_groups,
-                      n_groups);
+                      n_groups, row_mass);
 }
 
 __global__ void finalize_kernel(const PassScalars* sc, double n_rows_total, float z_regularization,

@@ -115,6 +115,13 @@ struct GemmParams {
   long long vocab_offset;      // global class id of local column 0
   float scale;                 // logit scale (> 0)
   const float* row_ref;        // [rows] row-reference mode: slab = exp(z - row_ref[i]); null = reference 0
+  // lists of columns whose logits are wanted (distillation; list_idx null = none): row i has the ascending columns
+  // list_idx[i * list_k + e]; those of tile t are e = list_start[t * list_start_ld + i] up to the same of tile t + 1
+  const int* list_idx;
+  const unsigned short* list_start;
+  float* list_z;               // out: z[i, list_idx[i][e]]
+  long long list_start_ld;
+  int list_k;
 
   // ---- EPI_F32: optional per-output-row factor (dx in row-reference mode: exp(ref - lse) (1 + 2 z_reg lse))
   const float* row_coef;
@@ -356,6 +363,31 @@ __device__ __forceinline__ void slab_chunk_via_tma(const GemmParams& p, const CU
   if (!kHalves || (c & 1) == 1) stage.commit(tmC, buf, lane, col0 + (kHalves ? (c - 1) : c) * 32, row0);
 }
 
+// The logits at the listed columns of this tile. A thread cannot index its registers by a column that differs from row
+// to row, but the accumulator is still in tensor memory: the warp walks the columns that any of its 32 rows lists, loads each once for all
+// rows, and the rows that list it keep it. 32 rows with 64 listed columns of 131072 have 4 such columns in a tile.
+__device__ __forceinline__ void gather_listed(const GemmParams& p, uint32_t taddr, int n_blk, long long r, bool row_ok) {
+  int at = 0, end = 0;
+  if (row_ok) {
+    at = p.list_start[(long long)n_blk * p.list_start_ld + r];
+    end = p.list_start[(long long)(n_blk + 1) * p.list_start_ld + r];
+  }
+  const int* idx = p.list_idx + r * p.list_k;
+  const int col0 = n_blk * BLOCK_N;
+  int next = at < end ? idx[at] - col0 : BLOCK_N;
+  for (;;) {
+    const int col = __reduce_min_sync(0xffffffffu, next);
+    if (col >= BLOCK_N) break;
+    const uint32_t v = tmem_ld_32x32b_x1(taddr + col);
+    tmem_ld_wait();
+    if (next == col) {
+      p.list_z[r * p.list_k + at] = __uint_as_float(v) * p.scale;
+      ++at;
+      next = at < end ? idx[at] - col0 : BLOCK_N;
+    }
+  }
+}
+
 // Forward epilogue. For its row i and this tile's 256 columns j (z = scale * acc):
 //   tile_max = max_j z,  tile_sum = sum_j exp(z - tile_max),  slab[i, j] = exp(z - tile_max)
 //   target_logit[i] = z[i, y_i] if column y_i lies in this tile
@@ -434,6 +466,7 @@ __device__ __forceinline__ void epilogue_forward_tilemax(const GemmParams& p, co
     }
     if (ycol >= 0) p.target_logit[r] = tv * p.scale;
   }
+  if (p.list_idx != nullptr) gather_listed(p, taddr, n_blk, r, row_ok);
 }
 
 // Forward epilogue, row-reference mode (bf16 and fp32 slabs, whose exponent range is that of fp32): one pass.
@@ -520,6 +553,7 @@ __device__ __forceinline__ void epilogue_forward_rowref(const GemmParams& p, con
     }
     if (ycol >= 0) p.target_logit[r] = tv * p.scale;
   }
+  if (p.list_idx != nullptr) gather_listed(p, taddr, n_blk, r, row_ok);
 }
 
 // fp16 slabs are always normalised per tile; bf16 / fp32 slabs per row unless the launch asks for tiles.

@@ -3,6 +3,7 @@
 #include "launch.h"
 
 #include "aux_kernels.cuh"
+#include "distill.cuh"
 #include "gemm_sm100.cuh"
 #include "peer_exchange.cuh"
 
@@ -13,6 +14,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 namespace lce {
@@ -410,6 +412,15 @@ int check_chunk(const lce_problem* p, int64_t row0, int64_t rows) {
   return LCE_OK;
 }
 
+// What distillation adds to the steps of a pass; the cross-entropy entry points run the same steps without it.
+struct Distill {
+  TeacherRows lists;   // of the chunk's rows
+  float* list_z;
+  const float* mass;   // of the chunk's rows
+  float grad_scale;    // takes the place of logit_scale in the gradients
+  float boost;         // power of two that the slab holds dZ multiplied with (per-tile mode)
+};
+
 inline int grid_for(long long items, int per_block, int sms, int waves) {
   long long g = (items + per_block - 1) / per_block;
   const long long cap = (long long)sms * waves;
@@ -467,9 +478,13 @@ int lce_begin(const lce_problem* p, const int64_t* labels, void* workspace, void
   return check_launch();
 }
 
-int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
-                      const int64_t* labels, int64_t row0, int64_t rows, void* workspace, float* row_parts_local,
-                      void* stream) {
+}  // extern "C"
+
+namespace {
+
+int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
+                  const int64_t* labels, int64_t row0, int64_t rows, void* workspace, float* row_parts_local,
+                  void* stream, const Distill* distill) {
   int v = validate_problem(p);
   if (v != LCE_OK) return v;
   if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
@@ -523,6 +538,15 @@ int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const v
   gp.vocab_offset = p->vocab_offset;
   gp.scale = p->logit_scale;
   gp.status = &w.scalars->status;
+  TeacherRows teacher = {};
+  if (distill != nullptr) {
+    teacher = distill->lists;
+    gp.list_idx = teacher.idx;
+    gp.list_start = teacher.start;
+    gp.list_z = distill->list_z;
+    gp.list_start_ld = teacher.start_ld;
+    gp.list_k = teacher.k;
+  }
 
   const int blocks = (int)((rows + 31) / 32);
   const long long* lab = reinterpret_cast<const long long*>(labels) + row0;
@@ -541,11 +565,11 @@ int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const v
     if (p->monitoring)
       row_stats_kernel<true><<<blocks, 256, 0, st>>>(gp.tile_max, gp.tile_sum, gp.tile_ez, gp.tile_sq,
                                                      gp.target_logit, lab, (int)rows, gp.n_tiles, p->chunk_rows,
-                                                     p->ignore_index, p->vocab_offset, p->vocab_local, parts);
+                                                     p->ignore_index, p->vocab_offset, p->vocab_local, teacher, parts);
     else
       row_stats_kernel<false><<<blocks, 256, 0, st>>>(gp.tile_max, gp.tile_sum, gp.tile_ez, gp.tile_sq,
                                                       gp.target_logit, lab, (int)rows, gp.n_tiles, p->chunk_rows,
-                                                      p->ignore_index, p->vocab_offset, p->vocab_local, parts);
+                                                      p->ignore_index, p->vocab_offset, p->vocab_local, teacher, parts);
     return check_launch();
   }
 
@@ -562,6 +586,7 @@ int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const v
     GemmParams pp = gp;
     pp.n_tiles = kProbeTiles;
     pp.store_slab = 0;
+    pp.list_idx = nullptr;
     if ((v = launch_gemm_dtype<false, true, EPI_FWD, false>(p->dtype, ta, tb, tc, pp, sms, st, pair)) != LCE_OK) return v;
     probe_ref_kernel<<<(int)((rows + 255) / 256), 256, 0, st>>>(gp.tile_max, p->chunk_rows, kProbeTiles, (int)rows,
                                                                w.row_ref + local0);
@@ -579,19 +604,19 @@ int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const v
       row_stats_rowref_kernel<true><<<blocks, 256, 0, st>>>(
           gp.tile_max, gp.tile_sum, gp.tile_ez, gp.tile_sq, gp.target_logit, lab, (int)rows, gp.n_tiles,
           p->chunk_rows, p->ignore_index, p->vocab_offset, p->vocab_local, ref_in, w.row_ref + local0,
-          w.row_base + local0, rescue, w.rescue_groups, (int)local0, run_if, parts);
+          w.row_base + local0, rescue, w.rescue_groups, (int)local0, run_if, teacher, parts);
     else
       row_stats_rowref_kernel<false><<<blocks, 256, 0, st>>>(
           gp.tile_max, gp.tile_sum, gp.tile_ez, gp.tile_sq, gp.target_logit, lab, (int)rows, gp.n_tiles,
           p->chunk_rows, p->ignore_index, p->vocab_offset, p->vocab_local, ref_in, w.row_ref + local0,
-          w.row_base + local0, rescue, w.rescue_groups, (int)local0, run_if, parts);
+          w.row_base + local0, rescue, w.rescue_groups, (int)local0, run_if, teacher, parts);
     if ((v = check_launch()) != LCE_OK) return v;
   }
   return LCE_OK;
 }
 
-int lce_combine_chunk(const lce_problem* p, const float* row_parts_all, const int64_t* labels, int64_t row0,
-                      int64_t rows, void* workspace, void* stream) {
+int combine_chunk(const lce_problem* p, const float* row_parts_all, const int64_t* labels, int64_t row0, int64_t rows,
+                  void* workspace, void* stream, const Distill* distill) {
   int v = validate_problem(p);
   if (v != LCE_OK) return v;
   if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
@@ -603,8 +628,24 @@ int lce_combine_chunk(const lce_problem* p, const float* row_parts_all, const in
   combine_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_parts_all + local0, p->world,
                                                        reinterpret_cast<const long long*>(labels) + row0, (int)rows,
                                                        p->chunk_rows, p->ignore_index, p->monitoring, w.lse + local0,
-                                                       w.scalars, w.rescue_groups, w.n_rescue);
+                                                       w.scalars, w.rescue_groups, w.n_rescue,
+                                                       distill != nullptr ? distill->mass : nullptr);
   return check_launch();
+}
+
+}  // namespace
+
+extern "C" {
+
+int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
+                      const int64_t* labels, int64_t row0, int64_t rows, void* workspace, float* row_parts_local,
+                      void* stream) {
+  return forward_chunk(p, x, x_ld, weight, w_ld, labels, row0, rows, workspace, row_parts_local, stream, nullptr);
+}
+
+int lce_combine_chunk(const lce_problem* p, const float* row_parts_all, const int64_t* labels, int64_t row0,
+                      int64_t rows, void* workspace, void* stream) {
+  return combine_chunk(p, row_parts_all, labels, row0, rows, workspace, stream, nullptr);
 }
 
 int lce_parts_bytes(const lce_problem* p, size_t* bytes) {
@@ -771,8 +812,8 @@ PeerBases bases_of(const lce_peer_table* peers) {
 // direct_dx (optional, one split only): the rows of dx themselves, element type of x, row stride direct_ld; the
 // epilogue then writes them instead of fp32 partials.
 int launch_dx_gemm(const lce_problem* p, const void* weight, int64_t w_ld, int64_t row0, int64_t rows,
-                   const Workspace& w, int sms, cudaStream_t st, const PeerScatter* scatter, void* direct_dx = nullptr,
-                   int64_t direct_ld = 0) {
+                   const Workspace& w, int sms, cudaStream_t st, const PeerScatter* scatter, float grad_scale,
+                   void* direct_dx = nullptr, int64_t direct_ld = 0) {
   const int es = elem_size(p->dtype);
   const long long local0 = row0 % p->chunk_rows;
   const long long v_pad = vocab_pad(p), h_pad = hidden_pad(p);
@@ -801,7 +842,7 @@ int launch_dx_gemm(const lce_problem* p, const void* weight, int64_t w_ld, int64
   gp.out_cols = (int)h_pad;
   gp.out_vector_ok = 1;
   gp.accumulate = 0;
-  gp.out_scale = p->logit_scale;
+  gp.out_scale = grad_scale;
   gp.out_div = &w.scalars->n_valid;
   gp.row_coef = row_reference_mode(p) ? w.row_coef + local0 : nullptr;
   gp.status = &w.scalars->status;
@@ -838,12 +879,8 @@ int launch_dx_gemm(const lce_problem* p, const void* weight, int64_t w_ld, int64
 
 long long peer_wait_limit_ns(int32_t wait_ms) { return (long long)(wait_ms > 0 ? wait_ms : 10000) * 1000000LL; }
 
-}  // namespace
-
-extern "C" {
-
-int lce_dx_chunk(const lce_problem* p, const void* weight, int64_t w_ld, int64_t row0, int64_t rows, void* workspace,
-                 void* dx, int64_t dx_ld, int32_t dx_dtype, void* stream) {
+int dx_chunk(const lce_problem* p, const void* weight, int64_t w_ld, int64_t row0, int64_t rows, void* workspace,
+             void* dx, int64_t dx_ld, int32_t dx_dtype, void* stream, float grad_scale) {
   int v = validate_problem(p);
   if (v != LCE_OK) return v;
   if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
@@ -859,9 +896,9 @@ int lce_dx_chunk(const lce_problem* p, const void* weight, int64_t w_ld, int64_t
   const long long h_pad = hidden_pad(p);
   if (w.dx_splits == 1 && dx_dtype == p->dtype) {
     // one split: the contraction's epilogue scales, converts and stores the dx rows itself
-    return launch_dx_gemm(p, weight, w_ld, row0, rows, w, sms, st, nullptr, dx, dx_ld);
+    return launch_dx_gemm(p, weight, w_ld, row0, rows, w, sms, st, nullptr, grad_scale, dx, dx_ld);
   }
-  if ((v = launch_dx_gemm(p, weight, w_ld, row0, rows, w, sms, st, nullptr)) != LCE_OK) return v;
+  if ((v = launch_dx_gemm(p, weight, w_ld, row0, rows, w, sms, st, nullptr, grad_scale)) != LCE_OK) return v;
 
   // fixed-order sum of the partials -> dx rows
   const float* part = w.dx_part + local0 * h_pad;
@@ -883,6 +920,17 @@ int lce_dx_chunk(const lce_problem* p, const void* weight, int64_t w_ld, int64_t
                                                     reinterpret_cast<float*>(dx_rows), dx_ld);
   }
   return check_launch();
+}
+
+}  // namespace
+
+extern "C" {
+
+int lce_dx_chunk(const lce_problem* p, const void* weight, int64_t w_ld, int64_t row0, int64_t rows, void* workspace,
+                 void* dx, int64_t dx_ld, int32_t dx_dtype, void* stream) {
+  const int v = validate_problem(p);
+  if (v != LCE_OK) return v;
+  return dx_chunk(p, weight, w_ld, row0, rows, workspace, dx, dx_ld, dx_dtype, stream, p->logit_scale);
 }
 
 int lce_peer_bytes(const lce_problem* p, int32_t dx_dtype, size_t* bytes) {
@@ -917,7 +965,7 @@ int lce_dx_chunk_peer(const lce_problem* p, const void* weight, int64_t w_ld, in
   sc.world = peers->world;
   sc.rank = peers->rank;
   sc.buf = (int)(epoch & 1u);
-  if ((v = launch_dx_gemm(p, weight, w_ld, row0, rows, w, sms, st, &sc)) != LCE_OK) return v;
+  if ((v = launch_dx_gemm(p, weight, w_ld, row0, rows, w, sms, st, &sc, p->logit_scale)) != LCE_OK) return v;
   peer_signal_kernel<<<1, 32, 0, st>>>(sc.bases, sc.world, sc.rank, 0, epoch, nullptr);
   return check_launch();
 }
@@ -1017,9 +1065,13 @@ int lce_dx_finish_peer(const lce_problem* p, int64_t row0, int64_t rows, void* w
   return check_launch();
 }
 
-int lce_dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0, int64_t rows, void* workspace,
-                 void* dweight, int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, int32_t first, int32_t last,
-                 void* stream) {
+}  // extern "C"
+
+namespace {
+
+int dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0, int64_t rows, void* workspace,
+             void* dweight, int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, int32_t first, int32_t last,
+             void* stream, float grad_scale) {
   int v = validate_problem(p);
   if (v != LCE_OK) return v;
   if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
@@ -1070,7 +1122,7 @@ int lce_dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0
   gp.a_k0 = (int)(rowref ? local0 : row0);
   gp.b_k0 = (int)local0;
   gp.accumulate = first ? 0 : 1;
-  gp.out_scale = p->logit_scale;
+  gp.out_scale = grad_scale;
   gp.out_div = &w.scalars->n_valid;
   gp.status = &w.scalars->status;
   CUtensorMap tc = ta;
@@ -1096,6 +1148,19 @@ int lce_dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0
     v = launch_gemm_dtype<true, true, EPI_F32, false>(p->dtype, ta, tb, tc, gp, sms, st, pair);
   }
   return v;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lce_dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0, int64_t rows, void* workspace,
+                 void* dweight, int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, int32_t first, int32_t last,
+                 void* stream) {
+  const int v = validate_problem(p);
+  if (v != LCE_OK) return v;
+  return dw_chunk(p, x, x_ld, row0, rows, workspace, dweight, dw_ld, dweight_residual, dwr_ld, first, last, stream,
+                  p->logit_scale);
 }
 
 int lce_backward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
@@ -1300,6 +1365,191 @@ int lce_debug_gemm(int32_t dtype, int32_t a_mn_major, int32_t b_mn_major, const 
   if (a_mn_major && !b_mn_major)
     return launch_gemm_dtype<true, false, EPI_F32, false>(dtype, ta, tb, tc, gp, sms, st, pair);
   return launch_gemm_dtype<true, true, EPI_F32, false>(dtype, ta, tb, tc, gp, sms, st, pair);
+}
+
+}  // extern "C"
+
+// ================================================================================================
+// Distillation from a teacher's top logits (lce_distill_pass)
+// ================================================================================================
+namespace {
+
+struct DistillWorkspace {
+  Workspace pass;
+  long long* labels;   // [n_rows_total] -1: the row counts, kIgnoredRow: it does not
+  float* mass;         // [n_rows_total]
+  float* plogp;        // [n_rows_total]
+  float* row_parts;    // [ROW_PARTS * chunk_rows]
+  int* list_idx;       // [chunk_rows, k]
+  float* list_q;
+  float* list_z;
+  unsigned short* start;  // [n_tiles + 1, chunk_rows]
+  size_t total;
+};
+constexpr long long kIgnoredRow = -100;
+
+DistillWorkspace layout_distill(const lce_problem* p, int k, void* base, int sms) {
+  DistillWorkspace w;
+  w.pass = layout_workspace(p, base, sms);
+  char* b = reinterpret_cast<char*>(base);
+  size_t off = align_up(w.pass.total, 256);
+  auto take = [&](size_t bytes) {
+    char* ptr = b + off;
+    off += align_up(bytes, 256);
+    return ptr;
+  };
+  const size_t n = (size_t)p->n_rows_total, rows = (size_t)p->chunk_rows;
+  w.labels = reinterpret_cast<long long*>(take(n * sizeof(long long)));
+  w.mass = reinterpret_cast<float*>(take(n * sizeof(float)));
+  w.plogp = reinterpret_cast<float*>(take(n * sizeof(float)));
+  w.row_parts = reinterpret_cast<float*>(take(ROW_PARTS * rows * sizeof(float)));
+  w.list_idx = reinterpret_cast<int*>(take(rows * k * sizeof(int)));
+  w.list_q = reinterpret_cast<float*>(take(rows * k * sizeof(float)));
+  w.list_z = reinterpret_cast<float*>(take(rows * k * sizeof(float)));
+  w.start = reinterpret_cast<unsigned short*>(take((size_t)(vocab_pad(p) / BLOCK_N + 1) * rows * sizeof(unsigned short)));
+  w.total = off;
+  return w;
+}
+
+int validate_distill(const lce_problem* p, int k) {
+  const int v = validate_problem(p);
+  if (v != LCE_OK) return v;
+  if (p->world != 1 || p->vocab_offset != 0 || p->chunk_buffers > 1 || p->z_regularization != 0.f || p->monitoring)
+    return LCE_ERR_INVALID_ARGUMENT;
+  if (k < 1) return LCE_ERR_INVALID_ARGUMENT;
+  if (k > kTeacherMax) return LCE_ERR_TOO_LARGE;
+  return LCE_OK;
+}
+
+// Rows [row0, row0 + rows) of the teacher's lists; lists == false: only what decides which rows count.
+int launch_prepare(const lce_problem* p, const TeacherInput& in, const DistillWorkspace& w, int64_t row0, int64_t rows,
+                   bool lists, cudaStream_t st) {
+  int padded = 1;
+  while (padded < in.k) padded <<= 1;
+  int per_block = kPrepareEntries / padded;
+  if (per_block > 32) per_block = 32;
+  const int grid = (int)((rows + per_block - 1) / per_block);
+  const int n_tiles = (int)(vocab_pad(p) / BLOCK_N);
+  auto launch = [&](auto kernel) {
+    kernel<<<grid, kPrepareThreads, 0, st>>>(in, row0, (int)rows, p->vocab_local, per_block, padded, kIgnoredRow,
+                                             w.labels + row0, w.mass + row0, w.plogp + row0, w.list_idx, w.list_q,
+                                             w.start, p->chunk_rows, n_tiles);
+  };
+  if (lists) launch(teacher_prepare_kernel<true>);
+  else launch(teacher_prepare_kernel<false>);
+  return check_launch();
+}
+
+template <typename T>
+void launch_distill_dz(const lce_problem* p, const DistillWorkspace& w, const Distill& d, const void* x, int64_t x_ld,
+                       int64_t row0, int64_t rows, int sms, cudaStream_t st) {
+  const long long v_pad = vocab_pad(p), h_pad = hidden_pad(p), rows_pad = round_up(rows, BLOCK_M);
+  const int n_vtiles = (int)(v_pad / BLOCK_N);
+  T* slab = reinterpret_cast<T*>(w.pass.slab);
+  if constexpr (!std::is_same<T, __half>::value) {  // fp16 slabs are always per tile
+    if (row_reference_mode(p)) {
+      distill_finish_kernel<T><<<(int)rows_pad, 256, 0, st>>>(
+          reinterpret_cast<const T*>(x) + row0 * x_ld, x_ld, reinterpret_cast<T*>(w.pass.xs), h_pad, (int)p->hidden,
+          slab, v_pad, w.pass.row_base, w.pass.lse, d.mass, d.lists, (int)rows, w.pass.row_coef);
+      return;
+    }
+  }
+  distill_dz_kernel<T><<<grid_for((rows_pad / 8) * n_vtiles, 1, sms, 16), 256, 0, st>>>(
+      slab, v_pad, w.pass.tile_max, w.pass.lse, d.mass, d.lists, (int)rows_pad, (int)rows, n_vtiles, p->chunk_rows,
+      d.boost);
+}
+
+}  // namespace
+
+extern "C" {
+
+int lce_distill_workspace_bytes(const lce_problem* p, int32_t k, size_t* bytes) {
+  const int v = validate_distill(p, k);
+  if (v != LCE_OK) return v;
+  if (bytes == nullptr) return LCE_ERR_INVALID_ARGUMENT;
+  *bytes = layout_distill(p, k, nullptr, sm_count_or_default()).total;
+  return LCE_OK;
+}
+
+int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const void* x, int64_t x_ld,
+                     const void* weight, int64_t w_ld, void* workspace, void* dx, int64_t dx_ld, void* dweight,
+                     int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, float* loss, void* stream) {
+  if (p_in == nullptr || teacher == nullptr) return LCE_ERR_INVALID_ARGUMENT;
+  int v = validate_distill(p_in, teacher->k);
+  if (v != LCE_OK) return v;
+  const float temperature = teacher->temperature;
+  if (!(temperature > 0.f) || !(temperature < INFINITY)) return LCE_ERR_INVALID_ARGUMENT;
+  if (teacher->logits_dtype != LCE_DTYPE_F16 && teacher->logits_dtype != LCE_DTYPE_BF16 &&
+      teacher->logits_dtype != LCE_DTYPE_F32)
+    return LCE_ERR_INVALID_ARGUMENT;
+  if (teacher->indices_bits != 32 && teacher->indices_bits != 64) return LCE_ERR_INVALID_ARGUMENT;
+  if (!teacher->logits || !teacher->indices || teacher->logits_ld < 0 || teacher->indices_ld < 0)
+    return LCE_ERR_INVALID_ARGUMENT;
+  if (!x || !weight || !workspace || !loss) return LCE_ERR_INVALID_ARGUMENT;
+  if (!p_in->want_grad && (dx || dweight)) return LCE_ERR_INVALID_ARGUMENT;
+  if (p_in->want_grad && !dx && !dweight) return LCE_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  if ((v = ensure_device(&sms)) != LCE_OK) return v;
+
+  lce_problem prob = *p_in;
+  const lce_problem* p = &prob;
+  prob.logit_scale = p_in->logit_scale / temperature;
+  prob.ignore_index = kIgnoredRow;
+  if (!(prob.logit_scale > 0.f)) return LCE_ERR_INVALID_ARGUMENT;
+  const DistillWorkspace w = layout_distill(p, teacher->k, workspace, sms);
+  cudaStream_t st = (cudaStream_t)stream;
+  TeacherInput in;
+  in.logits = teacher->logits;
+  in.indices = teacher->indices;
+  in.lse = teacher->lse;
+  in.logits_ld = teacher->logits_ld;
+  in.indices_ld = teacher->indices_ld;
+  in.k = teacher->k;
+  in.logits_dtype = teacher->logits_dtype;
+  in.indices_64 = teacher->indices_bits == 64;
+  in.inv_temperature = 1.f / temperature;
+
+  Distill d;
+  d.boost = p->dtype == LCE_DTYPE_F16 ? 16384.f : 1.f;
+  d.grad_scale = p_in->logit_scale * temperature / d.boost;
+  d.list_z = w.list_z;
+  d.lists.idx = w.list_idx;
+  d.lists.q = w.list_q;
+  d.lists.z = w.list_z;
+  d.lists.start = w.start;
+  d.lists.start_ld = p->chunk_rows;
+  d.lists.k = teacher->k;
+  d.lists.n_tiles = (int)(vocab_pad(p) / BLOCK_N);
+
+  const int64_t n_chunks = (p->n_rows_total + p->chunk_rows - 1) / p->chunk_rows;
+  const bool one_chunk = n_chunks == 1;
+  if ((v = launch_prepare(p, in, w, 0, p->n_rows_total, one_chunk, st)) != LCE_OK) return v;
+  const int64_t* labels = reinterpret_cast<const int64_t*>(w.labels);
+  if ((v = lce_begin(p, labels, workspace, stream)) != LCE_OK) return v;
+  for (int64_t ci = 0; ci < n_chunks; ++ci) {
+    const int64_t row0 = ci * p->chunk_rows;
+    const int64_t rows = std::min<int64_t>(p->chunk_rows, p->n_rows_total - row0);
+    d.mass = w.mass + row0;
+    d.lists.plogp = w.plogp + row0;
+    if (!one_chunk && (v = launch_prepare(p, in, w, row0, rows, true, st)) != LCE_OK) return v;
+    if ((v = forward_chunk(p, x, x_ld, weight, w_ld, labels, row0, rows, workspace, w.row_parts, stream, &d)) != LCE_OK)
+      return v;
+    if ((v = combine_chunk(p, w.row_parts, labels, row0, rows, workspace, stream, &d)) != LCE_OK) return v;
+    if (!p->want_grad) continue;
+    switch (p->dtype) {
+      case LCE_DTYPE_F16: launch_distill_dz<__half>(p, w, d, x, x_ld, row0, rows, sms, st); break;
+      case LCE_DTYPE_BF16: launch_distill_dz<__nv_bfloat16>(p, w, d, x, x_ld, row0, rows, sms, st); break;
+      default: launch_distill_dz<float>(p, w, d, x, x_ld, row0, rows, sms, st);
+    }
+    if ((v = check_launch()) != LCE_OK) return v;
+    if (dx && (v = dx_chunk(p, weight, w_ld, row0, rows, workspace, dx, dx_ld, p->dtype, stream, d.grad_scale)) != LCE_OK)
+      return v;
+    if (dweight && (v = dw_chunk(p, x, x_ld, row0, rows, workspace, dweight, dw_ld, dweight_residual, dwr_ld, ci == 0,
+                                 ci == n_chunks - 1, stream, d.grad_scale)) != LCE_OK)
+      return v;
+  }
+  distill_finalize_kernel<<<1, 32, 0, st>>>(w.pass.scalars, temperature, loss);
+  return check_launch();
 }
 
 }  // extern "C"

@@ -1,0 +1,207 @@
+"""Distillation of a vocabulary head from a teacher's top logits, fused with the head's matrix product.
+
+    z    = logit_scale * (x @ At)
+    q_ik = softmax over the row's K listed teacher logits / T       (or exp(t_ik / T - teacher_lse_i))
+    loss = T^2 / n * sum_i sum_k q_ik (log q_ik - log_softmax(z_i / T)[idx_ik])
+
+over the n rows whose list has any weight. The pass is the one of the cross-entropy loss -- row chunks, one slab of
+exponentials, both gradients during ``forward`` -- with K soft targets per row in the place of the label: nothing of
+size N x V exists beyond one chunk, and the teacher's distribution is never spread over the vocabulary. The reference
+project has no counterpart.
+"""
+from __future__ import annotations
+
+import os
+from typing import Optional
+
+import torch
+
+from . import _native
+from .ops import (
+    _DTYPE_CODE,
+    LinearCrossEntropyLoss,
+    _aligned_rows_like,
+    _autocast_target,
+    _device_guard,
+    _scaled_grads,
+    _tma_ready,
+    get_backend,
+    slab_mode_policy,
+)
+
+
+def _run_pass(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size, want_dx, want_dW):
+    """(loss, dx, dW); x (N, H) and At (H, V) as the kernels read them (:func:`_operands`)."""
+    backend = get_backend()
+    N, H = x.shape
+    V = At.shape[1]
+    dev = x.device
+    want_grad = want_dx or want_dW
+    N_group = -(-min(N, int(N_chunk_size)) // 128) * 128
+    capturing = dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    policy_key = (dev.index, x.dtype, H, V, N_group, 1, "distill")
+    if capturing and x.dtype != torch.float16 and os.environ.get("LCE_SLAB_MODE", "auto") == "auto":
+        # the policy polls an event, which a capture does not allow: the mode that never recomputes for small chunks,
+        # the default one otherwise
+        small = N_group * V < slab_mode_policy.small_slab_elems
+        slab_mode = _native.SLAB_PER_TILE if small else _native.SLAB_DEFAULT
+    else:
+        slab_mode = slab_mode_policy.choose(policy_key, x.dtype)
+    prob = _native.Problem(
+        n_rows_total=N, chunk_rows=N_group, hidden=H, vocab_local=V, vocab_offset=0, ignore_index=-100, world=1,
+        dtype=_DTYPE_CODE[x.dtype], monitoring=0, want_grad=1 if want_grad else 0, logit_scale=float(logit_scale),
+        z_regularization=0.0, slab_mode=slab_mode,
+    )
+    k = t.shape[1]
+    workspace = torch.empty(backend.distill_workspace_bytes(prob, k), dtype=torch.uint8, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    dx = torch.empty((N, H), dtype=x.dtype, device=dev) if want_dx else None
+    dW = dW_res = None
+    if want_dW:
+        dW = _aligned_rows_like((H, V), At.dtype, dev)
+        if N > N_group and At.dtype != torch.float32:
+            dW_res = _aligned_rows_like((H, V), At.dtype, dev)  # the rounding residual of the sum over the chunks
+    teacher = _native.Teacher(
+        logits=t.data_ptr(), indices=idx.data_ptr(), lse=None if lse is None else lse.data_ptr(),
+        logits_ld=t.stride(0), indices_ld=idx.stride(0), k=k, logits_dtype=_DTYPE_CODE[t.dtype],
+        indices_bits=64 if idx.dtype == torch.int64 else 32, temperature=float(temperature),
+    )
+    backend.distill_pass(prob, teacher, x, At, workspace, dx, dW, dW_res, loss)
+    if (getattr(backend, "requires_cuda", True) and not capturing and slab_mode == _native.SLAB_DEFAULT
+            and os.environ.get("LCE_SLAB_MODE", "auto") == "auto"):
+        slab_mode_policy.record(policy_key, backend, workspace)
+    return loss, dx, dW
+
+
+def _operands(x, At):
+    """x and At with rows on 16-byte boundaries and a hidden size that is a multiple of 8 (copies where they are not)."""
+    H, V = At.shape
+    H8 = -(-H // 8) * 8
+    if H8 != H:  # zero columns of x and zero rows of the weight leave the logits as they are
+        x_pad = x.new_zeros((x.shape[0], H8))
+        x_pad[:, :H] = x
+        A_pad = _aligned_rows_like((H8, V), At.dtype, At.device)
+        A_pad[:H] = At
+        A_pad[H:] = 0
+        return x_pad, A_pad
+    if not _tma_ready(x):
+        x = x.contiguous()
+    if not _tma_ready(At):
+        copy = _aligned_rows_like(At.shape, At.dtype, At.device)
+        copy.copy_(At)
+        At = copy
+    return x, At
+
+
+class LinearDistillationImplementation(torch.autograd.Function):
+    """Computes the loss and both gradients in ``forward``; ``backward`` multiplies them by ``grad_output``."""
+
+    @staticmethod
+    def forward(ctx, x_in, At_in, t, idx, lse, temperature, logit_scale, N_chunk_size):
+        with _device_guard(x_in):
+            H = x_in.shape[-1]
+            x, At = _operands(x_in.reshape(-1, H), At_in)
+            with torch.no_grad():
+                loss, dx, dW = _run_pass(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size,
+                                         bool(ctx.needs_input_grad[0]), bool(ctx.needs_input_grad[1]))
+            if dx is not None:
+                dx = dx[:, :H]
+            if dW is not None:
+                dW = dW[:H]
+            ctx.lce_grads = (dx, dW) if dx is not None or dW is not None else None
+            ctx.lce_x_shape = x_in.shape
+            ctx.lce_x_dtype = x_in.dtype
+            return loss
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        if ctx.lce_grads is None:
+            raise RuntimeError("backward called twice, or forward ran without any input requiring grad")
+        with _device_guard(grad_output), torch.no_grad():
+            gx, gA = _scaled_grads(ctx, grad_output)
+        return gx, gA, None, None, None, None, None, None
+
+
+def linear_distillation(
+    x: torch.Tensor,
+    teacher_logits: torch.Tensor,
+    teacher_indices: torch.Tensor,
+    At: torch.Tensor,
+    teacher_lse: Optional[torch.Tensor] = None,
+    temperature: float = 1.0,
+    logit_scale: float = 1.0,
+    N_chunk_size: int = 4096,
+) -> torch.Tensor:
+    """The distillation loss of the head ``x @ At`` against a teacher's top logits (a scalar, float32).
+
+    x: (..., H); At: (H, V), the transposed weight of :class:`LinearCrossEntropyLoss`; float16, bfloat16 or float32
+    (multiplied as TF32), any sizes. teacher_logits: (..., K) in any of these types; teacher_indices: (..., K) int64 or int32;
+    1 <= K <= 1024. Both as :func:`top_logits` returns them; any order will do.
+
+    The teacher's distribution is softmax(teacher_logits / temperature) over the K listed tokens, or, with
+    teacher_lse: (...) = logsumexp(all teacher logits / temperature), exp(teacher_logits / temperature - teacher_lse): then the
+    mass that the list leaves out has no target, and the student's mass on the listed tokens is drawn to Q = sum(q) times
+    its softmax. teacher_lse has to be at least the log-sum-exp of the listed logits.
+
+    An entry with an index outside [0, V) is not there, whatever its logit (lists of different lengths are padded with -1); one
+    with logit -inf has no weight; rows without any weight do not count (if none counts, the loss is NaN, like that of the
+    cross-entropy). NaN or +inf in an entry that is there make the loss NaN. An index that is listed twice counts twice.
+
+    Gradients for x and At only (those that are wanted are computed during the forward pass); under CUDA autocast x and At
+    are cast as :func:`set_autocast_policy` says.
+    """
+    assert x.dim() >= 1 and At.dim() == 2 and At.shape[0] == x.shape[-1], "x and the weight disagree on the hidden size"
+    rows = x.shape[:-1]
+    assert teacher_logits.shape[:-1] == rows, "teacher_logits must have one list per row of x"
+    assert teacher_indices.shape == teacher_logits.shape, "teacher_indices must have the shape of teacher_logits"
+    k = teacher_logits.shape[-1]
+    assert 1 <= k <= _native.TEACHER_MAX, f"between 1 and {_native.TEACHER_MAX} entries per row"
+    assert teacher_logits.dtype in _DTYPE_CODE, f"unsupported dtype {teacher_logits.dtype} of teacher_logits"
+    assert teacher_indices.dtype in (torch.int64, torch.int32), "teacher_indices must be int64 or int32"
+    assert temperature > 0 and temperature < float("inf"), "temperature must be positive"
+    assert logit_scale > 0
+    assert int(N_chunk_size) >= 1
+    assert x.numel() > 0 and At.shape[1] >= 1, "x must have at least one row"
+    if teacher_lse is not None:
+        assert teacher_lse.shape == rows, "teacher_lse must have one entry per row of x"
+        assert teacher_lse.is_floating_point(), "teacher_lse must be floating point"
+        teacher_lse = teacher_lse.detach().to(torch.float32).reshape(-1).contiguous()
+    given = [t for t in (x, At, teacher_logits, teacher_indices, teacher_lse) if t is not None]
+    assert all(t.device == x.device for t in given), "all tensors must be on one device"
+    target = _autocast_target(x)
+    if target is not None:
+        x, At = x.to(target), At.to(target)
+    assert x.dtype == At.dtype, "x and the weight must have the same dtype"
+    assert x.dtype in _DTYPE_CODE, f"unsupported dtype {x.dtype}"
+    if getattr(get_backend(), "requires_cuda", True) and not x.is_cuda:
+        raise RuntimeError("linear_cross_entropy_loss_b200 runs on CUDA tensors only; there is no CPU fallback")
+
+    def lists(t):
+        t = t.detach().reshape(-1, k)
+        return t if t.stride(1) == 1 or k == 1 else t.contiguous()
+
+    if not torch.is_grad_enabled():
+        x, At = x.detach(), At.detach()
+    with torch.autocast(device_type=x.device.type, enabled=False):
+        return LinearDistillationImplementation.apply(
+            x, At, lists(teacher_logits), lists(teacher_indices), teacher_lse, temperature, logit_scale, N_chunk_size)
+
+
+class LinearDistillationLoss(LinearCrossEntropyLoss):
+    """The head of :class:`LinearCrossEntropyLoss` (same constructor, weight and ``state_dict``) with
+    ``forward(x, teacher_logits, teacher_indices, teacher_lse=None)`` = :func:`linear_distillation`.
+
+    Assign ``distill.weight = head.weight`` to train one weight with both losses. ``ignore_index``, ``z_regularization`` and
+    ``monitoring`` have no meaning here.
+    """
+
+    def __init__(self, in_features: int, out_features: int, device=None, dtype=None, temperature: float = 1.0,
+                 logit_scale: float = 1.0, N_chunk_size: int = 4096, init_method=None):
+        assert temperature > 0
+        super().__init__(in_features, out_features, device=device, dtype=dtype, logit_scale=logit_scale,
+                         N_chunk_size=N_chunk_size, init_method=init_method)
+        self.temperature = temperature
+
+    def forward(self, x, teacher_logits, teacher_indices, teacher_lse=None):
+        return linear_distillation(x, teacher_logits, teacher_indices, self.weight, teacher_lse, self.temperature,
+                                   self.logit_scale, self.N_chunk_size)

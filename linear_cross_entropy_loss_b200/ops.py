@@ -185,6 +185,22 @@ class NativeBackend:
             "lce_grad_scale_cast",
         )
 
+    def distill_workspace_bytes(self, prob, k) -> int:
+        out = ctypes.c_size_t(0)
+        _native.check(self.lib.lce_distill_workspace_bytes(ctypes.byref(prob), k, ctypes.byref(out)),
+                      "lce_distill_workspace_bytes")
+        return int(out.value)
+
+    def distill_pass(self, prob, teacher, x, At, workspace, dx, dW, dW_res, loss):
+        _native.check(
+            self.lib.lce_distill_pass(
+                ctypes.byref(prob), ctypes.byref(teacher), _ptr(x), x.stride(0), _ptr(At), At.stride(0), _ptr(workspace),
+                _ptr(dx), 0 if dx is None else dx.stride(0), _ptr(dW), 0 if dW is None else dW.stride(0), _ptr(dW_res),
+                0 if dW_res is None else dW_res.stride(0), _ptr(loss), self._stream(workspace),
+            ),
+            "lce_distill_pass",
+        )
+
     def top_logits(self, logits, k, temperature, values, indices, lse):
         _native.check(
             self.lib.lce_top_logits(

@@ -1,10 +1,10 @@
-"""top_logits and sample_logits without a GPU: what the Python layer and the C ABI refuse, before any device is touched."""
+"""top_logits, sample_logits and linear_distillation without a GPU: what the Python layer and the C ABI refuse, before any device is touched."""
 import ctypes
 
 import pytest
 import torch
 
-from linear_cross_entropy_loss_b200 import _native, sample_logits, top_logits
+from linear_cross_entropy_loss_b200 import LinearDistillationLoss, _native, linear_distillation, sample_logits, top_logits
 
 
 @pytest.fixture(scope="module")
@@ -104,7 +104,7 @@ def test_no_rows_need_no_device(lib):
     assert lib.lce_sample_logits(1, None, 100, 0, 100, ctypes.byref(s), None, None, None) == 0
 
 
-def test_sampling_structure_has_the_layout_of_the_header(tmp_path):
+def check_layout(tmp_path, name, mirror, constants):
     import shutil
     import subprocess
     from pathlib import Path
@@ -113,13 +113,114 @@ def test_sampling_structure_has_the_layout_of_the_header(tmp_path):
     if gcc is None:
         pytest.skip("no C compiler")
     header = Path(__file__).resolve().parent.parent / "include" / "lce_b200.h"
-    fields = [f[0] for f in _native.Sampling._fields_]
+    fields = [f[0] for f in mirror._fields_]
     lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{header}"', "int main(void) {",
-             '  printf("%zu %d %d\\n", sizeof(lce_sampling), LCE_TOP_MAX, LCE_SAMPLING_U_F64);']
-    lines += [f'  printf("%zu\\n", offsetof(lce_sampling, {f}));' for f in fields] + ["  return 0;", "}"]
+             f'  printf("%zu\\n", sizeof({name}));']
+    lines += [f'  printf("%d\\n", (int){c});' for c, _ in constants]
+    lines += [f'  printf("%zu\\n", offsetof({name}, {f}));' for f in fields] + ["  return 0;", "}"]
     src, exe = tmp_path / "layout.c", tmp_path / "layout"
     src.write_text("\n".join(lines))
     subprocess.run([gcc, "-std=c99", "-Wall", "-Werror", "-pedantic", "-o", str(exe), str(src)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
-    assert got == ([ctypes.sizeof(_native.Sampling), _native.TOP_MAX, _native.SAMPLING_U_F64]
-                   + [getattr(_native.Sampling, f).offset for f in fields])
+    assert got == [ctypes.sizeof(mirror)] + [v for _, v in constants] + [getattr(mirror, f).offset for f in fields]
+
+
+def test_sampling_structure_has_the_layout_of_the_header(tmp_path):
+    check_layout(tmp_path, "lce_sampling", _native.Sampling,
+                 [("LCE_TOP_MAX", _native.TOP_MAX), ("LCE_SAMPLING_U_F64", _native.SAMPLING_U_F64)])
+
+
+# ---------------------------------------------------------------------------------------------------- distillation
+def distill_args(N=4, H=16, V=32, K=3):
+    return dict(x=torch.zeros(N, H), teacher_logits=torch.zeros(N, K), teacher_indices=torch.zeros(N, K, dtype=torch.int64),
+                At=torch.zeros(H, V))
+
+
+@pytest.mark.parametrize("change", [
+    dict(At=torch.zeros(15, 32)), dict(At=torch.zeros(16)), dict(At=torch.zeros(16, 0)), dict(x=torch.zeros(0, 16), teacher_logits=torch.zeros(0, 3), teacher_indices=torch.zeros(0, 3, dtype=torch.int64)),
+    dict(teacher_logits=torch.zeros(5, 3)), dict(teacher_indices=torch.zeros(4, 2, dtype=torch.int64)),
+    dict(teacher_indices=torch.zeros(4, 3)), dict(teacher_indices=torch.zeros(4, 3, dtype=torch.int16)),
+    dict(teacher_logits=torch.zeros(4, 3, dtype=torch.float64)), dict(teacher_logits=torch.zeros(4, 0), teacher_indices=torch.zeros(4, 0, dtype=torch.int64)),
+    dict(teacher_logits=torch.zeros(4, 1025), teacher_indices=torch.zeros(4, 1025, dtype=torch.int64)),
+    dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
+    dict(logit_scale=0.0), dict(N_chunk_size=0), dict(teacher_lse=torch.zeros(3)), dict(teacher_lse=torch.zeros(4, dtype=torch.int64)),
+    dict(At=torch.zeros(16, 32, dtype=torch.bfloat16)), dict(x=torch.zeros(4, 16, dtype=torch.float64), At=torch.zeros(16, 32, dtype=torch.float64)),
+    dict(teacher_indices=torch.zeros(4, 3, dtype=torch.int64, device="meta")),
+])
+def test_linear_distillation_refuses(change):
+    a = distill_args()
+    a.update(change)
+    with pytest.raises(AssertionError):
+        linear_distillation(**a)
+
+
+def test_linear_distillation_has_no_cpu_fallback():
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        linear_distillation(**distill_args())
+
+
+def test_distillation_module_is_a_head():
+    head = LinearDistillationLoss(16, 32, temperature=2.0, logit_scale=0.5)
+    assert head.weight.shape == (16, 32) and list(head.state_dict()) == ["weight"]
+    with pytest.raises(AssertionError):
+        LinearDistillationLoss(16, 32, temperature=0.0)
+
+
+def teacher(**kw):
+    base = dict(logits=16, indices=16, lse=None, logits_ld=8, indices_ld=8, k=8, logits_dtype=_native.DTYPE_BF16,
+                indices_bits=64, temperature=1.0)
+    base.update(kw)
+    return _native.Teacher(**base)
+
+
+def distill_problem(**kw):
+    base = dict(n_rows_total=1024, chunk_rows=256, hidden=256, vocab_local=4096, vocab_offset=0, ignore_index=-100,
+                world=1, dtype=_native.DTYPE_BF16, monitoring=0, want_grad=1, logit_scale=1.0, z_regularization=0.0)
+    base.update(kw)
+    return _native.Problem(**base)
+
+
+def call_distill(lib, p, t, **kw):
+    a = dict(x=16, w=16, ws=16, dx=16, dw=16, res=16, loss=16)
+    a.update(kw)
+    return lib.lce_distill_pass(ctypes.byref(p), None if t is None else ctypes.byref(t), a["x"], 256, a["w"], 4096, a["ws"],
+                                a["dx"], 256, a["dw"], 4096, a["res"], 4096, a["loss"], None)
+
+
+@pytest.mark.parametrize("p_kw,t_kw,code", [
+    (dict(world=2), {}, -1), (dict(vocab_offset=5), {}, -1), (dict(chunk_buffers=2), {}, -1), (dict(monitoring=1), {}, -1),
+    (dict(z_regularization=0.1), {}, -1), (dict(hidden=100), {}, -2), (dict(dtype=9), {}, -1), (dict(logit_scale=0.0), {}, -1),
+    ({}, dict(k=0), -1), ({}, dict(k=1025), -8), ({}, dict(temperature=0.0), -1), ({}, dict(temperature=float("nan")), -1),
+    ({}, dict(temperature=float("inf")), -1), ({}, dict(logits_dtype=3), -1), ({}, dict(indices_bits=16), -1), ({}, dict(logits=None), -1),
+    ({}, dict(indices=None), -1), ({}, dict(logits_ld=-1), -1), ({}, dict(indices_ld=-8), -1),
+])
+def test_distill_abi_refuses(lib, p_kw, t_kw, code):
+    assert call_distill(lib, distill_problem(**p_kw), teacher(**t_kw)) == code
+
+
+def test_distill_abi_refuses_missing_pointers(lib):
+    p = distill_problem()
+    assert call_distill(lib, p, None) == -1
+    for name in ("x", "w", "ws", "loss"):
+        assert call_distill(lib, p, teacher(), **{name: None}) == -1
+    assert call_distill(lib, p, teacher(), dx=None, dw=None) == -1
+    assert call_distill(lib, distill_problem(want_grad=0), teacher()) == -1
+
+
+def test_distill_workspace(lib):
+    out = ctypes.c_size_t(0)
+    plain = ctypes.c_size_t(0)
+    p = distill_problem()
+    assert lib.lce_workspace_bytes(ctypes.byref(p), ctypes.byref(plain)) == 0
+    sizes = []
+    for k in (1, 64, 1024):
+        assert lib.lce_distill_workspace_bytes(ctypes.byref(p), k, ctypes.byref(out)) == 0
+        sizes.append(out.value - plain.value)
+        assert out.value >= plain.value + 1024 * 16 + 256 * k * 12 + 17 * 256 * 2
+    assert sizes[2] - sizes[1] == 256 * 960 * 12
+    assert lib.lce_distill_workspace_bytes(ctypes.byref(p), 8, None) == -1
+    assert lib.lce_distill_workspace_bytes(ctypes.byref(p), 0, ctypes.byref(out)) == -1
+
+
+def test_teacher_structure_has_the_layout_of_the_header(tmp_path):
+    check_layout(tmp_path, "lce_teacher", _native.Teacher, [("LCE_TEACHER_MAX", _native.TEACHER_MAX)])
