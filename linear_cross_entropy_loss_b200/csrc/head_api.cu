@@ -7,27 +7,69 @@ namespace {
 
 using namespace lce;
 
+static_assert(LCE_TOP_MAX == kTopMax, "the header's limit");
+
 int check_rows(int dtype, const void* logits, long long ld, long long rows, long long vocab) {
   if (dtype != LCE_DTYPE_F16 && dtype != LCE_DTYPE_BF16 && dtype != LCE_DTYPE_F32) return LCE_ERR_INVALID_ARGUMENT;
   if (rows < 0 || vocab <= 0 || ld < 0 || (rows > 0 && logits == nullptr)) return LCE_ERR_INVALID_ARGUMENT;
-  if (rows > (1ll << 30) || vocab > (1ll << 30)) return LCE_ERR_TOO_LARGE;
+  if (rows > (1ll << 27) || vocab > (1ll << 30)) return LCE_ERR_TOO_LARGE;
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == LCE_DTYPE_F32 ? 3u : 1u)) != 0) return LCE_ERR_MISALIGNED;
   return LCE_OK;
 }
 
-int power_of_two_from(long long n) {
-  int p = 1;
-  while (p < n) p <<= 1;
-  return p;
+// SMs of the current device (148 where that cannot be asked), read once per device.
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// One launch of `blocks` blocks in clusters of `parts`.
+template <typename... Args, typename... Given>
+int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size_t smem, int parts, cudaStream_t st,
+                    Given... given) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)blocks);
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)parts;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = parts > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, kernel, Args(given)...) != cudaSuccess) {
+    cudaGetLastError();
+    return LCE_ERR_CUDA;
+  }
+  return check_launch();
+}
+
+// Blocks that share a row: doubled while the blocks of all rows fit the GPU at once (four of kTopThreads on an SM), a part
+// keeps a whole batch, and the lists of all parts fit one.
+template <typename T>
+int top_parts(int64_t rows, int64_t vocab, int k) {
+  const int64_t batch = (int64_t)kTopThreads * kTopUnroll * (16 / (int)sizeof(T));
+  int parts = 1;
+  while (parts < 8 && rows * parts * 2 <= 4ll * sm_count() && vocab >= batch * parts && k * parts * 2 <= kTopList) parts *= 2;
+  return parts;
 }
 
 template <typename T>
 int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int k, float inv_t, void* values,
                int64_t* indices, float* lse, cudaStream_t st) {
-  top_logits_kernel<T><<<(int)rows, kTopThreads, 0, st>>>(
-      reinterpret_cast<const T*>(logits), ld, (uint32_t)vocab, k, power_of_two_from(k), inv_t,
-      reinterpret_cast<T*>(values), reinterpret_cast<long long*>(indices), lse);
-  return check_launch();
+  const int parts = top_parts<T>(rows, vocab, k);
+  return launch_clusters(top_logits_kernel<T>, rows * parts, kTopThreads, 0, parts, st,
+                         reinterpret_cast<const T*>(logits), (long long)ld, (uint32_t)vocab, k, parts, inv_t,
+                         reinterpret_cast<T*>(values), reinterpret_cast<long long*>(indices), lse);
 }
 
 template <typename T>
@@ -49,7 +91,7 @@ int lce_top_logits(int32_t dtype, const void* logits, int64_t ld, int64_t rows, 
   const int v = check_rows(dtype, logits, ld, rows, vocab);
   if (v != LCE_OK) return v;
   if (k < 1 || !(temperature > 0.f)) return LCE_ERR_INVALID_ARGUMENT;
-  if (k > vocab || k > kTopMax) return LCE_ERR_TOO_LARGE;
+  if (k > vocab || k > LCE_TOP_MAX) return LCE_ERR_TOO_LARGE;
   if (rows == 0) return LCE_OK;
   if (!values || !indices || !lse) return LCE_ERR_INVALID_ARGUMENT;
   cudaStream_t st = (cudaStream_t)stream;

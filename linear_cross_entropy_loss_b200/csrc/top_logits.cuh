@@ -1,51 +1,85 @@
-// top_logits: the k largest logits of each row with their indices, and the row's log-sum-exp.
+// top_logits: the k largest logits of each row with their indices, and the row's log-sum-exp. The row is read once
+// (row_top.cuh); `parts` blocks of a cluster share a row when there are too few rows to fill the GPU.
 #pragma once
 
-#include "row_select.cuh"
+#include "row_top.cuh"
+
+#include <cooperative_groups.h>
 
 namespace lce {
 
-constexpr int kTopMax = 1024;
-constexpr int kTopThreads = 512;
-
-// One block per row. k <= min(vocab, kTopMax); `padded`: k rounded up to a power of two.
-template <typename T>
-__global__ void __launch_bounds__(kTopThreads)
-top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int k, int padded, float inv_temperature,
-                  T* __restrict__ values, long long* __restrict__ indices, float* __restrict__ lse) {
-  __shared__ SelectScratch s;
-  __shared__ float scratch[32];
-  __shared__ unsigned long long list[kTopMax];
-  __shared__ int listed;
-  const long long r = blockIdx.x;
-  const T* row = logits + r * ld;
-  const RowCut cut = find_cut(row, vocab, (unsigned long long)k, s, [](float, uint32_t, uint32_t) { return 1ull; });
-  if (threadIdx.x == 0) listed = 0;
-  for (int i = threadIdx.x; i < padded; i += blockDim.x) list[i] = 0;
-  __syncthreads();
-  float m = -INFINITY;
-  bool nan = false;
-  for (uint32_t j = threadIdx.x; j < vocab; j += blockDim.x) {
-    const float l = logit_to_float(row[j]);
-    const uint32_t key = order_key(l);
-    m = fmaxf(m, l);
-    nan |= l != l;
-    if (inside(cut, key, j)) list[atomicAdd(&listed, 1)] = order_pair(key, j);
+// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then holds the row's k first
+// entries, sorted. k * parts <= kTopList. The other blocks return with their part done.
+__device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
+  thin_list(s, k);
+  if (parts > 1) {
+    if (s.count > unsigned(kTopList / parts)) sort_list(s, k);  // many equal logits: exactly k
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    if (cluster.block_rank() == 0) {
+      unsigned int at = s.count;
+      for (int part = 1; part < parts; ++part) {
+        const TopShared* other = cluster.map_shared_rank(&s, part);
+        const unsigned int n = other->count;
+        for (unsigned int i = threadIdx.x; i < n; i += kTopThreads) s.list[at + i] = other->list[i];
+        at += n;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        s.count = at;
+        float m = s.part_ref;
+        for (int part = 1; part < parts; ++part) m = fmaxf(m, cluster.map_shared_rank(&s, part)->part_ref);
+        float sum = 0.f;
+        for (int part = 0; part < parts; ++part) {
+          const TopShared* other = cluster.map_shared_rank(&s, part);
+          if (other->part_ref > -INFINITY) sum += other->part_sum * fast_exp2(other->part_ref - m);
+        }
+        s.part_ref = m;
+        s.part_sum = sum;
+      }
+    }
+    cluster.sync();
+    if (cluster.block_rank() != 0) return;
+    thin_list(s, k);
   }
-  m = block_max(m, scratch);
-  nan = block_max(nan ? 1.f : 0.f, scratch) > 0.f;
-  float sum = 0.f;
-  if (m > -INFINITY && m < INFINITY)
-    for (uint32_t j = threadIdx.x; j < vocab; j += blockDim.x)
-      sum += __expf((logit_to_float(row[j]) - m) * inv_temperature);
-  sum = block_sum(sum, scratch);
-  if (threadIdx.x == 0)
-    lse[r] = nan ? __uint_as_float(0x7fc00000u) : ((m > -INFINITY && m < INFINITY) ? m * inv_temperature + logf(sum) : m);
-  block_sort_descending(list, padded);
-  for (int i = threadIdx.x; i < k; i += blockDim.x) {
-    const uint32_t j = pair_index(list[i]);
-    values[r * k + i] = row[j];
-    indices[r * k + i] = j;
+  sort_list(s, k);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads, 4)
+top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int k, int parts, float inv_temperature,
+                  T* __restrict__ values, long long* __restrict__ indices, float* __restrict__ lse) {
+  __shared__ TopShared s;
+  const long long r = blockIdx.x / parts;
+  const int part = int(blockIdx.x % parts);
+  const RowVectors<T> row(logits + r * ld, vocab);
+  const int share = (row.vectors + parts - 1) / parts;
+  const int v0 = min(part * share, row.vectors), v1 = min(v0 + share, row.vectors);
+  const float log2_scale = inv_temperature * 1.4426950408889634f;
+  float ref, sum;
+  stream_top<T, true>(s, row, v0, v1, k, log2_scale, ref, sum);
+  const float m = block_max(ref, s.scratch);
+  sum = block_sum(ref > -INFINITY ? sum * fast_exp2(ref - m) : 0.f, s.scratch);
+  if (threadIdx.x == 0) {
+    s.part_ref = m;
+    s.part_sum = sum;
+  }
+  merge_lists(s, k, parts);
+  if (part != 0) return;
+  for (int i = threadIdx.x; i < k; i += kTopThreads) {
+    const unsigned long long e = s.list[i];
+    values[r * k + i] = T(key_to_float(pair_key(e)));
+    indices[r * k + i] = pair_index(e);
+  }
+  if (threadIdx.x == 0) {
+    // The sum is over 2^(l * log2_scale), whose exponents are right to the rounding of log2_scale; at the largest
+    // logit, which carries the sum, that rounding is put back.
+    const uint32_t first = pair_key(s.list[0]);
+    const double largest = double(key_to_float(first));
+    const double put_back = largest * (double(inv_temperature) - double(log2_scale) * 0.69314718055994531);
+    float v = float((double(s.part_ref) + double(log2f(s.part_sum))) * 0.69314718055994531 + put_back);
+    if (first >= kKeyPosInf || first == kKeyNegInf) v = key_to_float(first);  // +inf, NaN; nothing but -inf
+    lse[r] = v;
   }
 }
 
