@@ -1,14 +1,16 @@
-// The k largest logits of a row, found while the row streams past once: a short list in shared memory collects every
-// logit that may still be among the k largest, and its bound rises as the row goes on.
+// The k largest logits of a row, found while the row streams past once.
 //
-// * The row is read in batches of kTopThreads * kTopUnroll vectors of 16 bytes, the next batch on its way while one is
-//   looked at. One comparison of a vector's maximum with the bound decides for all its elements, so the elements cost
-//   no more than their share of the log-sum-exp (or nothing where that is not wanted).
-// * The first bound comes from the first batch: the k-th largest of its vectors' maxima. At least k elements reach it, and of
-//   a row of random order about k per batch do.
-// * When the list runs full it is cut back to the k first of the order, and from then on only larger logits enter:
-//   an equal one that comes later has a higher index. A batch that would overflow the list (rows in rising order, or
-//   many equal logits) is taken again vector by vector.
+// The row is looked at in vectors of 16 bytes (4 or 8 logits). A list in shared memory keeps the vectors that come first
+// by (largest logit descending, place ascending): the k first of them hold the k first logits, since a vector ahead of
+// another has a logit ahead of all of its. So the streaming loop handles one number per vector: one comparison of its
+// maximum with the bound of the list, and what enters is one entry, however its logits lie. At the end the k vectors are
+// read again and their logits ranked.
+//
+// * Vectors come in batches of kTopThreads * kTopUnroll, the next batch on its way while one is looked at.
+// * The first bound comes from the first batch: the k-th largest of its maxima.
+// * A list that holds twice what is wanted is cut back and the bound raised behind its last entry, so of a row of random
+//   order about k (1 + ln(batches)) vectors enter. An equal maximum that comes later is behind: after a cut only larger ones enter.
+// * Between two batches the list holds at most kTopFull entries, so a batch always fits.
 // A row may be split over the blocks of a cluster; the first block then takes the others' lists.
 #pragma once
 
@@ -22,15 +24,18 @@ namespace lce {
 constexpr int kTopMax = 1024;
 constexpr int kTopThreads = 256;
 constexpr int kTopUnroll = 4;
-constexpr int kTopList = 4096;             // entries of the list
-constexpr int kTopFull = kTopList / 2;     // cut back above this: one more step of 256 vectors still fits
-static_assert(kTopFull >= kTopMax && kTopFull + kTopThreads * 8 <= kTopList, "a step has to fit the list");
+constexpr int kTopList = 2048;             // vectors in the list
+constexpr int kTopFull = kTopList - kTopThreads * kTopUnroll;
+constexpr int kTopElements = 2 * kTopMax;  // logits of the last step: what is kept, and as many from the next vectors
+static_assert(kTopFull >= kTopMax, "the list keeps k vectors and takes a batch");
 
 struct TopShared {
-  unsigned long long list[kTopList];
+  unsigned long long list[kTopList];         // order_pair(largest logit, vector)
+  unsigned long long elements[kTopElements]; // order_pair(logit, index)
   unsigned int counters[34];
   unsigned int range[2];
-  unsigned int count;
+  unsigned int count;        // entries of `list`
+  unsigned int n_elements;   // entries of `elements`
   unsigned long long bound;  // keys from here on enter (2^32: none)
   float scratch[32];
   float part_ref, part_sum;  // log-sum-exp of this block's part
@@ -120,15 +125,30 @@ __device__ __forceinline__ float largest(const uint4& v, const __half*) {
   return max_nan(__low2float(m), __high2float(m));
 }
 
-// Smallest range [lo, ...] of keys that `count_from` says holds at least k entries, or one close to it: stops where the
-// number lies in k .. k + slack. count_from(key): this thread's number of entries >= key.
+// A key that at least k of the block's entries reach, and (unless many are equal) at most k + slack. Bisection of the
+// range of the keys; every step is one count over the block. least / most: over this thread's entries; count_from(key):
+// how many of this thread's entries are >= key. With fewer than k entries: 0.
 template <typename CountFrom>
-__device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, uint32_t lo, uint32_t hi,
+__device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, uint32_t least, uint32_t most,
                                               CountFrom count_from) {
-  // entries >= lo: at least k (the caller sees to it); entries > hi: none
   if (threadIdx.x < 34) s.counters[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    s.range[0] = 0xffffffffu;
+    s.range[1] = 0;
+  }
   __syncthreads();
-  unsigned long long above = (unsigned long long)hi + 1;  // fewer than k from here on
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMin(&s.range[0], least);
+    atomicMax(&s.range[1], most);
+  }
+  const unsigned int all = __reduce_add_sync(0xffffffffu, (unsigned int)count_from(0u));
+  if ((threadIdx.x & 31) == 0) atomicAdd(&s.counters[33], all);
+  __syncthreads();
+  if (int(s.counters[33]) < k) return 0u;
+  uint32_t lo = s.range[0];                                      // k or more from here on
+  unsigned long long above = (unsigned long long)s.range[1] + 1;  // fewer than k from here on
   for (int step = 0; above - lo > 1; ++step) {
     const uint32_t mid = uint32_t(lo + (above - lo) / 2);
     const unsigned int mine = __reduce_add_sync(0xffffffffu, (unsigned int)count_from(mid));
@@ -145,89 +165,52 @@ __device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, ui
   return lo;
 }
 
-// Keeps the entries of the list for which stay(entry) holds, in place: chunk by chunk, each read before any place up to
+// Keeps the entries of a list for which stay(entry) holds, in place: chunk by chunk, each read before any place up to
 // its end is written.
 template <typename Stay>
-__device__ __forceinline__ void filter_list(TopShared& s, int n, Stay stay) {
+__device__ __forceinline__ void filter_list(unsigned long long* list, unsigned int& count, int n, Stay stay) {
   __syncthreads();
-  if (threadIdx.x == 0) s.count = 0;
+  if (threadIdx.x == 0) count = 0;
   for (int i0 = 0; i0 < n; i0 += kTopThreads) {
     const int at = i0 + int(threadIdx.x);
-    const unsigned long long e = at < n ? s.list[at] : 0;
+    const unsigned long long e = at < n ? list[at] : 0;
     __syncthreads();
-    if (at < n && stay(e)) s.list[atomicAdd(&s.count, 1u)] = e;
+    if (at < n && stay(e)) list[atomicAdd(&count, 1u)] = e;
   }
   __syncthreads();
 }
 
-// Leaves at least the k first entries of the order in the list, and few more unless many are equal.
-__device__ __forceinline__ void thin_list(TopShared& s, int k) {
+// Sorts a list of n entries (room for the next power of two of them) and keeps the first k.
+__device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int& count, int n, int k) {
   __syncthreads();
-  const int n = min(int(s.count), kTopList);
-  if (n <= k + k / 4 + 32) return;
-  if (threadIdx.x == 0) {
-    s.range[0] = 0xffffffffu;
-    s.range[1] = 0;
-  }
+  int padded = 2;
+  while (padded < n) padded <<= 1;
+  for (int i = n + threadIdx.x; i < padded; i += kTopThreads) list[i] = 0;
+  block_sort_descending(list, padded);
+  if (threadIdx.x == 0) count = min(n, k);
+  __syncthreads();
+}
+
+// Leaves at least the k first entries of a list, and at most `most_left` (k <= most_left) of them. Returns a key that
+// all of them reach; what comes behind them in the order has a smaller one, or the same.
+__device__ __noinline__ uint32_t cut_list(TopShared& s, unsigned long long* list, unsigned int& count, int k, int most_left) {
+  __syncthreads();
+  const int n = int(count);
   uint32_t least = 0xffffffffu, most = 0;
   for (int i = threadIdx.x; i < n; i += kTopThreads) {
-    const uint32_t key = pair_key(s.list[i]);
+    const uint32_t key = pair_key(list[i]);
     least = min(least, key);
     most = max(most, key);
   }
-  __syncthreads();
-  least = __reduce_min_sync(0xffffffffu, least);
-  most = __reduce_max_sync(0xffffffffu, most);
-  if ((threadIdx.x & 31) == 0) {
-    atomicMin(&s.range[0], least);
-    atomicMax(&s.range[1], most);
-  }
-  __syncthreads();
-  const uint32_t from = bound_for(s, k, k / 4 + 16, s.range[0], s.range[1], [&](uint32_t key) {
+  const uint32_t from = bound_for(s, k, min(k / 4 + 16, most_left - k), least, most, [&](uint32_t key) {
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += kTopThreads) c += pair_key(s.list[i]) >= key;
+    for (int i = threadIdx.x; i < n; i += kTopThreads) c += pair_key(list[i]) >= key;
     return c;
   });
-  filter_list(s, n, [&](unsigned long long e) { return pair_key(e) >= from; });
-}
-
-// Sorts the list and cuts it to its first k entries.
-__device__ __forceinline__ void sort_list(TopShared& s, int k) {
-  __syncthreads();
-  const int n = min(int(s.count), kTopList);
-  int padded = 2;
-  while (padded < n) padded <<= 1;
-  for (int i = n + threadIdx.x; i < padded; i += kTopThreads) s.list[i] = 0;
-  block_sort_descending(s.list, padded);
-  if (threadIdx.x == 0) s.count = min(n, k);
-  __syncthreads();
-}
-
-// Cuts a full list back to its first k entries and raises the bound above the last of them.
-__device__ __noinline__ void cut_list(TopShared& s, int k) {
-  thin_list(s, k);
-  sort_list(s, k);
-  if (threadIdx.x == 0 && int(s.count) == k) s.bound = (unsigned long long)pair_key(s.list[k - 1]) + 1;
-  __syncthreads();
-}
-
-template <typename T>
-__device__ __forceinline__ bool enter_list(TopShared& s, const RowVectors<T>& row, int v, const uint4& raw) {
-  float f[RowVectors<T>::kPer];
-  unpack(raw, f, static_cast<const T*>(nullptr));
-  const unsigned long long bound = s.bound;
-  const int e = row.first_of(v);
-  bool full = false;
-#pragma unroll
-  for (int i = 0; i < RowVectors<T>::kPer; ++i) {
-    const uint32_t key = order_key(f[i]);
-    if (key >= bound && e + i >= 0 && uint32_t(e + i) < row.vocab) {
-      const unsigned int at = atomicAdd(&s.count, 1u);
-      if (at < unsigned(kTopList)) s.list[at] = order_pair(key, uint32_t(e + i));
-      full |= at >= unsigned(kTopFull);
-    }
-  }
-  return full;
+  filter_list(list, count, n, [&](unsigned long long e) { return pair_key(e) >= from; });
+  if (int(count) <= most_left) return from;
+  sort_list(list, count, int(count), k);  // too many equal ones to tell apart by their keys
+  return pair_key(list[k - 1]);
 }
 
 // The bound as a float that a vector's maximum can be held against: !(maximum < it) where an element may enter.
@@ -236,13 +219,14 @@ __device__ __forceinline__ float bound_value(unsigned long long bound) {
   return bound <= 0xffffffffull ? key_to_float(uint32_t(bound)) : __uint_as_float(0x7fc00000u);
 }
 
-// Vectors [v0, v1) of the row into the list, which then holds this part's k largest among its entries (all of
-// them if there are fewer than k). kSum: the thread's share of sum_j 2^(l_j * log2_scale - ref) goes to (ref, sum).
+// Vectors [v0, v1) of the row into the list, which then has the k first of them among its entries (all of them if there
+// are fewer than k). kSum: the thread's share of sum_j 2^(l_j * log2_scale - ref) goes to (ref, sum).
 template <typename T, bool kSum>
 __device__ void stream_top(TopShared& s, const RowVectors<T>& row, int v0, int v1, int k, float log2_scale, float& ref,
                            float& sum) {
   constexpr int kBatch = kTopThreads * kTopUnroll;
   const T* tag = nullptr;
+  const int limit = min(2 * k + 64, kTopFull);
   __syncthreads();
   if (threadIdx.x == 0) {
     s.count = 0;
@@ -289,7 +273,13 @@ __device__ void stream_top(TopShared& s, const RowVectors<T>& row, int v0, int v
 #pragma unroll
       for (int u = 0; u < kTopUnroll; ++u)
         key[u] = vb + u * kTopThreads + int(threadIdx.x) < v1 ? order_key(top[u]) : 0u;
-      const uint32_t from = bound_for(s, k, k / 4 + 4, 0u, 0xffffffffu, [&](uint32_t b) {
+      uint32_t least = 0xffffffffu, most = 0;
+#pragma unroll
+      for (int u = 0; u < kTopUnroll; ++u) {
+        least = min(least, key[u]);
+        most = max(most, key[u]);
+      }
+      const uint32_t from = bound_for(s, k, k / 4 + 4, least, most, [&](uint32_t b) {
         int c = 0;
 #pragma unroll
         for (int u = 0; u < kTopUnroll; ++u) c += key[u] >= b;
@@ -303,33 +293,79 @@ __device__ void stream_top(TopShared& s, const RowVectors<T>& row, int v0, int v
 #pragma unroll
     for (int u = 0; u < kTopUnroll; ++u) {
       const int v = vb + u * kTopThreads + int(threadIdx.x);
-      if (!(top[u] < bound) && v < v1) full |= enter_list(s, row, v, cur[u]);
-    }
-    if (__syncthreads_or(full)) {
-      if (s.count <= unsigned(kTopList)) {
-        cut_list(s, k);
-      } else {
-        // more than the list holds: what was there before this batch, then the batch vector by vector
-        // (of the entries of earlier batches none was lost: they had their places before this batch began)
-        const int before = row.first_of(vb);  // the batch's first element
-        filter_list(s, kTopList, [&](unsigned long long e) { return before > 0 && pair_index(e) < uint32_t(before); });
-#pragma unroll
-        for (int u = 0; u < kTopUnroll; ++u) {
-          const int v = vb + u * kTopThreads + int(threadIdx.x);
-          if (v < v1) enter_list(s, row, v, cur[u]);
-          __syncthreads();
-          const bool cut = s.count > unsigned(kTopFull);
-          __syncthreads();
-          if (cut) cut_list(s, k);
+      if (!(top[u] < bound) && v < v1) {
+        const uint32_t key = order_key(top[u]);
+        if (key >= s.bound) {
+          const unsigned int at = atomicAdd(&s.count, 1u);
+          s.list[at] = order_pair(key, uint32_t(v));
+          full |= at >= unsigned(limit);
         }
       }
-      bound = bound_value(s.bound);
+    }
+    if (__syncthreads_or(full)) {
+      const uint32_t from = cut_list(s, s.list, s.count, k, limit);
+      if (threadIdx.x == 0) s.bound = (unsigned long long)from + 1;
       __syncthreads();
+      bound = bound_value(s.bound);
     }
 #pragma unroll
     for (int u = 0; u < kTopUnroll; ++u) cur[u] = nxt[u];
   }
   __syncthreads();
+}
+
+// The list's vectors read again: s.elements then holds the k first logits of the row (all of them if there are fewer),
+// sorted, s.n_elements of them.
+template <typename T>
+__device__ __forceinline__ void rank_elements(TopShared& s, const RowVectors<T>& row, int k) {
+  __syncthreads();
+  const int n = int(s.count);
+  if (threadIdx.x == 0) {
+    s.n_elements = 0;
+    s.range[0] = 0xffffffffu;
+  }
+  __syncthreads();
+  uint32_t least = 0xffffffffu;
+  for (int i = threadIdx.x; i < n; i += kTopThreads) least = min(least, pair_key(s.list[i]));
+  least = __reduce_min_sync(0xffffffffu, least);
+  if ((threadIdx.x & 31) == 0) atomicMin(&s.range[0], least);
+  __syncthreads();
+  uint32_t from = n >= k ? s.range[0] : 0u;  // n logits reach it
+  constexpr int kStep = kTopMax / RowVectors<T>::kPer;  // vectors at a time: their logits fit beside what is kept
+  static_assert(kStep <= kTopThreads, "one vector per thread");
+  int m = 0;
+  for (int i0 = 0; i0 < n; i0 += kStep) {
+    const int i = i0 + int(threadIdx.x);
+    if (int(threadIdx.x) < kStep && i < n) {
+      const int v = int(pair_index(s.list[i]));
+      const int e = row.first_of(v);
+      float f[RowVectors<T>::kPer];
+      unpack(row.load(v), f, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int j = 0; j < RowVectors<T>::kPer; ++j) {
+        const uint32_t key = order_key(f[j]);
+        if (key >= from && e + j >= 0 && uint32_t(e + j) < row.vocab)
+          s.elements[atomicAdd(&s.n_elements, 1u)] = order_pair(key, uint32_t(e + j));
+      }
+    }
+    __syncthreads();
+    m = int(s.n_elements);
+    __syncthreads();
+    if (i0 + kStep < n && m > kTopMax) from = cut_list(s, s.elements, s.n_elements, k, kTopMax);
+  }
+  if (m <= kTopThreads) {
+    // few: every entry's place is the number of entries ahead of it
+    __syncthreads();
+    const unsigned long long mine = int(threadIdx.x) < m ? s.elements[threadIdx.x] : 0;
+    int place = 0;
+    for (int i = 0; i < m; ++i) place += s.elements[i] > mine;
+    __syncthreads();
+    if (int(threadIdx.x) < m) s.elements[place] = mine;
+    if (threadIdx.x == 0) s.n_elements = min(m, k);
+    __syncthreads();
+  } else {
+    sort_list(s.elements, s.n_elements, m, k);
+  }
 }
 
 }  // namespace lce

@@ -8,12 +8,11 @@
 
 namespace lce {
 
-// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then holds the row's k first
-// entries, sorted. k * parts <= kTopList. The other blocks return with their part done.
+// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then has the row's k first vectors
+// among its entries. k * parts <= kTopList. The other blocks return with their part done.
 __device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
-  thin_list(s, k);
   if (parts > 1) {
-    if (s.count > unsigned(kTopList / parts)) sort_list(s, k);  // many equal logits: exactly k
+    if (s.count > unsigned(kTopList / parts)) cut_list(s, s.list, s.count, k, kTopList / parts);
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     cluster.sync();
     if (cluster.block_rank() == 0) {
@@ -40,9 +39,9 @@ __device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
     }
     cluster.sync();
     if (cluster.block_rank() != 0) return;
-    thin_list(s, k);
   }
-  sort_list(s, k);
+  __syncthreads();
+  if (s.count > unsigned(k + k / 4 + 32)) cut_list(s, s.list, s.count, k, min(2 * k + 64, kTopFull));
 }
 
 template <typename T>
@@ -66,15 +65,16 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   }
   merge_lists(s, k, parts);
   if (part != 0) return;
+  rank_elements(s, row, k);
   for (int i = threadIdx.x; i < k; i += kTopThreads) {
-    const unsigned long long e = s.list[i];
+    const unsigned long long e = s.elements[i];
     values[r * k + i] = T(key_to_float(pair_key(e)));
     indices[r * k + i] = pair_index(e);
   }
   if (threadIdx.x == 0) {
     // The sum is over 2^(l * log2_scale), whose exponents are right to the rounding of log2_scale; at the largest
     // logit, which carries the sum, that rounding is put back.
-    const uint32_t first = pair_key(s.list[0]);
+    const uint32_t first = pair_key(s.elements[0]);
     const double largest = double(key_to_float(first));
     const double put_back = largest * (double(inv_temperature) - double(log2_scale) * 0.69314718055994531);
     float v = float((double(s.part_ref) + double(log2f(s.part_sum))) * 0.69314718055994531 + put_back);
