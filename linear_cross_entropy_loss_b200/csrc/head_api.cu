@@ -57,7 +57,7 @@ int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size
 // keeps a whole batch, and the lists of all parts fit one.
 template <typename T>
 int top_parts(int64_t rows, int64_t vocab, int k) {
-  const int64_t batch = (int64_t)kTopThreads * kTopUnroll * (16 / (int)sizeof(T));
+  const int64_t batch = (int64_t)kTopBatch * (32 / (int)sizeof(T));
   int parts = 1;
   while (parts < 8 && rows * parts * 2 <= 4ll * sm_count() && vocab >= batch * parts && k * parts * 2 <= kTopList) parts *= 2;
   return parts;

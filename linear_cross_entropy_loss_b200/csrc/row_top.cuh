@@ -1,17 +1,20 @@
 // The k largest logits of a row, found while the row streams past once.
 //
-// The row is looked at in vectors of 16 bytes (4 or 8 logits). A list in shared memory keeps the vectors that come first
-// by (largest logit descending, place ascending): the k first of them hold the k first logits, since a vector ahead of
-// another has a logit ahead of all of its. So the streaming loop handles one number per vector: one comparison of its
-// maximum with the bound of the list, and what enters is one entry, however its logits lie. At the end the k vectors are
-// read again and their logits ranked.
+// The row is looked at in groups of 32 bytes (8 or 16 logits). The k groups that come first by (largest logit descending,
+// place ascending) hold the k first logits, since a group ahead of another has a logit ahead of all of its. So only the groups'
+// maxima are kept, and the search works on them:
 //
-// * Vectors come in batches of kTopThreads * kTopUnroll, the next batch on its way while one is looked at.
-// * The first bound comes from the first batch: the k-th largest of its maxima.
-// * A list that holds twice what is wanted is cut back and the bound raised behind its last entry, so of a row of random
-//   order about k (1 + ln(batches)) vectors enter. An equal maximum that comes later is behind: after a cut only larger ones enter.
-// * Between two batches the list holds at most kTopFull entries, so a batch always fits.
-// A row may be split over the blocks of a cluster; the first block then takes the others' lists.
+// 1. Stream: each thread loads two groups at a time, the next two on their way; a group's maximum goes to shared memory,
+//    and four running maxima of the thread's groups stay in registers. No barrier, nothing that depends on the data.
+// 2. Bound: the k-th largest of the block's 1024 running maxima. At least k groups reach it, and of a row of random order
+//    about k (1 + k / 2048) do.
+// 3. Collect: the groups that reach the bound go to a list. If it runs full (rows in an unlucky order, many equal
+//    logits, several segments) it is cut back to its first k and the bound raised behind the last of them: an equal maximum that
+//    comes later is behind.
+// 4. Rank: the logits of the listed groups are read again and those that reach the bound sorted.
+//
+// A row with more groups than the shared array takes goes through 1 to 3 in segments. A row may also be split over
+// the blocks of a cluster; the first block then takes the others' lists.
 #pragma once
 
 #include "ptx.cuh"
@@ -23,16 +26,23 @@ namespace lce {
 
 constexpr int kTopMax = 1024;
 constexpr int kTopThreads = 256;
-constexpr int kTopUnroll = 4;
-constexpr int kTopList = 2048;             // vectors in the list
-constexpr int kTopFull = kTopList - kTopThreads * kTopUnroll;
-constexpr int kTopElements = 2 * kTopMax;  // logits of the last step: what is kept, and as many from the next vectors
-static_assert(kTopFull >= kTopMax, "the list keeps k vectors and takes a batch");
+constexpr int kTopUnroll = 2;                              // groups a thread loads at a time
+constexpr int kTopBatch = kTopThreads * kTopUnroll;
+constexpr int kTopChunk = 4 * kTopThreads;                 // groups looked at between two cuts of the list
+constexpr int kTopSegmentBytes = 16384;                    // shared array of the maxima
+constexpr int kTopList = 2048;                             // groups in the list
+constexpr int kTopFull = kTopList - kTopChunk;             // most of them before a chunk: the chunk fits
+constexpr int kTopElements = 2 * kTopMax;                  // logits of the last step: what is kept, and as many more
+constexpr int kSearchSteps = 33;  // of bound_for: a step leaves a fifth of the range, or one key less
+static_assert(kTopFull >= kTopMax, "the list keeps k groups and takes a chunk");
 
 struct TopShared {
-  unsigned long long list[kTopList];         // order_pair(largest logit, vector)
-  unsigned long long elements[kTopElements]; // order_pair(logit, index)
-  unsigned int counters[34];
+  unsigned long long list[kTopList];         // order_pair(largest logit, group)
+  union {
+    unsigned long long elements[kTopElements]; // order_pair(logit, index); after the last segment
+    uint4 maxima[kTopSegmentBytes / 16];       // the segment's groups: their maxima in the type of the logits
+  };
+  unsigned int counters[2 * kSearchSteps + 1];
   unsigned int range[2];
   unsigned int count;        // entries of `list`
   unsigned int n_elements;   // entries of `elements`
@@ -41,47 +51,78 @@ struct TopShared {
   float part_ref, part_sum;  // log-sum-exp of this block's part
 };
 
-// Streaming 16-byte load of data that is read once.
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+struct Group {
+  uint32_t w[8];
+};
+// Streaming 32-byte load of data that is read once.
+__device__ __forceinline__ Group load_stream(const void* p) {
+  Group g;
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(g.w[0]), "=r"(g.w[1]), "=r"(g.w[2]), "=r"(g.w[3]), "=r"(g.w[4]), "=r"(g.w[5]), "=r"(g.w[6]),
+                 "=r"(g.w[7])
                : "l"(p));
-  return v;
+  return g;
 }
 
-// A row as 16-byte vectors on 16-byte boundaries. Vector v holds the elements v * kPer - lead + 0 .. kPer - 1; those
-// outside the row (before its first or after its last vector's end) read as -inf.
+// Two floats in one 64-bit register: half the instructions for the arithmetic around the exponentials.
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(unsigned long long v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// A row as 32-byte groups on 32-byte boundaries. Group v holds the elements v * kPer - lead + 0 .. kPer - 1; those
+// outside the row (before its first or after its last element) read as -inf.
 template <typename T>
-struct RowVectors {
-  static constexpr int kPer = 16 / int(sizeof(T));
+struct RowGroups {
+  static constexpr int kPer = 32 / int(sizeof(T));
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, unsigned short>;
+  static constexpr uint32_t kNegInf =
+      sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00u : 0xff80u);
   const T* row;
   uint32_t vocab;
   int lead;
-  int vectors;
-  __device__ __forceinline__ RowVectors(const T* row_, uint32_t vocab_) : row(row_), vocab(vocab_) {
-    lead = int((reinterpret_cast<uintptr_t>(row_) & 15u) / sizeof(T));
-    vectors = int((vocab + uint32_t(lead) + kPer - 1) / kPer);
+  int groups;
+  __device__ __forceinline__ RowGroups(const T* row_, uint32_t vocab_) : row(row_), vocab(vocab_) {
+    lead = int((reinterpret_cast<uintptr_t>(row_) & 31u) / sizeof(T));
+    groups = int((vocab + uint32_t(lead) + kPer - 1) / kPer);
   }
   __device__ __forceinline__ int first_of(int v) const { return v * kPer - lead; }
-  __device__ __forceinline__ uint4 load(int v) const {
+  // Whether the groups a .. b - 1 lie inside the row, and where group 0 would begin.
+  __device__ __forceinline__ bool whole(int a, int b) const {
+    return first_of(a) >= 0 && (long long)b * kPer - lead <= (long long)vocab;
+  }
+  __device__ __forceinline__ const char* base() const { return reinterpret_cast<const char*>(row - lead); }
+  __device__ __forceinline__ bool exists(int e) const { return e >= 0 && uint32_t(e) < vocab; }
+  __device__ __forceinline__ Group load(int v) const {
     const int e = first_of(v);
     if (e >= 0 && uint32_t(e + kPer) <= vocab) return load_stream(row + e);
-    using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, unsigned short>;
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    Group g = {};
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const bool exists = e + i >= 0 && uint32_t(e + i) < vocab;
-      const uint32_t b = exists ? uint32_t(reinterpret_cast<const Bits*>(row)[e + i]) : kNegInf;
-      w[i * int(sizeof(T)) / 4] |= b << (8 * (i * int(sizeof(T)) % 4));
+      const uint32_t b = exists(e + i) ? uint32_t(reinterpret_cast<const Bits*>(row)[e + i]) : kNegInf;
+      g.w[i * int(sizeof(T)) / 4] |= b << (8 * (i * int(sizeof(T)) % 4));
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return g;
   }
-  static constexpr uint32_t kNegInf =
-      sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00u : 0xff80u);
-  static __device__ __forceinline__ uint4 nothing() {
-    constexpr uint32_t b = sizeof(T) == 4 ? kNegInf : kNegInf * 0x10001u;
-    return make_uint4(b, b, b, b);
+  static __device__ __forceinline__ Group nothing() {
+    Group g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g.w[i] = sizeof(T) == 4 ? kNegInf : kNegInf * 0x10001u;
+    return g;
   }
 };
 
@@ -90,48 +131,66 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// The elements of a vector as floats, and the largest of them (NaN if one is).
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[4], const float*) {
-  f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+// The two elements of a 16-bit type in one word.
+__device__ __forceinline__ void halves(uint32_t w, float& a, float& b, const __nv_bfloat16*) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], const __nv_bfloat16*) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void halves(uint32_t w, float& a, float& b, const __half*) {
+  const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  a = t.x;
+  b = t.y;
+}
+// The largest of a group (NaN if one is).
+__device__ __forceinline__ float largest(const Group& g, const float*) {
+  float m = __uint_as_float(g.w[0]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 1; i < 8; ++i) m = max_nan(m, __uint_as_float(g.w[i]));
+  return m;
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], const __half*) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+template <typename T2, typename T>
+__device__ __forceinline__ float largest_of_pairs(const Group& g, const T* tag) {
+  const T2* h = reinterpret_cast<const T2*>(g.w);
+  const T2 m = __hmax2_nan(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])),
+                           __hmax2_nan(__hmax2_nan(h[4], h[5]), __hmax2_nan(h[6], h[7])));
+  float a, b;
+  halves(*reinterpret_cast<const uint32_t*>(&m), a, b, tag);
+  return max_nan(a, b);
+}
+__device__ __forceinline__ float largest(const Group& g, const __nv_bfloat16* t) {
+  return largest_of_pairs<__nv_bfloat162>(g, t);
+}
+__device__ __forceinline__ float largest(const Group& g, const __half* t) { return largest_of_pairs<__half2>(g, t); }
+
+// sum_j 2^(l_j * scale + minus) of a group, added to two sums.
+template <typename T>
+__device__ __forceinline__ unsigned long long add_exponentials(unsigned long long sum2, const Group& g,
+                                                               unsigned long long scale2, unsigned long long minus2,
+                                                               const T* tag) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
+  for (int i = 0; i < 8; ++i) {
+    float a, b;
+    if constexpr (sizeof(T) == 4) {
+      if (i & 1) continue;
+      a = __uint_as_float(g.w[i]);
+      b = __uint_as_float(g.w[i + 1]);
+    } else {
+      halves(g.w[i], a, b, tag);
+    }
+    unpack2(fma2(pack2(a, b), scale2, minus2), a, b);
+    sum2 = add2(sum2, pack2(fast_exp2(a), fast_exp2(b)));
   }
-}
-__device__ __forceinline__ float largest(const uint4& v, const float*) {
-  return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
-}
-__device__ __forceinline__ float largest(const uint4& v, const __nv_bfloat16*) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-  return max_nan(__low2float(m), __high2float(m));
-}
-__device__ __forceinline__ float largest(const uint4& v, const __half*) {
-  const __half2* h = reinterpret_cast<const __half2*>(&v);
-  const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-  return max_nan(__low2float(m), __high2float(m));
+  return sum2;
 }
 
-// A key that at least k of the block's entries reach, and (unless many are equal) at most k + slack. Bisection of the
-// range of the keys; every step is one count over the block. least / most: over this thread's entries; count_from(key):
-// how many of this thread's entries are >= key. With fewer than k entries: 0.
+// A key that at least k of the block's entries reach, and (unless many are equal) at most k + slack. The range of the keys
+// is cut into five parts at a time (a step costs a barrier and a trip through shared memory, whatever it counts).
+// least / most: over this thread's entries; count_from(key): how many of this thread's entries are >= key. With
+// fewer than k entries: 0.
 template <typename CountFrom>
 __device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, uint32_t least, uint32_t most,
                                               CountFrom count_from) {
-  if (threadIdx.x < 34) s.counters[threadIdx.x] = 0;
+  if (threadIdx.x < 2 * kSearchSteps + 1) s.counters[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
     s.range[0] = 0xffffffffu;
     s.range[1] = 0;
@@ -139,28 +198,45 @@ __device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, ui
   __syncthreads();
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
+  const unsigned int all = __reduce_add_sync(0xffffffffu, (unsigned int)count_from(0u));
   if ((threadIdx.x & 31) == 0) {
     atomicMin(&s.range[0], least);
     atomicMax(&s.range[1], most);
+    atomicAdd(&s.counters[2 * kSearchSteps], all);
   }
-  const unsigned int all = __reduce_add_sync(0xffffffffu, (unsigned int)count_from(0u));
-  if ((threadIdx.x & 31) == 0) atomicAdd(&s.counters[33], all);
   __syncthreads();
-  if (int(s.counters[33]) < k) return 0u;
+  if (int(s.counters[2 * kSearchSteps]) < k) return 0u;
   uint32_t lo = s.range[0];                                      // k or more from here on
   unsigned long long above = (unsigned long long)s.range[1] + 1;  // fewer than k from here on
   for (int step = 0; above - lo > 1; ++step) {
-    const uint32_t mid = uint32_t(lo + (above - lo) / 2);
-    const unsigned int mine = __reduce_add_sync(0xffffffffu, (unsigned int)count_from(mid));
-    if ((threadIdx.x & 31) == 0 && mine != 0) atomicAdd(&s.counters[step], mine);
-    __syncthreads();
-    const int total = int(s.counters[step]);
-    if (total >= k) {
-      lo = mid;
-      if (total <= k + slack) break;
-    } else {
-      above = mid;
+    const unsigned long long width = above - lo;
+    uint32_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = uint32_t(lo + width * (i + 1) / 5);
+    // two counts in a word: none is above 2^16
+    unsigned int low = (unsigned int)count_from(at[0]) | (unsigned int)count_from(at[1]) << 16;
+    unsigned int high = (unsigned int)count_from(at[2]) | (unsigned int)count_from(at[3]) << 16;
+    low = __reduce_add_sync(0xffffffffu, low);
+    high = __reduce_add_sync(0xffffffffu, high);
+    if ((threadIdx.x & 31) == 0) {
+      atomicAdd(&s.counters[2 * step], low);
+      if (high != 0) atomicAdd(&s.counters[2 * step + 1], high);
     }
+    __syncthreads();
+    low = s.counters[2 * step];
+    high = s.counters[2 * step + 1];
+    const int total[4] = {int(low & 0xffffu), int(low >> 16), int(high & 0xffffu), int(high >> 16)};
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (total[i] >= k) {
+        if (at[i] > lo) lo = at[i];
+        near = total[i] <= k + slack;
+      } else if (at[i] < above) {
+        above = at[i];
+      }
+    }
+    if (near) break;
   }
   return lo;
 }
@@ -219,105 +295,142 @@ __device__ __forceinline__ float bound_value(unsigned long long bound) {
   return bound <= 0xffffffffull ? key_to_float(uint32_t(bound)) : __uint_as_float(0x7fc00000u);
 }
 
-// Vectors [v0, v1) of the row into the list, which then has the k first of them among its entries (all of them if there
+// Groups [v0, v1) of the row into the list, which then has the k first of them among its entries (all of them if there
 // are fewer than k). kSum: the thread's share of sum_j 2^(l_j * log2_scale - ref) goes to (ref, sum).
 template <typename T, bool kSum>
-__device__ void stream_top(TopShared& s, const RowVectors<T>& row, int v0, int v1, int k, float log2_scale, float& ref,
-                           float& sum) {
-  constexpr int kBatch = kTopThreads * kTopUnroll;
+__device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row, int v0, int v1, int k, float log2_scale,
+                                           float& ref, float& sum) {
+  constexpr int kSegment = kTopSegmentBytes / int(sizeof(T));  // groups
+  static_assert(kSegment % kTopChunk == 0 && kSegment % (2 * kTopBatch) == 0, "segments are whole chunks");
   const T* tag = nullptr;
   const int limit = min(2 * k + 64, kTopFull);
+  T* const maxima = reinterpret_cast<T*>(s.maxima);
   __syncthreads();
   if (threadIdx.x == 0) {
     s.count = 0;
     s.bound = 0;
   }
-  uint4 cur[kTopUnroll], nxt[kTopUnroll];
-  auto fetch = [&](int vb, uint4(&to)[kTopUnroll]) {
+  auto fetch = [&](int vb, Group(&to)[kTopUnroll]) {
+    if (row.whole(vb, vb + kTopBatch) && vb + kTopBatch <= v1) {
+      const char* at = row.base() + ((long long)vb + int(threadIdx.x)) * 32;
 #pragma unroll
-    for (int u = 0; u < kTopUnroll; ++u) {
-      const int v = vb + u * kTopThreads + int(threadIdx.x);
-      to[u] = v < v1 ? row.load(v) : RowVectors<T>::nothing();
+      for (int u = 0; u < kTopUnroll; ++u) to[u] = load_stream(at + u * kTopThreads * 32);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kTopUnroll; ++u) {
+        const int v = vb + u * kTopThreads + int(threadIdx.x);
+        to[u] = v < v1 ? row.load(v) : RowGroups<T>::nothing();
+      }
     }
   };
   ref = -INFINITY;
   sum = 0.f;
+  Group cur[kTopUnroll], nxt[kTopUnroll];
   fetch(v0, cur);
-  __syncthreads();
-  float bound = -INFINITY;
-  for (int vb = v0; vb < v1; vb += kBatch) {
-    if (vb + kBatch < v1) fetch(vb + kBatch, nxt);
-    float top[kTopUnroll];
+  for (int seg = v0; seg < v1; seg += kSegment) {
+    const int end = min(seg + kSegment, v1);
+    float run[2 * kTopUnroll];
 #pragma unroll
-    for (int u = 0; u < kTopUnroll; ++u) top[u] = largest(cur[u], tag);
-    if (kSum) {
-      float m = ref;
-#pragma unroll
-      for (int u = 0; u < kTopUnroll; ++u) m = fmaxf(m, top[u] * log2_scale);  // passes a NaN over
-      if (m > ref) {
-        sum *= fast_exp2(ref - m);
-        ref = m;
-      }
-      const float minus = ref > -INFINITY ? -ref : 0.f;
+    for (int i = 0; i < 2 * kTopUnroll; ++i) run[i] = -INFINITY;
+    auto take = [&](int vb, const Group(&g)[kTopUnroll], float* most) {
+      float top[kTopUnroll];
 #pragma unroll
       for (int u = 0; u < kTopUnroll; ++u) {
-        float f[RowVectors<T>::kPer];
-        unpack(cur[u], f, tag);
-#pragma unroll
-        for (int i = 0; i < RowVectors<T>::kPer; ++i) sum += fast_exp2(fmaf(f[i], log2_scale, minus));
+        top[u] = largest(g[u], tag);
+        maxima[vb - seg + u * kTopThreads + int(threadIdx.x)] = T(top[u]);
+        most[u] = max_nan(most[u], top[u]);
       }
+      if (kSum) {
+        float m = ref;
+#pragma unroll
+        for (int u = 0; u < kTopUnroll; ++u) m = fmaxf(m, top[u] * log2_scale);  // passes a NaN over
+        if (m > ref) {
+          sum *= fast_exp2(ref - m);
+          ref = m;
+        }
+        const float minus = ref > -INFINITY ? -ref : 0.f;
+        const unsigned long long scale2 = pack2(log2_scale, log2_scale), minus2 = pack2(minus, minus);
+        unsigned long long sum2 = 0;
+#pragma unroll
+        for (int u = 0; u < kTopUnroll; ++u) sum2 = add_exponentials(sum2, g[u], scale2, minus2, tag);
+        float even, odd;
+        unpack2(sum2, even, odd);
+        sum += even + odd;
+      }
+    };
+    for (int vb = seg; vb < end; vb += 2 * kTopBatch) {
+      if (vb + kTopBatch < v1) fetch(vb + kTopBatch, nxt);
+      take(vb, cur, run);
+      if (vb + 2 * kTopBatch < v1) fetch(vb + 2 * kTopBatch, cur);
+      if (vb + kTopBatch < end) take(vb + kTopBatch, nxt, run + kTopUnroll);
     }
-    if (vb == v0 && v1 - v0 > kTopThreads && k <= kTopThreads * kTopUnroll / 2) {
-      // the k-th largest of the vectors' maxima (vectors that do not exist count as nothing)
-      uint32_t key[kTopUnroll];
+    __syncthreads();
+    // the first bound; with more wanted than half the running maxima they say too little, and the groups' own are searched
+    uint32_t from;
+    if (k <= kTopThreads * kTopUnroll) {
+      uint32_t key[2 * kTopUnroll], least = 0xffffffffu, most = 0;
 #pragma unroll
-      for (int u = 0; u < kTopUnroll; ++u)
-        key[u] = vb + u * kTopThreads + int(threadIdx.x) < v1 ? order_key(top[u]) : 0u;
-      uint32_t least = 0xffffffffu, most = 0;
-#pragma unroll
-      for (int u = 0; u < kTopUnroll; ++u) {
-        least = min(least, key[u]);
-        most = max(most, key[u]);
+      for (int i = 0; i < 2 * kTopUnroll; ++i) {
+        key[i] = seg + i * kTopThreads + int(threadIdx.x) < end ? order_key(run[i]) : 0u;  // 0: no group
+        least = min(least, key[i]);
+        most = max(most, key[i]);
       }
-      const uint32_t from = bound_for(s, k, k / 4 + 4, least, most, [&](uint32_t b) {
+      from = bound_for(s, k, k / 4 + 4, least, most, [&](uint32_t b) {
         int c = 0;
 #pragma unroll
-        for (int u = 0; u < kTopUnroll; ++u) c += key[u] >= b;
+        for (int i = 0; i < 2 * kTopUnroll; ++i) c += key[i] >= b;
         return c;
       });
-      if (threadIdx.x == 0) s.bound = from;
-      __syncthreads();
-      bound = bound_value(from);
+    } else {
+      uint32_t least = 0xffffffffu, most = 0;
+      for (int i = threadIdx.x; i < end - seg; i += kTopThreads) {
+        const uint32_t key = order_key(logit_to_float(maxima[i]));
+        least = min(least, key);
+        most = max(most, key);
+      }
+      from = bound_for(s, k, 64, least, most, [&](uint32_t b) {
+        int c = 0;
+        for (int i = threadIdx.x; i < end - seg; i += kTopThreads) c += order_key(logit_to_float(maxima[i])) >= b;
+        return c;
+      });
     }
-    bool full = false;
+    if (threadIdx.x == 0) s.bound = max(s.bound, (unsigned long long)from);
+    __syncthreads();
+    float bound = bound_value(s.bound);
+    for (int c = seg; c < end; c += kTopChunk) {
+      bool full = false;
+      T four[4];
+      const int at = c - seg + 4 * int(threadIdx.x);
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(four) = reinterpret_cast<const uint4*>(maxima)[at / 4];
+      else *reinterpret_cast<uint2*>(four) = reinterpret_cast<const uint2*>(maxima)[at / 4];
 #pragma unroll
-    for (int u = 0; u < kTopUnroll; ++u) {
-      const int v = vb + u * kTopThreads + int(threadIdx.x);
-      if (!(top[u] < bound) && v < v1) {
-        const uint32_t key = order_key(top[u]);
-        if (key >= s.bound) {
-          const unsigned int at = atomicAdd(&s.count, 1u);
-          s.list[at] = order_pair(key, uint32_t(v));
-          full |= at >= unsigned(limit);
+      for (int i = 0; i < 4; ++i) {
+        const float top = logit_to_float(four[i]);
+        if (!(top < bound) && seg + at + i < end) {
+          const uint32_t key = order_key(top);
+          if (key >= s.bound) {
+            const unsigned int place = atomicAdd(&s.count, 1u);
+            s.list[place] = order_pair(key, uint32_t(seg + at + i));
+            full |= place >= unsigned(limit);
+          }
         }
       }
+      if (__syncthreads_or(full)) {
+        const uint32_t least = cut_list(s, s.list, s.count, k, limit);
+        if (threadIdx.x == 0) s.bound = (unsigned long long)least + 1;
+        __syncthreads();
+        bound = bound_value(s.bound);
+      }
     }
-    if (__syncthreads_or(full)) {
-      const uint32_t from = cut_list(s, s.list, s.count, k, limit);
-      if (threadIdx.x == 0) s.bound = (unsigned long long)from + 1;
-      __syncthreads();
-      bound = bound_value(s.bound);
-    }
-#pragma unroll
-    for (int u = 0; u < kTopUnroll; ++u) cur[u] = nxt[u];
   }
   __syncthreads();
 }
 
-// The list's vectors read again: s.elements then holds the k first logits of the row (all of them if there are fewer),
+// The listed groups' logits again: s.elements then holds the k first logits of the row (all of them if there are fewer),
 // sorted, s.n_elements of them.
 template <typename T>
-__device__ __forceinline__ void rank_elements(TopShared& s, const RowVectors<T>& row, int k) {
+__device__ __forceinline__ void rank_elements(TopShared& s, const RowGroups<T>& row, int k) {
+  constexpr int kPer = RowGroups<T>::kPer;
   __syncthreads();
   const int n = int(s.count);
   if (threadIdx.x == 0) {
@@ -331,31 +444,26 @@ __device__ __forceinline__ void rank_elements(TopShared& s, const RowVectors<T>&
   if ((threadIdx.x & 31) == 0) atomicMin(&s.range[0], least);
   __syncthreads();
   uint32_t from = n >= k ? s.range[0] : 0u;  // n logits reach it
-  constexpr int kStep = kTopMax / RowVectors<T>::kPer;  // vectors at a time: their logits fit beside what is kept
-  static_assert(kStep <= kTopThreads, "one vector per thread");
   int m = 0;
-  for (int i0 = 0; i0 < n; i0 += kStep) {
-    const int i = i0 + int(threadIdx.x);
-    if (int(threadIdx.x) < kStep && i < n) {
-      const int v = int(pair_index(s.list[i]));
-      const int e = row.first_of(v);
-      float f[RowVectors<T>::kPer];
-      unpack(row.load(v), f, static_cast<const T*>(nullptr));
+  for (int i0 = 0; i0 < n * kPer; i0 += kTopMax) {
 #pragma unroll
-      for (int j = 0; j < RowVectors<T>::kPer; ++j) {
-        const uint32_t key = order_key(f[j]);
-        if (key >= from && e + j >= 0 && uint32_t(e + j) < row.vocab)
-          s.elements[atomicAdd(&s.n_elements, 1u)] = order_pair(key, uint32_t(e + j));
+    for (int j = 0; j < kTopMax / kTopThreads; ++j) {
+      const int i = i0 + j * kTopThreads + int(threadIdx.x);
+      if (i < n * kPer) {
+        const int e = row.first_of(int(pair_index(s.list[i / kPer]))) + i % kPer;
+        if (row.exists(e)) {
+          const uint32_t key = order_key(logit_to_float(row.row[e]));
+          if (key >= from) s.elements[atomicAdd(&s.n_elements, 1u)] = order_pair(key, uint32_t(e));
+        }
       }
     }
     __syncthreads();
     m = int(s.n_elements);
     __syncthreads();
-    if (i0 + kStep < n && m > kTopMax) from = cut_list(s, s.elements, s.n_elements, k, kTopMax);
+    if (m > kTopMax && i0 + kTopMax < n * kPer) from = cut_list(s, s.elements, s.n_elements, k, kTopMax);
   }
   if (m <= kTopThreads) {
     // few: every entry's place is the number of entries ahead of it
-    __syncthreads();
     const unsigned long long mine = int(threadIdx.x) < m ? s.elements[threadIdx.x] : 0;
     int place = 0;
     for (int i = 0; i < m; ++i) place += s.elements[i] > mine;

@@ -8,7 +8,7 @@
 
 namespace lce {
 
-// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then has the row's k first vectors
+// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then has the row's k first groups
 // among its entries. k * parts <= kTopList. The other blocks return with their part done.
 __device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
   if (parts > 1) {
@@ -51,9 +51,9 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   __shared__ TopShared s;
   const long long r = blockIdx.x / parts;
   const int part = int(blockIdx.x % parts);
-  const RowVectors<T> row(logits + r * ld, vocab);
-  const int share = (row.vectors + parts - 1) / parts;
-  const int v0 = min(part * share, row.vectors), v1 = min(v0 + share, row.vectors);
+  const RowGroups<T> row(logits + r * ld, vocab);
+  const int share = (row.groups + parts - 1) / parts;
+  const int v0 = min(part * share, row.groups), v1 = min(v0 + share, row.groups);
   const float log2_scale = inv_temperature * 1.4426950408889634f;
   float ref, sum;
   stream_top<T, true>(s, row, v0, v1, k, log2_scale, ref, sum);
