@@ -3,6 +3,8 @@
 #include "sample_logits.cuh"
 #include "top_logits.cuh"
 
+#include <algorithm>
+
 namespace {
 
 using namespace lce;
@@ -72,14 +74,64 @@ int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
                          reinterpret_cast<T*>(values), reinterpret_cast<long long*>(indices), lse);
 }
 
+// Blocks that share a row of sample_row_kernel, and the vectors of 16 bytes that each keeps in shared memory (0: too long a
+// row, it is read again for each sweep). A block keeps up to 64 KiB, so that two are on an SM; few rows are split further, down to 8 KiB; up
+// to 192 KiB where eight blocks are not enough.
+void row_layout(int64_t rows, int64_t vocab, int es, int* parts, int* cache_vectors) {
+  const int64_t bytes = vocab * es + 32;
+  int n = 1;
+  while (n < kRowParts && bytes > n * (64ll << 10)) n *= 2;
+  while (n < kRowParts && rows * n * 2 <= 2ll * sm_count() && bytes > n * (16ll << 10)) n *= 2;
+  const int64_t vectors = (bytes + 15) / 16;
+  const int64_t each = (vectors + n - 1) / n;
+  *parts = n;
+  *cache_vectors = each * 16 <= (192ll << 10) ? (int)each : 0;
+}
+
+// Dynamic shared memory above 48 KiB has to be allowed for each kernel, once per device.
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+  static std::atomic<uint64_t> done{0};  // one bit per device; one counter per kernel type
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return LCE_ERR_CUDA;
+  if (dev < 0 || dev >= 64) return LCE_ERR_UNSUPPORTED_DEVICE;
+  if ((done.load(std::memory_order_relaxed) >> dev) & 1u) return LCE_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return LCE_ERR_CUDA;
+  }
+  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return LCE_OK;
+}
+
 template <typename T>
-int launch_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, const SampleParams& p, int64_t* tokens,
+int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, SampleParams p, int64_t* tokens_,
                   float* logprobs, cudaStream_t st) {
-  int bits = kWeightBits;  // the sum over the row stays below 2^62
-  while (bits > 0 && (vocab << bits) > (1ll << 62)) --bits;
-  sample_logits_kernel<T><<<(int)rows, kSampleThreads, 0, st>>>(reinterpret_cast<const T*>(logits), ld, (uint32_t)vocab,
-                                                                bits, p, reinterpret_cast<long long*>(tokens), logprobs);
-  return check_launch();
+  const T* logits = reinterpret_cast<const T*>(logits_);
+  long long* tokens = reinterpret_cast<long long*>(tokens_);
+  p.weight_bits = kWeightBits;  // the sum over the row stays below 2^62
+  while (p.weight_bits > 0 && (vocab << p.weight_bits) > (1ll << 62)) --p.weight_bits;
+  // top_k for all rows: one of the two kernels has them all, but for greedy rows, which the list has. A top_k for each row: both run,
+  // and a cluster whose row is the other's ends at once.
+  const bool each = p.top_k != nullptr;
+  const int want = each ? 256 : (int)std::min<long long>(std::max<long long>(p.top_k_all, 1), kTopMax);
+  const int list_parts = top_parts<T>(rows, vocab, want);
+  p.list_limit = std::min(kTopMax, kTopList / list_parts);
+  const bool greedy = p.temperature != nullptr || !(p.temperature_all > 0.0);
+  const bool lists = each || greedy || (p.top_k_all >= 1 && p.top_k_all <= p.list_limit);
+  const bool others = each || ((p.temperature != nullptr || p.temperature_all > 0.0) &&
+                               !(p.top_k_all >= 1 && p.top_k_all <= p.list_limit));
+  int v;
+  if (lists && (v = launch_clusters(sample_list_kernel<T>, rows * list_parts, kTopThreads, 0, list_parts, st, logits,
+                                    (long long)ld, (uint32_t)vocab, list_parts, p, tokens, logprobs)) != LCE_OK)
+    return v;
+  if (!others) return LCE_OK;
+  int parts = 1, cache = 0;
+  row_layout(rows, vocab, (int)sizeof(T), &parts, &cache);
+  const size_t fixed = (sizeof(RowShared) + 15) / 16 * 16;
+  if ((v = allow_smem(sample_row_kernel<T>, fixed + (192u << 10))) != LCE_OK) return v;
+  return launch_clusters(sample_row_kernel<T>, rows * parts, kRowThreads, fixed + (size_t)cache * 16, parts, st, logits,
+                         (long long)ld, (uint32_t)vocab, parts, cache, p, tokens, logprobs);
 }
 
 }  // namespace
@@ -114,7 +166,7 @@ int lce_sample_logits(int32_t dtype, const void* logits, int64_t ld, int64_t row
   if (!s->min_p && !(s->min_p_all >= 0.0 && s->min_p_all <= 1.0)) return LCE_ERR_INVALID_ARGUMENT;
   if (rows == 0) return LCE_OK;
   if (!s->u || !tokens || !logprobs) return LCE_ERR_INVALID_ARGUMENT;
-  SampleParams p;
+  SampleParams p = {};
   p.u = s->u;
   p.u_is_double = s->u_dtype == LCE_SAMPLING_U_F64;
   p.temperature = s->temperature;

@@ -20,6 +20,7 @@
 #include "ptx.cuh"
 #include "vocab_row.cuh"
 
+#include <cooperative_groups.h>
 #include <type_traits>
 
 namespace lce {
@@ -131,6 +132,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// What a NaN is to the search: larger than everything (listing), or nothing, like -inf (drawing).
+enum class Nan { kFirst, kNever };
+template <Nan kNan>
+__device__ __forceinline__ uint32_t search_key(float f) {
+  return kNan == Nan::kNever && f != f ? kKeyNegInf : order_key(f);
+}
+template <Nan kNan>
+__device__ __forceinline__ float larger(float a, float b) {
+  return kNan == Nan::kFirst ? max_nan(a, b) : fmaxf(a, b);
+}
+
 // The two elements of a 16-bit type in one word.
 __device__ __forceinline__ void halves(uint32_t w, float& a, float& b, const __nv_bfloat16*) {
   a = __uint_as_float(w << 16);
@@ -141,26 +153,31 @@ __device__ __forceinline__ void halves(uint32_t w, float& a, float& b, const __h
   a = t.x;
   b = t.y;
 }
-// The largest of a group (NaN if one is).
+// The largest of a group (kFirst: NaN if one is).
+template <Nan kNan>
 __device__ __forceinline__ float largest(const Group& g, const float*) {
   float m = __uint_as_float(g.w[0]);
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, __uint_as_float(g.w[i]));
+  for (int i = 1; i < 8; ++i) m = larger<kNan>(m, __uint_as_float(g.w[i]));
   return m;
 }
-template <typename T2, typename T>
+template <Nan kNan, typename T2, typename T>
 __device__ __forceinline__ float largest_of_pairs(const Group& g, const T* tag) {
   const T2* h = reinterpret_cast<const T2*>(g.w);
-  const T2 m = __hmax2_nan(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])),
-                           __hmax2_nan(__hmax2_nan(h[4], h[5]), __hmax2_nan(h[6], h[7])));
+  auto two = [](T2 a, T2 b) { return kNan == Nan::kFirst ? __hmax2_nan(a, b) : __hmax2(a, b); };
+  const T2 m = two(two(two(h[0], h[1]), two(h[2], h[3])), two(two(h[4], h[5]), two(h[6], h[7])));
   float a, b;
   halves(*reinterpret_cast<const uint32_t*>(&m), a, b, tag);
-  return max_nan(a, b);
+  return larger<kNan>(a, b);
 }
+template <Nan kNan>
 __device__ __forceinline__ float largest(const Group& g, const __nv_bfloat16* t) {
-  return largest_of_pairs<__nv_bfloat162>(g, t);
+  return largest_of_pairs<kNan, __nv_bfloat162>(g, t);
 }
-__device__ __forceinline__ float largest(const Group& g, const __half* t) { return largest_of_pairs<__half2>(g, t); }
+template <Nan kNan>
+__device__ __forceinline__ float largest(const Group& g, const __half* t) {
+  return largest_of_pairs<kNan, __half2>(g, t);
+}
 
 // sum_j 2^(l_j * scale + minus) of a group, added to two sums.
 template <typename T>
@@ -297,7 +314,7 @@ __device__ __forceinline__ float bound_value(unsigned long long bound) {
 
 // Groups [v0, v1) of the row into the list, which then has the k first of them among its entries (all of them if there
 // are fewer than k). kSum: the thread's share of sum_j 2^(l_j * log2_scale - ref) goes to (ref, sum).
-template <typename T, bool kSum>
+template <typename T, bool kSum, Nan kNan>
 __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row, int v0, int v1, int k, float log2_scale,
                                            float& ref, float& sum) {
   constexpr int kSegment = kTopSegmentBytes / int(sizeof(T));  // groups
@@ -336,9 +353,9 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
       float top[kTopUnroll];
 #pragma unroll
       for (int u = 0; u < kTopUnroll; ++u) {
-        top[u] = largest(g[u], tag);
+        top[u] = largest<kNan>(g[u], tag);
         maxima[vb - seg + u * kTopThreads + int(threadIdx.x)] = T(top[u]);
-        most[u] = max_nan(most[u], top[u]);
+        most[u] = larger<kNan>(most[u], top[u]);
       }
       if (kSum) {
         float m = ref;
@@ -371,7 +388,7 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
       uint32_t key[2 * kTopUnroll], least = 0xffffffffu, most = 0;
 #pragma unroll
       for (int i = 0; i < 2 * kTopUnroll; ++i) {
-        key[i] = seg + i * kTopThreads + int(threadIdx.x) < end ? order_key(run[i]) : 0u;  // 0: no group
+        key[i] = seg + i * kTopThreads + int(threadIdx.x) < end ? search_key<kNan>(run[i]) : 0u;  // 0: no group
         least = min(least, key[i]);
         most = max(most, key[i]);
       }
@@ -384,13 +401,13 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
     } else {
       uint32_t least = 0xffffffffu, most = 0;
       for (int i = threadIdx.x; i < end - seg; i += kTopThreads) {
-        const uint32_t key = order_key(logit_to_float(maxima[i]));
+        const uint32_t key = search_key<kNan>(logit_to_float(maxima[i]));
         least = min(least, key);
         most = max(most, key);
       }
       from = bound_for(s, k, 64, least, most, [&](uint32_t b) {
         int c = 0;
-        for (int i = threadIdx.x; i < end - seg; i += kTopThreads) c += order_key(logit_to_float(maxima[i])) >= b;
+        for (int i = threadIdx.x; i < end - seg; i += kTopThreads) c += search_key<kNan>(logit_to_float(maxima[i])) >= b;
         return c;
       });
     }
@@ -407,7 +424,7 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
       for (int i = 0; i < 4; ++i) {
         const float top = logit_to_float(four[i]);
         if (!(top < bound) && seg + at + i < end) {
-          const uint32_t key = order_key(top);
+          const uint32_t key = search_key<kNan>(top);
           if (key >= s.bound) {
             const unsigned int place = atomicAdd(&s.count, 1u);
             s.list[place] = order_pair(key, uint32_t(seg + at + i));
@@ -426,9 +443,45 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
   __syncthreads();
 }
 
+// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then has the row's k first groups
+// among its entries. k * parts <= kTopList. The other blocks return with their part done.
+__device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
+  if (parts > 1) {
+    if (s.count > unsigned(kTopList / parts)) cut_list(s, s.list, s.count, k, kTopList / parts);
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    if (cluster.block_rank() == 0) {
+      unsigned int at = s.count;
+      for (int part = 1; part < parts; ++part) {
+        const TopShared* other = cluster.map_shared_rank(&s, part);
+        const unsigned int n = other->count;
+        for (unsigned int i = threadIdx.x; i < n; i += kTopThreads) s.list[at + i] = other->list[i];
+        at += n;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        s.count = at;
+        float m = s.part_ref;
+        for (int part = 1; part < parts; ++part) m = fmaxf(m, cluster.map_shared_rank(&s, part)->part_ref);
+        float sum = 0.f;
+        for (int part = 0; part < parts; ++part) {
+          const TopShared* other = cluster.map_shared_rank(&s, part);
+          if (other->part_ref > -INFINITY) sum += other->part_sum * fast_exp2(other->part_ref - m);
+        }
+        s.part_ref = m;
+        s.part_sum = sum;
+      }
+    }
+    cluster.sync();
+    if (cluster.block_rank() != 0) return;
+  }
+  __syncthreads();
+  if (s.count > unsigned(k + k / 4 + 32)) cut_list(s, s.list, s.count, k, min(2 * k + 64, kTopFull));
+}
+
 // The listed groups' logits again: s.elements then holds the k first logits of the row (all of them if there are fewer),
 // sorted, s.n_elements of them.
-template <typename T>
+template <Nan kNan, typename T>
 __device__ __forceinline__ void rank_elements(TopShared& s, const RowGroups<T>& row, int k) {
   constexpr int kPer = RowGroups<T>::kPer;
   __syncthreads();
@@ -452,7 +505,7 @@ __device__ __forceinline__ void rank_elements(TopShared& s, const RowGroups<T>& 
       if (i < n * kPer) {
         const int e = row.first_of(int(pair_index(s.list[i / kPer]))) + i % kPer;
         if (row.exists(e)) {
-          const uint32_t key = order_key(logit_to_float(row.row[e]));
+          const uint32_t key = search_key<kNan>(logit_to_float(row.row[e]));
           if (key >= from) s.elements[atomicAdd(&s.n_elements, 1u)] = order_pair(key, uint32_t(e));
         }
       }

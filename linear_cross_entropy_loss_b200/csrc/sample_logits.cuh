@@ -2,9 +2,13 @@
 //   w_j = exp((l_j - max) / T); order: logit descending, index ascending
 //   kept: the first top_k of the order; of those the shortest prefix that holds top_p of their mass; of those w >= min_p
 //   token = the first j in index order at which the kept weights, added up, exceed u * (their sum)
+//
+// Rows with a short list (top_k up to `list_limit`, or greedy) go through the search of top_logits and are drawn
+// from the sorted list (sample_list_kernel). All others keep the row in shared memory, spread over a cluster, and sweep over it
+// (sample_row_kernel): the largest logit; a histogram over the order for each cut; the kept weights; the place of the token.
 #pragma once
 
-#include "row_select.cuh"
+#include "row_top.cuh"
 
 namespace lce {
 
@@ -19,103 +23,660 @@ struct SampleParams {
   double top_p_all;
   double min_p_all;
   long long top_k_all;
+  int weight_bits;
+  int list_limit;            // rows with 1 <= top_k <= list_limit (greedy ones count as 1) go through the list
 };
 
-constexpr int kSampleThreads = 512;
-
-template <typename T>
-__global__ void __launch_bounds__(kSampleThreads)
-sample_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int weight_bits, const SampleParams p,
-                     long long* __restrict__ tokens, float* __restrict__ logprobs) {
-  __shared__ SelectScratch s;
-  __shared__ float scratch[32];
-  __shared__ double table[32];
-  const long long r = blockIdx.x;
-  const T* row = logits + r * ld;
-  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
-  float m = -INFINITY;
-  unsigned long long allowed = 0;
-  for (uint32_t j = threadIdx.x; j < vocab; j += blockDim.x) {
-    const float l = logit_to_float(row[j]);
-    m = fmaxf(m, l);  // a NaN is passed over
-    allowed += l > -INFINITY;
+// One row's settings, with whatever stands outside their range taken as the nearest that means something.
+struct RowSettings {
+  double temperature;
+  double top_p;   // >= 1: no cut
+  double lowest;  // least weight_steps of a kept token
+  double u;
+  long long top_k;  // 0: no cut
+  bool greedy;
+};
+__device__ __forceinline__ RowSettings row_settings(const SampleParams& p, long long r) {
+  RowSettings s;
+  s.temperature = p.temperature ? double(p.temperature[r]) : p.temperature_all;
+  s.top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+  s.top_p = p.top_p ? double(p.top_p[r]) : p.top_p_all;
+  const double min_p = p.min_p ? double(p.min_p[r]) : p.min_p_all;
+  s.lowest = min_p > 0.0 ? 32.0 * log2(fmin(min_p, 1.0)) : -INFINITY;
+  s.u = p.u_is_double ? reinterpret_cast<const double*>(p.u)[r] : double(reinterpret_cast<const float*>(p.u)[r]);
+  s.u = s.u > 0.0 ? fmin(s.u, 1.0) : 0.0;
+  s.greedy = !(s.temperature > 0.0);
+  if (s.greedy) {
+    s.temperature = 1.0;
+    s.top_k = 1;
   }
-  m = block_max(m, scratch);
-  allowed = block_sum(allowed, s.reduce);
-  if (!(m > -INFINITY)) {  // nothing may be drawn
-    if (threadIdx.x == 0) {
-      tokens[r] = -1;
-      logprobs[r] = -INFINITY;
-    }
+  if (s.top_k < 0) s.top_k = 0;
+  if (!(s.top_p < 1.0)) s.top_p = 1.0;
+  return s;
+}
+__device__ __forceinline__ bool by_list(const SampleParams& p, const RowSettings& s) {
+  return s.top_k >= 1 && s.top_k <= p.list_limit;
+}
+__device__ __forceinline__ RowWeights row_weights(const SampleParams& p, const RowSettings& s, float largest,
+                                                  const double* table) {
+  RowWeights w;
+  w.largest = largest;
+  w.only_largest = largest == INFINITY;
+  w.steps = fmin(46.166241308446828 / s.temperature, 1e300);  // 32 log2(e) / T
+  w.to_int = exp2(double(52 - p.weight_bits));
+  w.table = table;
+  return w;
+}
+// Smallest prefix whose mass reaches top_p of the whole.
+__device__ __forceinline__ unsigned long long mass_target(double top_p, unsigned long long mass) {
+  const double goal = ceil(fmax(top_p, 0.0) * double(mass));
+  const unsigned long long target = goal < 1.0 ? 1ull : (unsigned long long)goal;
+  return target < mass ? target : mass;
+}
+__device__ __forceinline__ unsigned long long draw_target(double u, unsigned long long total) {
+  const unsigned long long goal = (unsigned long long)(u * double(total));
+  return goal < total ? goal : total - 1;
+}
+__device__ __forceinline__ float log_share(const SampleParams& p, const RowSettings& s, const RowWeights& w, float logit,
+                                           unsigned long long weight, unsigned long long total) {
+  if (s.greedy) return 0.f;
+  if (w.only_largest) return float(log(double(weight) / double(total)));
+  return float(weight_steps(w, logit) * kStepLn2 - log(ldexp(double(total), -p.weight_bits)));
+}
+__device__ __forceinline__ void draw_nothing(long long r, long long* tokens, float* logprobs) {
+  tokens[r] = -1;
+  logprobs[r] = -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------
+// rows with a short list
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads, 4)
+sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int parts, const SampleParams p,
+                   long long* __restrict__ tokens, float* __restrict__ logprobs) {
+  __shared__ TopShared s;
+  __shared__ double table[32];
+  __shared__ unsigned long long reduce[32];
+  const long long r = blockIdx.x / parts;
+  const int part = int(blockIdx.x % parts);
+  const RowSettings set = row_settings(p, r);
+  if (!by_list(p, set)) return;  // the whole cluster
+  const int k = int(min((long long)vocab, set.top_k));
+  const RowGroups<T> row(logits + r * ld, vocab);
+  const int share = (row.groups + parts - 1) / parts;
+  const int v0 = min(part * share, row.groups), v1 = min(v0 + share, row.groups);
+  float ref, sum;
+  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  stream_top<T, false, Nan::kNever>(s, row, v0, v1, k, 1.f, ref, sum);
+  merge_lists(s, k, parts);
+  if (part != 0) return;
+  rank_elements<Nan::kNever>(s, row, k);
+
+  const int n = int(s.n_elements);
+  const uint32_t first = pair_key(s.elements[0]);
+  if (first == kKeyNegInf) {
+    if (threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
     return;
   }
-  double T_row = p.temperature ? double(p.temperature[r]) : p.temperature_all;
-  long long k = p.top_k ? p.top_k[r] : p.top_k_all;
-  const double top_p = p.top_p ? double(p.top_p[r]) : p.top_p_all;
-  const double min_p = p.min_p ? double(p.min_p[r]) : p.min_p_all;
-  double u = p.u_is_double ? reinterpret_cast<const double*>(p.u)[r] : double(reinterpret_cast<const float*>(p.u)[r]);
-  u = u > 0.0 ? u : 0.0;
-  if (!(T_row > 0.0)) {  // greedy
-    T_row = 1.0;
-    k = 1;
+  const RowWeights w = row_weights(p, set, key_to_float(first), table);
+  // thread t has the ranks 4 t .. 4 t + 3
+  constexpr int kEach = kTopMax / kTopThreads;
+  unsigned long long mine[kEach], sum4 = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int rank = kEach * int(threadIdx.x) + i;
+    mine[i] = rank < n ? row_weight(w, key_to_float(pair_key(s.elements[rank]))) : 0ull;
+    sum4 += mine[i];
   }
-  RowWeights w;
-  w.largest = m;
-  w.only_largest = m == INFINITY;
-  w.steps = fmin(46.166241308446828 / T_row, 1e300);  // 32 log2(e) / T
-  w.to_int = exp2(double(52 - weight_bits));
-  w.table = table;
-
-  auto weight = [&](float l) { return l > -INFINITY ? row_weight(w, l) : 0ull; };
-  RowCut cut = {0u, kNoIndexLimit};
-  if (k > 0 && (unsigned long long)k < allowed)
-    cut = find_cut(row, vocab, (unsigned long long)k, s,
-                   [](float l, uint32_t, uint32_t) { return l > -INFINITY ? 1ull : 0ull; });
-  if (top_p < 1.0) {
-    unsigned long long mass = 0;
-    for (uint32_t j = threadIdx.x; j < vocab; j += blockDim.x) {
-      const float l = logit_to_float(row[j]);
-      if (inside(cut, order_key(l), j)) mass += weight(l);
+  unsigned long long mass;
+  unsigned long long before = block_prefix(sum4, reduce, &mass);
+  const unsigned long long target = set.top_p < 1.0 ? mass_target(set.top_p, mass) : mass;
+  unsigned long long* weights = s.list;            // by rank; 0 where a token is not kept
+  unsigned long long* by_index = s.list + kTopMax;
+  sum4 = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int rank = kEach * int(threadIdx.x) + i;
+    bool keep = before < target;
+    if (rank < n && !w.only_largest)
+      keep = keep && weight_steps(w, key_to_float(pair_key(s.elements[rank]))) >= set.lowest;
+    before += mine[i];
+    if (!keep) mine[i] = 0;
+    weights[rank] = mine[i];
+    sum4 += mine[i];
+  }
+  const unsigned long long total = block_sum(sum4, reduce);
+  const unsigned long long goal = draw_target(set.u, total);
+  // the kept weights are a prefix of the ranks; in index order they are added up
+  int kept = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) kept += mine[i] != 0;
+  kept = int(block_sum((unsigned long long)kept, reduce));
+  if (kept <= kTopThreads) {
+    const int i = int(threadIdx.x);
+    if (i < kept) {
+      const uint32_t index = pair_index(s.elements[i]);
+      unsigned long long at = 0;
+      for (int j = 0; j < kept; ++j) at += pair_index(s.elements[j]) < index ? weights[j] : 0ull;
+      if (at <= goal && goal < at + weights[i]) {
+        tokens[r] = index;
+        logprobs[r] = log_share(p, set, w, key_to_float(pair_key(s.elements[i])), weights[i], total);
+      }
     }
-    mass = block_sum(mass, s.reduce);
-    const double goal = ceil(fmax(top_p, 0.0) * double(mass));
-    unsigned long long target = goal < 1.0 ? 1ull : (unsigned long long)goal;
-    if (target > mass) target = mass;
-    const RowCut outer = cut;
-    cut = find_cut(row, vocab, target, s,
-                   [&](float l, uint32_t key, uint32_t j) { return inside(outer, key, j) ? weight(l) : 0ull; });
+  } else {
+    for (int i = threadIdx.x; i < kTopMax; i += kTopThreads)
+      by_index[i] = i < kept ? order_pair(0xffffffffu - pair_index(s.elements[i]), uint32_t(i)) : 0ull;
+    block_sort_descending(by_index, kTopMax);
+    sum4 = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = kEach * int(threadIdx.x) + i;
+      mine[i] = at < kept ? weights[pair_index(by_index[at])] : 0ull;
+      sum4 += mine[i];
+    }
+    before = block_prefix(sum4, reduce, &mass);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (mine[i] != 0 && before <= goal && goal < before + mine[i]) {
+        const unsigned long long e = s.elements[pair_index(by_index[kEach * int(threadIdx.x) + i])];
+        tokens[r] = pair_index(e);
+        logprobs[r] = log_share(p, set, w, key_to_float(pair_key(e)), mine[i], total);
+      }
+      before += mine[i];
+    }
   }
-  // (l - max) / T >= log(min_p), in the steps of the weights
-  const double lowest = min_p > 0.0 ? 32.0 * log2(fmin(min_p, 1.0)) : -INFINITY;
-  auto kept = [&](float l, uint32_t j) {
-    if (!(l > -INFINITY) || !inside(cut, order_key(l), j)) return 0ull;
-    if (!w.only_largest && !(weight_steps(w, l) >= lowest)) return 0ull;
+}
+
+// ---------------------------------------------------------------------------------------------
+// all other rows
+// ---------------------------------------------------------------------------------------------
+constexpr int kRowThreads = 512;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowBins = 2048;
+constexpr int kRowList = 2048;
+constexpr int kRowPieces = 64;  // of a warp's stretch: kept weights are added up for each
+constexpr int kRowParts = 8;
+
+// Everything up to and including (key, index) in the order is inside.
+struct RowCut {
+  uint32_t key;
+  uint32_t index;
+};
+constexpr uint32_t kNoIndexLimit = 0xffffffffu;
+__device__ __forceinline__ bool inside(const RowCut& c, uint32_t key, uint32_t index) {
+  return key > c.key || (key == c.key && index <= c.index);
+}
+
+struct RowShared {
+  union {
+    struct {
+      uint32_t lo[kRowBins], hi[kRowBins];  // a 64-bit sum in two words
+    } bins;
+    unsigned long long list[kRowList];      // the elements of one bin, order_pair(key, index)
+  };
+  unsigned long long pieces[kRowWarps * kRowPieces];
+  unsigned long long reduce[32];
+  float reduce_f[32];
+  double table[32];
+  // written by the blocks of the cluster, each into its own place
+  float part_max[kRowParts], part_min[kRowParts];
+  unsigned long long part_sum[kRowParts];
+  uint32_t part_least[kRowParts], part_most[kRowParts], part_listed[kRowParts];
+  // written by one block into all
+  unsigned long long found_before;
+  uint32_t found_bin;
+  RowCut found_cut;
+  unsigned int listed;
+  uint32_t piece;
+  unsigned long long piece_before;
+};
+
+__device__ __forceinline__ uint4 load_piece(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void copy_async16(void* smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// One block's stretch of a row in vectors of 16 bytes, each warp's stretch of it in turn contiguous, so that the order
+// of blocks, warps, steps, lanes and elements is the order of the indices.
+template <typename T>
+struct RowStretch {
+  static constexpr int kPer = 16 / int(sizeof(T));
+  const T* row;
+  uint32_t vocab;
+  int lead;        // elements between the 16-byte boundary below the row and its start
+  int begin, end;  // this warp's vectors
+  int steps;       // of 32 vectors
+  int per_piece;   // steps of a piece
+  uint4* cache;    // this lane's vector of step 0, or null: the row is read from global memory each time
+
+  __device__ __forceinline__ uint4 load(int v) const {
+    const long long e = (long long)v * kPer - lead;
+    if (e >= 0 && e + kPer <= (long long)vocab) return load_piece(row + e);
+    constexpr uint32_t none = RowGroups<T>::kNegInf;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool exists = e + i >= 0 && e + i < (long long)vocab;
+      const uint32_t b = exists ? uint32_t(reinterpret_cast<const typename RowGroups<T>::Bits*>(row)[e + i]) : none;
+      w[i * int(sizeof(T)) / 4] |= b << (8 * (i * int(sizeof(T)) % 4));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // f(step, first element's index, the elements) for this lane's vector of a step; elements outside the row are -inf.
+  template <typename F>
+  __device__ __forceinline__ void at_step(int step, F f) const {
+    const int v = begin + step * 32 + int(threadIdx.x & 31);
+    if (v >= end) return;
+    const uint4 raw = cache != nullptr ? cache[step * 32] : load(v);
+    float l[kPer];
+    if constexpr (sizeof(T) == 4) {
+      l[0] = __uint_as_float(raw.x); l[1] = __uint_as_float(raw.y);
+      l[2] = __uint_as_float(raw.z); l[3] = __uint_as_float(raw.w);
+    } else {
+      const T* tag = nullptr;
+      halves(raw.x, l[0], l[1], tag);
+      halves(raw.y, l[2], l[3], tag);
+      halves(raw.z, l[4], l[5], tag);
+      halves(raw.w, l[6], l[7], tag);
+    }
+    f(uint32_t(v * kPer - lead), l);
+  }
+  template <typename F>
+  __device__ __forceinline__ void sweep(F f) const {
+    for (int step = 0; step < steps; ++step)
+      at_step(step, [&](uint32_t index, float(&l)[kPer]) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (l[i] > -INFINITY) f(index + i, l[i]);  // neither -inf nor NaN
+      });
+  }
+};
+
+struct RowCluster {
+  cooperative_groups::cluster_group group;
+  int rank, parts;
+  RowShared& s;
+  __device__ __forceinline__ RowShared& of(int part) const { return *group.map_shared_rank(&s, part); }
+};
+
+struct Crossing {
+  uint32_t bin;
+  unsigned long long before;  // what lies in the bins ahead of it
+  unsigned long long total;
+};
+
+// Sums amount(index, logit) by bin(logit) over the row (elements with bin >= kRowBins are left out) and finds the bin in
+// which target(total) is reached, bin 0 first.
+template <typename T, typename Amount, typename Bin, typename Target>
+__device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStretch<T>& x, Amount amount, Bin bin, Target target) {
+  RowShared& s = c.s;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) s.bins.lo[i] = s.bins.hi[i] = 0;
+  __syncthreads();
+  x.sweep([&](uint32_t index, float l) {
+    const uint32_t b = bin(l);
+    if (b >= uint32_t(kRowBins)) return;
+    const unsigned long long a = amount(index, l);
+    if (a == 0) return;
+    const uint32_t low = uint32_t(a);
+    const uint32_t was = atomicAdd(&s.bins.lo[b], low);
+    const uint32_t high = uint32_t(a >> 32) + (was + low < was ? 1u : 0u);  // the carry goes along
+    if (high != 0) atomicAdd(&s.bins.hi[b], high);
+  });
+  c.group.sync();
+  // each block adds up its share of the bins over all blocks; bins_each consecutive ones per thread
+  const int share = kRowBins / c.parts;
+  const int each = share >= kRowThreads ? share / kRowThreads : 1;
+  const int first = c.rank * share + each * int(threadIdx.x);
+  unsigned long long sum[kRowBins / kRowThreads] = {}, mine = 0;
+  if (each * int(threadIdx.x) < share) {
+    for (int part = 0; part < c.parts; ++part) {
+      const RowShared& other = c.of(part);
+#pragma unroll
+      for (int i = 0; i < kRowBins / kRowThreads; ++i)
+        if (i < each) sum[i] += ((unsigned long long)other.bins.hi[first + i] << 32) + other.bins.lo[first + i];
+    }
+#pragma unroll
+    for (int i = 0; i < kRowBins / kRowThreads; ++i) mine += sum[i];
+  }
+  unsigned long long block_total;
+  unsigned long long before = block_prefix(mine, s.reduce, &block_total);
+  if (int(threadIdx.x) < c.parts) c.of(threadIdx.x).part_sum[c.rank] = block_total;
+  c.group.sync();
+  Crossing found;
+  found.total = 0;
+  for (int part = 0; part < c.parts; ++part) {
+    if (part < c.rank) before += s.part_sum[part];
+    found.total += s.part_sum[part];
+  }
+  const unsigned long long goal = target(found.total);
+#pragma unroll
+  for (int i = 0; i < kRowBins / kRowThreads; ++i) {
+    if (sum[i] != 0 && before < goal && goal <= before + sum[i])
+      for (int part = 0; part < c.parts; ++part) {
+        c.of(part).found_bin = uint32_t(first + i);
+        c.of(part).found_before = before;
+      }
+    before += sum[i];
+  }
+  c.group.sync();
+  found.bin = s.found_bin;
+  found.before = s.found_before;
+  return found;
+}
+
+// The place in the order at which the amounts reach `target`, given that this happens among the elements that `active`
+// selects and that `before` lies ahead of them. weight(index, logit): their amounts, equal for equal logits.
+template <typename T, typename Amount, typename Active>
+__device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStretch<T>& x, unsigned long long before,
+                                             unsigned long long target, Amount amount, Active active) {
+  RowShared& s = c.s;
+  uint32_t from = 0, to = 0xffffffffu;  // keys that still matter
+  for (;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    uint32_t least = 0xffffffffu, most = 0;
+    x.sweep([&](uint32_t index, float l) {
+      const uint32_t key = order_key(l);
+      if (key < from || key > to || !active(index, l)) return;
+      least = min(least, key);
+      most = max(most, key);
+      const unsigned int at = atomicAdd(&s.listed, 1u);
+      if (at < unsigned(kRowList)) s.list[at] = order_pair(key, index);
+    });
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    uint32_t* scratch = reinterpret_cast<uint32_t*>(s.reduce);
+    if ((threadIdx.x & 31) == 0) {
+      scratch[threadIdx.x >> 5] = least;
+      scratch[32 + (threadIdx.x >> 5)] = most;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < kRowWarps; ++i) {
+        least = min(least, scratch[i]);
+        most = max(most, scratch[32 + i]);
+      }
+      for (int part = 0; part < c.parts; ++part) {
+        c.of(part).part_least[c.rank] = least;
+        c.of(part).part_most[c.rank] = most;
+        c.of(part).part_listed[c.rank] = s.listed;
+      }
+    }
+    c.group.sync();
+    unsigned int n = 0;
+    least = 0xffffffffu;
+    most = 0;
+    for (int part = 0; part < c.parts; ++part) {
+      n += s.part_listed[part];
+      least = min(least, s.part_least[part]);
+      most = max(most, s.part_most[part]);
+    }
+    if (n <= unsigned(kRowList)) {
+      // few enough: the first block takes them all, sorts them and adds their amounts up
+      if (c.rank == 0) {
+        unsigned int at = s.listed;
+        for (int part = 1; part < c.parts; ++part) {
+          const RowShared& other = c.of(part);
+          const unsigned int more = s.part_listed[part];
+          for (unsigned int i = threadIdx.x; i < more; i += kRowThreads) s.list[at + i] = other.list[i];
+          at += more;
+        }
+        int padded = 2;
+        while (padded < int(n)) padded <<= 1;
+        for (int i = int(n) + int(threadIdx.x); i < padded; i += kRowThreads) s.list[i] = 0;
+        block_sort_descending(s.list, padded);
+        unsigned long long seen = before;
+        for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
+          const int i = i0 + int(threadIdx.x);
+          unsigned long long a = 0;
+          if (i < int(n)) a = amount(pair_index(s.list[i]), key_to_float(pair_key(s.list[i])));
+          unsigned long long sum;
+          const unsigned long long place = seen + block_prefix(a, s.reduce, &sum);
+          if (a != 0 && place < target && target <= place + a)
+            for (int part = 0; part < c.parts; ++part)
+              c.of(part).found_cut = RowCut{pair_key(s.list[i]), pair_index(s.list[i])};
+          seen += sum;
+          if (seen >= target) break;
+        }
+      }
+      c.group.sync();
+      return s.found_cut;
+    }
+    if (least == most) {
+      // one value: the m-th of its places
+      const unsigned long long each = amount(kNoIndexLimit, key_to_float(least));
+      unsigned long long m = (target - before + each - 1) / each;
+      auto is_one = [&](uint32_t index, float l) { return order_key(l) == least && active(index, l); };
+      unsigned long long mine = 0;
+      x.sweep([&](uint32_t index, float l) { mine += is_one(index, l); });
+      // in index order: lanes of a step, steps, warps, blocks
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      unsigned long long total;
+      unsigned long long ahead = block_prefix((threadIdx.x & 31) == 0 ? mine : 0ull, s.reduce, &total);
+      ahead = __shfl_sync(0xffffffffu, ahead, 0);
+      if (int(threadIdx.x) < c.parts) c.of(threadIdx.x).part_sum[c.rank] = total;
+      c.group.sync();
+      for (int part = 0; part < c.rank; ++part) ahead += s.part_sum[part];
+      if (ahead < m && m <= ahead + mine) {
+        for (int step = 0; step < x.steps; ++step) {
+          unsigned long long here = 0;
+          x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+            for (int i = 0; i < RowStretch<T>::kPer; ++i) here += l[i] > -INFINITY && is_one(index + i, l[i]);
+          });
+          unsigned long long inc = here;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long other = __shfl_up_sync(0xffffffffu, inc, o);
+            if (int(threadIdx.x & 31) >= o) inc += other;
+          }
+          unsigned long long at = ahead + inc - here;
+          if (at < m && m <= at + here)
+            x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+              for (int i = 0; i < RowStretch<T>::kPer; ++i)
+                if (l[i] > -INFINITY && is_one(index + i, l[i]) && ++at == m)
+                  for (int part = 0; part < c.parts; ++part) c.of(part).found_cut = RowCut{least, index + i};
+            });
+          ahead += __shfl_sync(0xffffffffu, inc, 31);
+        }
+      }
+      c.group.sync();
+      return s.found_cut;
+    }
+    // too many of several values: a finer histogram over their keys (a fraction of 2048 of the range at least)
+    int shift = 0;
+    while (((most - least) >> shift) >= uint32_t(kRowBins)) ++shift;
+    const uint32_t a = least, b = most;
+    const Crossing at = find_bin(
+        c, x, [&](uint32_t index, float l) { return active(index, l) ? amount(index, l) : 0ull; },
+        [&](float l) {
+          const uint32_t key = order_key(l);
+          return key >= a && key <= b ? (b - key) >> shift : uint32_t(kRowBins);
+        },
+        [&](unsigned long long) { return target - before; });
+    before += at.before;
+    to = b - (at.bin << shift);
+    const uint32_t down = (1u << shift) - 1u;
+    from = to - a > down ? to - down : a;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 2)
+sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int parts, int cache_vectors,
+                  const SampleParams p, long long* __restrict__ tokens, float* __restrict__ logprobs) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  RowShared& s = *reinterpret_cast<RowShared*>(dynamic);
+  const long long r = blockIdx.x / parts;
+  const RowSettings set = row_settings(p, r);
+  if (by_list(p, set)) return;  // the whole cluster
+  RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  RowStretch<T> x;
+  x.row = logits + r * ld;
+  x.vocab = vocab;
+  x.lead = int((reinterpret_cast<uintptr_t>(x.row) & 15u) / sizeof(T));
+  const int vectors = int(((long long)vocab + x.lead + RowStretch<T>::kPer - 1) / RowStretch<T>::kPer);
+  const int per_block = (vectors + parts - 1) / parts;
+  const int per_warp = (per_block + kRowThreads - 1) / kRowThreads * 32;
+  const int block_begin = min(c.rank * per_block, vectors), block_end = min(block_begin + per_block, vectors);
+  x.begin = min(block_begin + warp * per_warp, block_end);
+  x.end = min(x.begin + per_warp, block_end);
+  x.steps = (x.end - x.begin + 31) / 32;
+  x.per_piece = (per_warp / 32 + kRowPieces - 1) / kRowPieces;
+  x.cache = nullptr;
+  if (cache_vectors > 0) {
+    uint4* cache = reinterpret_cast<uint4*>(dynamic + (sizeof(RowShared) + 15) / 16 * 16) + (x.begin - block_begin) + lane;
+    for (int step = 0; step < x.steps; ++step) {
+      const int v = x.begin + step * 32 + lane;
+      if (v >= x.end) break;
+      const long long e = (long long)v * RowStretch<T>::kPer - x.lead;
+      if (e >= 0 && e + RowStretch<T>::kPer <= (long long)vocab) copy_async16(cache + step * 32, x.row + e);
+      else cache[step * 32] = x.load(v);
+    }
+    copy_async_wait();  // a lane reads back what it has copied itself
+    x.cache = cache;
+  }
+  if (threadIdx.x < 32) s.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+
+  // ---- the largest logit, and the smallest that may be drawn
+  float top = -INFINITY, low = INFINITY;
+  x.sweep([&](uint32_t, float l) {
+    top = fmaxf(top, l);
+    low = fminf(low, l);
+  });
+  top = block_max(top, s.reduce_f);
+  low = -block_max(-low, s.reduce_f);
+  if (int(threadIdx.x) < parts) {
+    c.of(threadIdx.x).part_max[c.rank] = top;
+    c.of(threadIdx.x).part_min[c.rank] = low;
+  }
+  c.group.sync();
+  for (int part = 0; part < parts; ++part) {
+    top = fmaxf(top, s.part_max[part]);
+    low = fminf(low, s.part_min[part]);
+  }
+  if (!(top > -INFINITY)) {
+    if (c.rank == 0 && threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
+    return;  // the whole cluster; nothing of it is read any more
+  }
+  const RowWeights w = row_weights(p, set, top, s.table);
+  auto weight = [&](float l) { return row_weight(w, l); };
+
+  // ---- the cuts. First bins: equal steps of the logit below the largest, down to where weights round to nothing (what
+  // is below shares the last bin).
+  const float reach = float(46.0 * 0.69314718055994531 * set.temperature);
+  const bool all_in_reach = top - low <= reach;
+  const float range = fminf(top - low, reach);
+  const float per_bin = w.only_largest ? 1.f : (range > 0.f ? float(kRowBins) / range : 0.f);
+  auto bin = [&](float l) {
+    return l == top ? 0u : uint32_t(min(kRowBins - 1, __float2int_rz((top - l) * per_bin)));
+  };
+  RowCut cut{0u, kNoIndexLimit};
+  if (set.top_k > 0 && set.top_k < (long long)vocab) {
+    const unsigned long long k = (unsigned long long)set.top_k;
+    auto one = [](uint32_t, float) { return 1ull; };
+    const Crossing at = find_bin(c, x, one, bin, [&](unsigned long long total) { return total < k ? total : k; });
+    // a cut among weights of nothing changes nothing
+    if (at.total > k && (all_in_reach || at.bin + 1 < uint32_t(kRowBins)))
+      cut = find_place(c, x, at.before, k, one, [&](uint32_t, float l) { return bin(l) == at.bin; });
+  }
+  if (set.top_p < 1.0) {
+    const RowCut outer = cut;
+    auto amount = [&](uint32_t index, float l) { return inside(outer, order_key(l), index) ? weight(l) : 0ull; };
+    unsigned long long target = 0;
+    const Crossing at = find_bin(c, x, amount, bin, [&](unsigned long long total) {
+      target = mass_target(set.top_p, total);
+      return target;
+    });
+    cut = find_place(c, x, at.before, target, [&](uint32_t, float l) { return weight(l); },
+                     [&](uint32_t index, float l) { return bin(l) == at.bin && inside(outer, order_key(l), index); });
+  }
+
+  // ---- the kept weights, piece by piece
+  auto kept = [&](uint32_t index, float l) {
+    if (!(l > -INFINITY) || !inside(cut, order_key(l), index)) return 0ull;
+    if (!w.only_largest && !(weight_steps(w, l) >= set.lowest)) return 0ull;
     return weight(l);
   };
-  unsigned long long total = 0;
-  for (uint32_t j = threadIdx.x; j < vocab; j += blockDim.x) total += kept(logit_to_float(row[j]), j);
-  total = block_sum(total, s.reduce);
-  unsigned long long goal = (unsigned long long)(fmin(u, 1.0) * double(total));
-  if (goal >= total) goal = total - 1;
-  unsigned long long seen = 0;
-  for (uint32_t j0 = 0; j0 < vocab; j0 += blockDim.x) {
-    const uint32_t j = j0 + threadIdx.x;
-    float l = -INFINITY;
-    unsigned long long a = 0;
-    if (j < vocab) {
-      l = logit_to_float(row[j]);
-      a = kept(l, j);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRowWarps * kRowPieces; i += kRowThreads) s.pieces[i] = 0;
+  __syncthreads();
+  for (int step0 = 0; step0 < x.steps; step0 += x.per_piece) {
+    unsigned long long mine = 0;
+    for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step)
+      x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+#pragma unroll
+        for (int i = 0; i < RowStretch<T>::kPer; ++i) mine += kept(index + i, l[i]);
+      });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s.pieces[warp * kRowPieces + step0 / x.per_piece] = mine;
+  }
+  __syncthreads();
+  constexpr int kEach = kRowWarps * kRowPieces / kRowThreads;
+  unsigned long long mine = 0, block_total;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) mine += s.pieces[kEach * threadIdx.x + i];
+  unsigned long long before = block_prefix(mine, s.reduce, &block_total);
+  if (int(threadIdx.x) < parts) c.of(threadIdx.x).part_sum[c.rank] = block_total;
+  c.group.sync();
+  // ---- the token: no block touches another's memory from here on
+  unsigned long long total = 0, block_before = 0;
+  for (int part = 0; part < parts; ++part) {
+    if (part < c.rank) block_before += s.part_sum[part];
+    total += s.part_sum[part];
+  }
+  const unsigned long long goal = draw_target(set.u, total);
+  if (goal < block_before || goal >= block_before + block_total) return;
+  before += block_before;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const unsigned long long a = s.pieces[kEach * threadIdx.x + i];
+    if (a != 0 && before <= goal && goal < before + a) {
+      s.piece = kEach * threadIdx.x + i;
+      s.piece_before = before;
     }
-    unsigned long long sum;
-    const unsigned long long at = seen + block_prefix(a, s.reduce, &sum);
-    if (a != 0 && at <= goal && goal < at + a) {
-      tokens[r] = j;
-      const double log_share = w.only_largest ? log(double(a) / double(total))
-                                              : weight_steps(w, l) * kStepLn2 - log(ldexp(double(total), -weight_bits));
-      logprobs[r] = float(log_share);
+    before += a;
+  }
+  __syncthreads();
+  if (warp != int(s.piece) / kRowPieces) return;
+  const int step0 = int(s.piece) % kRowPieces * x.per_piece;
+  before = s.piece_before;
+  for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step) {
+    unsigned long long here = 0;
+    x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+#pragma unroll
+      for (int i = 0; i < RowStretch<T>::kPer; ++i) here += kept(index + i, l[i]);
+    });
+    unsigned long long inc = here;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long other = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += other;
     }
-    seen += sum;
-    if (seen > goal) break;
+    unsigned long long at = before + inc - here;
+    if (at <= goal && goal < at + here)
+      x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+        for (int i = 0; i < RowStretch<T>::kPer; ++i) {
+          const unsigned long long a = kept(index + i, l[i]);
+          if (a != 0 && at <= goal && goal < at + a) {
+            tokens[r] = index + i;
+            logprobs[r] = log_share(p, set, w, l[i], a, total);
+          }
+          at += a;
+        }
+      });
+    before += __shfl_sync(0xffffffffu, inc, 31);
   }
 }
 

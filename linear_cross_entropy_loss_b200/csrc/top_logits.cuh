@@ -4,45 +4,7 @@
 
 #include "row_top.cuh"
 
-#include <cooperative_groups.h>
-
 namespace lce {
-
-// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then has the row's k first groups
-// among its entries. k * parts <= kTopList. The other blocks return with their part done.
-__device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
-  if (parts > 1) {
-    if (s.count > unsigned(kTopList / parts)) cut_list(s, s.list, s.count, k, kTopList / parts);
-    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-    cluster.sync();
-    if (cluster.block_rank() == 0) {
-      unsigned int at = s.count;
-      for (int part = 1; part < parts; ++part) {
-        const TopShared* other = cluster.map_shared_rank(&s, part);
-        const unsigned int n = other->count;
-        for (unsigned int i = threadIdx.x; i < n; i += kTopThreads) s.list[at + i] = other->list[i];
-        at += n;
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        s.count = at;
-        float m = s.part_ref;
-        for (int part = 1; part < parts; ++part) m = fmaxf(m, cluster.map_shared_rank(&s, part)->part_ref);
-        float sum = 0.f;
-        for (int part = 0; part < parts; ++part) {
-          const TopShared* other = cluster.map_shared_rank(&s, part);
-          if (other->part_ref > -INFINITY) sum += other->part_sum * fast_exp2(other->part_ref - m);
-        }
-        s.part_ref = m;
-        s.part_sum = sum;
-      }
-    }
-    cluster.sync();
-    if (cluster.block_rank() != 0) return;
-  }
-  __syncthreads();
-  if (s.count > unsigned(k + k / 4 + 32)) cut_list(s, s.list, s.count, k, min(2 * k + 64, kTopFull));
-}
 
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads, 4)
@@ -56,7 +18,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const int v0 = min(part * share, row.groups), v1 = min(v0 + share, row.groups);
   const float log2_scale = inv_temperature * 1.4426950408889634f;
   float ref, sum;
-  stream_top<T, true>(s, row, v0, v1, k, log2_scale, ref, sum);
+  stream_top<T, true, Nan::kFirst>(s, row, v0, v1, k, log2_scale, ref, sum);
   const float m = block_max(ref, s.scratch);
   sum = block_sum(ref > -INFINITY ? sum * fast_exp2(ref - m) : 0.f, s.scratch);
   if (threadIdx.x == 0) {
@@ -65,7 +27,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   }
   merge_lists(s, k, parts);
   if (part != 0) return;
-  rank_elements(s, row, k);
+  rank_elements<Nan::kFirst>(s, row, k);
   for (int i = threadIdx.x; i < k; i += kTopThreads) {
     const unsigned long long e = s.elements[i];
     values[r * k + i] = T(key_to_float(pair_key(e)));
