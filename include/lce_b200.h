@@ -311,6 +311,17 @@ int lce_distill_pass(const lce_problem* p, const lce_teacher* teacher, const voi
                      const void* weight, int64_t w_ld, void* workspace, void* dx, int64_t dx_ld, void* dweight,
                      int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, float* loss, void* stream);
 
+/* dst[r, c] = src[r, c] for src rows that start anywhere (src_ld elements apart) and dst rows on 16-byte boundaries: what x and W
+ * need before a pass when their sizes are not multiples of 16 bytes. Whole vectors of 16 bytes are written, so dst_ld must
+ * be at least cols rounded up to them; what lies behind column cols is unspecified. No counterpart in the reference. */
+int lce_align_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype, int64_t rows,
+                   int64_t cols, void* stream);
+
+/* Two matrices times *dev_factor in place, in one launch; a factor of exactly 1 leaves them untouched. Both of element
+ * type dtype, columns % 8 == 0, rows on 16-byte boundaries. No counterpart in the reference. */
+int lce_grad_scale_pair(void* a, int64_t a_ld, int64_t a_rows, int64_t a_cols, void* b, int64_t b_ld, int64_t b_rows,
+                        int64_t b_cols, int32_t dtype, const float* dev_factor, void* stream);
+
 /* ---- operators on given logits ------------------------------------------------------------------
  * No counterpart in the reference. They need no workspace; logits: [rows, vocab] device memory of element type dtype, rows
  * ld elements apart (ld >= 0, any alignment of the element type).

@@ -220,6 +220,8 @@ SIGNATURES = {
         [ctypes.POINTER(Problem), ctypes.POINTER(Teacher), _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64,
          _vp, _vp],
     ),
+    "lce_align_rows": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp]),
+    "lce_grad_scale_pair": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
     "lce_top_logits": (
         ctypes.c_int, [_i32, _vp, _i64, _i64, _i64, _i32, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "lce_sample_logits": (

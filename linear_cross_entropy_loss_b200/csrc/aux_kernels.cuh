@@ -124,9 +124,12 @@ struct TeacherRows {
   long long start_ld;
   int k;
   int n_tiles;
+  const float* mass;  // [rows] sum of the row's weights
+  float* lse;         // [rows] out: the row's log-sum-exp
+  double* row_loss;   // [rows] out: mass * lse - sum q z + sum q log q; 0 for rows that do not count
 };
 
-// What takes the place of the label's logit: sum_e q z - sum_e q log q, for the block's 32 rows r0 + 0 .. 31 (8 warps, four rows
+// The listed part of the loss: sum_e q z - sum_e q log q, for the block's 32 rows r0 + 0 .. 31 (8 warps, four rows
 // each; dots is complete after the caller's next __syncthreads).
 __device__ __forceinline__ void listed_dots(const TeacherRows& t, int r0, int rows, float* dots /*[32]*/) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -139,6 +142,13 @@ __device__ __forceinline__ void listed_dots(const TeacherRows& t, int r0, int ro
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) dots[i] = d - t.plogp[r];
   }
+}
+
+// One row of a distillation: there is one shard and no monitoring, so its log-sum-exp and its loss are known here.
+__device__ __forceinline__ void listed_row(const TeacherRows& t, int r, bool valid, float base, float sum, float dot) {
+  const float lse = base + logf(sum);
+  t.lse[r] = lse;
+  t.row_loss[r] = valid ? (double)t.mass[r] * (double)lse - (double)dot : 0.0;
 }
 
 // Block = 32 rows x 8 warps; warp w walks V tiles w, w+8, ...; lane = row. Per-tile statistics are
@@ -177,11 +187,15 @@ row_stats_kernel(const float* __restrict__ tile_max, const float* __restrict__ t
       q += sm[w][3][lane];
     }
     const long long yv = labels[r];
+    if (teacher.idx != nullptr) {
+      listed_row(teacher, r, yv != ignore_index, m, s, dots[lane]);
+      return;
+    }
     const long long yl = yv - vocab_offset;
     const bool own = (yv != ignore_index) && yl >= 0 && yl < vocab_local;
     parts[0 * stat_ld + r] = m;
     parts[1 * stat_ld + r] = s;
-    parts[2 * stat_ld + r] = teacher.idx != nullptr ? dots[lane] : (own ? target_logit[r] : 0.f);
+    parts[2 * stat_ld + r] = own ? target_logit[r] : 0.f;
     parts[3 * stat_ld + r] = u;
     parts[4 * stat_ld + r] = q;
     parts[5 * stat_ld + r] = m;
@@ -236,14 +250,18 @@ row_stats_rowref_kernel(const float* __restrict__ tile_max, const float* __restr
     }
     const float ref = (row_ref_in != nullptr) ? row_ref_in[r] : 0.f;
     const long long yv = labels[r];
-    const long long yl = yv - vocab_offset;
-    const bool own = (yv != ignore_index) && yl >= 0 && yl < vocab_local;
-    parts[0 * stat_ld + r] = ref;
-    parts[1 * stat_ld + r] = s;
-    parts[2 * stat_ld + r] = teacher.idx != nullptr ? dots[lane] : (own ? target_logit[r] : 0.f);
-    parts[3 * stat_ld + r] = u;
-    parts[4 * stat_ld + r] = q;
-    parts[5 * stat_ld + r] = m;
+    if (teacher.idx != nullptr) {
+      listed_row(teacher, r, yv != ignore_index, ref, s, dots[lane]);
+    } else {
+      const long long yl = yv - vocab_offset;
+      const bool own = (yv != ignore_index) && yl >= 0 && yl < vocab_local;
+      parts[0 * stat_ld + r] = ref;
+      parts[1 * stat_ld + r] = s;
+      parts[2 * stat_ld + r] = own ? target_logit[r] : 0.f;
+      parts[3 * stat_ld + r] = u;
+      parts[4 * stat_ld + r] = q;
+      parts[5 * stat_ld + r] = m;
+    }
     row_base_out[r] = ref;
     row_ref_out[r] = m;
     if (!(m - ref <= kRefAbove && m - ref >= -kRefBelow)) {  // also catches NaN / inf
@@ -274,12 +292,11 @@ __device__ __forceinline__ float ld_coherent(const float* p) {
 
 // Body of the combine step, for one block of 1024 threads per chunk. parts_all: [world][ROW_PARTS][stat_ld].
 // rescue_groups: n_groups ints of this chunk's buffers; the last one is the chunk's "any group flagged" word.
-// row_mass: distillation, the sum of the row's teacher weights (null: 1, a label).
 template <bool kCoherent>
 __device__ __forceinline__ void combine_rows(const float* parts_all, int world, const long long* __restrict__ labels,
                                              int rows, long long stat_ld, long long ignore_index, int monitoring,
                                              float* __restrict__ lse_out, PassScalars* sc, int* rescue_groups,
-                                             int n_groups, const float* row_mass = nullptr) {
+                                             int n_groups) {
   __shared__ double scratch_d[32];
   __shared__ float scratch_f[32];
   double a_nll = 0.0, a_lse2 = 0.0, a_ent = 0.0, a_norm = 0.0;
@@ -298,7 +315,7 @@ __device__ __forceinline__ void combine_rows(const float* parts_all, int world, 
     lse_out[r] = lse;
     const bool valid = labels[r] != ignore_index;
     if (valid) {
-      a_nll += (row_mass != nullptr ? (double)row_mass[r] * (double)lse : (double)lse) - (double)t;
+      a_nll += (double)lse - (double)t;
       a_lse2 += (double)lse * (double)lse;
       if (monitoring) a_ent += (double)lse - (double)u / (double)s;
     }
@@ -331,9 +348,9 @@ __device__ __forceinline__ void combine_rows(const float* parts_all, int world, 
 __global__ void __launch_bounds__(1024)
 combine_kernel(const float* __restrict__ parts_all, int world, const long long* __restrict__ labels, int rows,
                long long stat_ld, long long ignore_index, int monitoring, float* __restrict__ lse_out,
-               PassScalars* sc, int* rescue_groups, int n_groups, const float* __restrict__ row_mass) {
+               PassScalars* sc, int* rescue_groups, int n_groups) {
   combine_rows<false>(parts_all, world, labels, rows, stat_ld, ignore_index, monitoring, lse_out, sc, rescue_groups,
-                      n_groups, row_mass);
+                      n_groups);
 }
 
 __global__ void finalize_kernel(const PassScalars* sc, double n_rows_total, float z_regularization,

@@ -19,7 +19,7 @@ namespace lce {
 
 constexpr int kTeacherMax = 1024;         // entries per row
 constexpr int kPrepareThreads = 256;
-constexpr int kPrepareEntries = 2048;     // entries a block holds: rows of a block x their length rounded up to 2^n
+constexpr int kPrepareEntries = 4096;     // entries a block holds: its rows x their length rounded up to 2^n
 
 struct TeacherInput {
   const void* logits;
@@ -50,7 +50,8 @@ __device__ __forceinline__ uint32_t teacher_column(const TeacherInput& t, long l
 // Row r of the launch is row row0 + r of the problem. kLists: false writes labels / mass / plogp only (every row of the
 // problem, so that the valid rows can be counted before the first chunk), true the lists of one chunk too.
 //   labels[r] = -1 where the row counts (Q != 0), else ignored
-// One block holds `rows_per_block` rows of `padded` (a power of two) entries each.
+// One warp has a row, of `padded` (a power of two) entries; a block has rows_per_block <= 8 of them, as many as its shared
+// memory holds. The work is short chains of shuffles and shared-memory steps, so what counts is that many warps run at once.
 template <bool kLists>
 __global__ void __launch_bounds__(kPrepareThreads)
 teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long vocab, int rows_per_block, int padded,
@@ -58,19 +59,18 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
                        float* __restrict__ plogp, int* __restrict__ list_idx, float* __restrict__ list_q,
                        unsigned short* __restrict__ start, long long start_ld, int n_tiles) {
   __shared__ unsigned long long list[kPrepareEntries];  // column << 32 | bits of q
-  __shared__ int lengths[32];
+  __shared__ int lengths[kPrepareThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = blockIdx.x * rows_per_block;
-  for (int b = warp; b < rows_per_block; b += kPrepareThreads / 32) {
-    const int r = first + b;
-    unsigned long long* mine = list + b * padded;
-    const bool exists = r < rows;
+  const int r = first + warp;
+  unsigned long long* mine = list + warp * padded;
+  if (warp < rows_per_block && r < rows) {
     float top = -INFINITY;
     bool bad = false;  // NaN or +inf among the entries that are there
     for (int k = lane; k < padded; k += 32) {
       uint32_t col = 0xffffffffu;
       float l = -INFINITY;
-      if (exists && k < t.k) {
+      if (k < t.k) {
         col = teacher_column(t, row0 + r, k, vocab);
         if (col != 0xffffffffu) l = teacher_logit(t, row0 + r, k) * t.inv_temperature;
         if (!(l > -INFINITY) && l == l) col = 0xffffffffu;  // -inf: no weight
@@ -79,19 +79,19 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
       top = fmaxf(top, l);
       mine[k] = ((unsigned long long)col << 32) | __float_as_uint(l);
     }
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     bad = __any_sync(0xffffffffu, bad);
     float base = top;  // q = exp(l - base) / total
     float total = 1.f;
-    __syncwarp();
     if (t.lse != nullptr) {
-      base = exists ? t.lse[row0 + r] : 0.f;
+      base = t.lse[row0 + r];
     } else {
-      float s = 0.f;
+      total = 0.f;
       for (int k = lane; k < padded; k += 32)
-        if (uint32_t(mine[k] >> 32) != 0xffffffffu) s += expf(__uint_as_float(uint32_t(mine[k])) - base);
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      total = s;
+        if (uint32_t(mine[k] >> 32) != 0xffffffffu) total += expf(__uint_as_float(uint32_t(mine[k])) - base);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     const float log_total = logf(total);
     float sum = 0.f, ent = 0.f;
@@ -107,75 +107,94 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
       }
       mine[k] = ((unsigned long long)col << 32) | __float_as_uint(q);
     }
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
       ent += __shfl_xor_sync(0xffffffffu, ent, o);
     }
-    if (lane == 0 && exists) {
+    if (lane == 0) {
       labels[r] = sum == 0.f ? ignored : -1;  // a NaN counts: it has to reach the loss
       mass[r] = sum;
       plogp[r] = ent;
     }
-  }
-  if (!kLists) return;
-
-  // every row by column, ascending (the columns that are not there come last)
-  for (int size = 2; size <= padded; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < rows_per_block * padded / 2; i += kPrepareThreads) {
-        const int lo = ((i & ~(stride - 1)) << 1) | (i & (stride - 1));
-        const int hi = lo | stride;
-        const unsigned long long x = list[lo], y = list[hi];
-        const bool ascending = (lo & (padded - 1) & size) == 0 || size == padded;
-        if ((x > y) == ascending) {
-          list[lo] = y;
-          list[hi] = x;
+    if (kLists) {
+      // by column, ascending (what is not there comes last)
+      for (int size = 2; size <= padded; size <<= 1) {
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+          __syncwarp();
+          for (int i = lane; i < padded / 2; i += 32) {
+            const int lo = ((i & ~(stride - 1)) << 1) | (i & (stride - 1));
+            const int hi = lo | stride;
+            const unsigned long long x = mine[lo], y = mine[hi];
+            if ((x > y) == ((lo & size) == 0)) {
+              mine[lo] = y;
+              mine[hi] = x;
+            }
+          }
         }
       }
-    }
-  }
-  __syncthreads();
-  // equal columns become one entry with the sum of their q (in ascending order of q)
-  for (int b = warp; b < rows_per_block; b += kPrepareThreads / 32) {
-    unsigned long long* mine = list + b * padded;
-    int length = 0;
-    for (int k0 = 0; k0 < padded; k0 += 32) {
-      const int k = k0 + lane;
-      const uint32_t col = k < padded ? uint32_t(mine[k] >> 32) : 0xffffffffu;
-      const uint32_t before = k > 0 && k < padded ? uint32_t(mine[k - 1] >> 32) : 0xffffffffu;
-      const bool head = col != 0xffffffffu && (k == 0 || col != before);
-      float q = 0.f;
-      if (head)
-        for (int m = k; m < padded && uint32_t(mine[m] >> 32) == col; ++m) q += __uint_as_float(uint32_t(mine[m]));
-      const uint32_t heads = __ballot_sync(0xffffffffu, head);
-      const int at = length + __popc(heads & ((1u << lane) - 1u));
-      if (head && first + b < rows) {
-        list_idx[(long long)(first + b) * t.k + at] = int(col);
-        list_q[(long long)(first + b) * t.k + at] = q;
+      __syncwarp();
+      // equal columns become one entry with the sum of their q (in ascending order of q); the list moves together in place
+      int length = 0;
+      for (int k0 = 0; k0 < padded; k0 += 32) {
+        const int k = k0 + lane;
+        const uint32_t col = k < padded ? uint32_t(mine[k] >> 32) : 0xffffffffu;
+        // (a place before k0 may have been written already, with an entry of no higher column)
+        const uint32_t before = k > k0 && k < padded ? uint32_t(mine[k - 1] >> 32) : 0xffffffffu;
+        const bool head = col != 0xffffffffu && (k == k0 ? length == 0 || uint32_t(mine[length - 1] >> 32) != col : col != before);
+        float q = 0.f;
+        if (head)
+          for (int m = k; m < padded && uint32_t(mine[m] >> 32) == col; ++m) q += __uint_as_float(uint32_t(mine[m]));
+        const uint32_t heads = __ballot_sync(0xffffffffu, head);
+        const int at = length + __popc(heads & ((1u << lane) - 1u));
+        if (head) {
+          mine[at] = ((unsigned long long)col << 32) | __float_as_uint(q);
+          list_idx[(long long)r * t.k + at] = int(col);
+          list_q[(long long)r * t.k + at] = q;
+        }
+        length += __popc(heads);
+        __syncwarp();
       }
-      length += __popc(heads);
+      if (lane == 0) lengths[warp] = length;
     }
-    if (lane == 0) lengths[b] = length;
   }
+  if (!kLists) return;
   __syncthreads();
   // start[tile][r]: entries of row r with a column before tile * 256
   for (int i = threadIdx.x; i < (n_tiles + 1) * rows_per_block; i += kPrepareThreads) {
-    const int tile = i / rows_per_block, b = i - tile * rows_per_block, r = first + b;
-    if (r >= rows) continue;
-    const int* idx = list_idx + (long long)r * t.k;
+    const int tile = i / rows_per_block, b = i - tile * rows_per_block;
+    if (first + b >= rows) continue;
+    const unsigned long long* row = list + b * padded;
+    const unsigned long long from = (unsigned long long)tile << 40;  // column tile * 256
     int lo = 0, hi = lengths[b];
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (idx[mid] < tile * 256) lo = mid + 1;
+      if (row[mid] < from) lo = mid + 1;
       else hi = mid;
     }
-    start[(long long)tile * start_ld + r] = (unsigned short)lo;
+    start[(long long)tile * start_ld + first + b] = (unsigned short)lo;
   }
 }
 
 // dZ / T * n of one listed entry.
 __device__ __forceinline__ float listed_dz(float z, float lse, float mass, float q) { return expf(z - lse) * mass - q; }
+
+// The chunk's conditional re-run is behind: its flags are counted and cleared for the next chunk. One block.
+__device__ __forceinline__ void close_rescue(PassScalars* sc, int* rescue_groups, int n_groups, int rows) {
+  int flagged = 0;
+  for (int g0 = 0; g0 < n_groups; g0 += blockDim.x) {
+    const int g = g0 + int(threadIdx.x);
+    flagged += __syncthreads_count(g + 1 < n_groups && rescue_groups[g] != 0);
+    if (g < n_groups) rescue_groups[g] = 0;
+  }
+  if (threadIdx.x == 0) {
+    sc->rerun_groups += flagged;
+    sc->seen_groups += (rows + 255) >> 8;
+  }
+}
+__global__ void close_rescue_kernel(PassScalars* sc, int* rescue_groups, int n_groups, int rows) {
+  close_rescue(sc, rescue_groups, n_groups, rows);
+}
 
 // Row-reference mode (see row_finish_kernel): one block per row,
 //   C = Q exp(ref - lse);  xs = C x;  slab[listed] = (Q softmax - q) / C, from the fp32 logit and rounded once.
@@ -184,7 +203,7 @@ __global__ void __launch_bounds__(256)
 distill_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ xs, long long xs_ld, int hidden,
                       T* __restrict__ slab, long long slab_ld, const float* __restrict__ ref,
                       const float* __restrict__ lse, const float* __restrict__ mass, const TeacherRows t,
-                      int rows_valid, float* __restrict__ row_coef) {
+                      int rows_valid, float* __restrict__ row_coef, PassScalars* sc, int* rescue_groups, int n_groups) {
   const int r = blockIdx.x;
   const bool exists = r < rows_valid;
   const float l = exists ? lse[r] : 0.f;
@@ -192,6 +211,7 @@ distill_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ x
   float C = Q != 0.f ? Q * __expf(ref[r] - l) : 0.f;
   if (Q != 0.f && fabsf(C) < 1e-30f) C = 1e-30f;  // keeps the entries finite
   if (threadIdx.x == 0) row_coef[r] = C;
+  if (r == 0) close_rescue(sc, rescue_groups, n_groups, rows_valid);
   if (Q != 0.f) {
     const int n = t.start[(long long)t.n_tiles * t.start_ld + r];
     for (int k = threadIdx.x; k < n; k += blockDim.x) {
@@ -260,11 +280,89 @@ distill_dz_kernel(T* __restrict__ slab, long long slab_ld, const float* __restri
   }
 }
 
-__global__ void distill_finalize_kernel(const PassScalars* sc, float temperature, float* __restrict__ loss) {
-  if (threadIdx.x != 0 || blockIdx.x != 0) return;
-  double v = sc->sum_nll / (double)sc->n_valid * ((double)temperature * (double)temperature);  // no valid row: NaN
+// One block: loss = T^2 / n * the sum of the rows' losses, always added up in the same order.
+__global__ void __launch_bounds__(1024)
+distill_finalize_kernel(const PassScalars* sc, const double* __restrict__ row_loss, long long rows, float temperature,
+                        float* __restrict__ loss) {
+  __shared__ double scratch[32];
+  double v = 0.0;
+  for (long long r = threadIdx.x; r < rows; r += blockDim.x) v += row_loss[r];
+  v = block_sum_double(v, scratch);
+  if (threadIdx.x != 0) return;
+  v = v / (double)sc->n_valid * ((double)temperature * (double)temperature);  // no valid row: NaN
   if (sc->status != 0) v = NAN;
   *loss = (float)v;
+}
+
+// dst[r, c] = src[r, c] for rows that start anywhere: dst rows lie on 16-byte boundaries (dst_ld elements apart, whole
+// vectors of them are written). A vector of dst is cut out of the two aligned vectors of src that hold it, so both sides move
+// 16 bytes at a time. T: the bits of an element.
+template <typename T>
+__global__ void __launch_bounds__(256)
+align_rows_kernel(const T* __restrict__ src, long long src_ld, T* __restrict__ dst, long long dst_ld, long long rows,
+                  long long cols) {
+  constexpr int kPer = 16 / int(sizeof(T));
+  const long long per_row = (cols + kPer - 1) / kPer;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(src);
+  const uintptr_t end = reinterpret_cast<uintptr_t>(src + (rows - 1) * src_ld + cols);
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * per_row;
+       i += (long long)gridDim.x * blockDim.x) {
+    const long long r = i / per_row, c = (i - r * per_row) * kPer;
+    const T* from = src + r * src_ld + c;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+    const uintptr_t low = at & ~uintptr_t(15);
+    uint32_t w[8];
+    if (low >= begin && low + 32 <= end) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(low)), b = __ldg(reinterpret_cast<const uint4*>(low) + 1);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+      const int bytes = int(at - low);
+      if (bytes & 8) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+      }
+      if (bytes & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+      }
+      if (bytes & 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if (c + k < cols) w[k * int(sizeof(T)) / 4] |= uint32_t(from[k]) << (8 * (k * int(sizeof(T)) % 4));
+    }
+    *reinterpret_cast<uint4*>(dst + r * dst_ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Two matrices times *factor, in place; untouched where the factor is exactly 1. Blocks below `split` have the first.
+template <typename T>
+__global__ void __launch_bounds__(256)
+scale_pair_kernel(T* a, long long a_ld, long long a_rows, long long a_cols, T* b, long long b_ld, long long b_rows,
+                  long long b_cols, int split, const float* __restrict__ factor) {
+  const float f = *factor;
+  if (f == 1.0f) return;
+  const bool second = int(blockIdx.x) >= split;
+  T* m = second ? b : a;
+  const long long ld = second ? b_ld : a_ld, per_row = (second ? b_cols : a_cols) / 8;
+  const long long n = (second ? b_rows : a_rows) * per_row;
+  const long long block = second ? blockIdx.x - split : blockIdx.x, blocks = second ? gridDim.x - split : split;
+  for (long long i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) {
+    const long long r = i / per_row, c = (i - r * per_row) * 8;
+    Vec8<T> v;
+    v.load(m + r * ld + c);
+    float e[8];
+    v.to_float(e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] *= f;
+    v.from_float(e);
+    v.store(m + r * ld + c);
+  }
 }
 
 }  // namespace lce

@@ -416,7 +416,6 @@ int check_chunk(const lce_problem* p, int64_t row0, int64_t rows) {
 struct Distill {
   TeacherRows lists;   // of the chunk's rows
   float* list_z;
-  const float* mass;   // of the chunk's rows
   float grad_scale;    // takes the place of logit_scale in the gradients
   float boost;         // power of two that the slab holds dZ multiplied with (per-tile mode)
 };
@@ -488,7 +487,7 @@ int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void*
   int v = validate_problem(p);
   if (v != LCE_OK) return v;
   if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
-  if (!x || !weight || !labels || !workspace || !row_parts_local) return LCE_ERR_INVALID_ARGUMENT;
+  if (!x || !weight || !labels || !workspace || (!row_parts_local && distill == nullptr)) return LCE_ERR_INVALID_ARGUMENT;
   if (x_ld < p->hidden || w_ld < p->vocab_local) return LCE_ERR_INVALID_ARGUMENT;
   int sms = 0;
   if ((v = ensure_device(&sms)) != LCE_OK) return v;
@@ -541,6 +540,7 @@ int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void*
   TeacherRows teacher = {};
   if (distill != nullptr) {
     teacher = distill->lists;
+    teacher.lse += local0;
     gp.list_idx = teacher.idx;
     gp.list_start = teacher.start;
     gp.list_z = distill->list_z;
@@ -550,7 +550,7 @@ int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void*
 
   const int blocks = (int)((rows + 31) / 32);
   const long long* lab = reinterpret_cast<const long long*>(labels) + row0;
-  float* parts = row_parts_local + local0;
+  float* parts = row_parts_local != nullptr ? row_parts_local + local0 : nullptr;
   auto launch_forward = [&]() {
     return p->monitoring ? launch_gemm_dtype<false, true, EPI_FWD, true>(p->dtype, ta, tb, tc, gp, sms, st, pair)
                          : launch_gemm_dtype<false, true, EPI_FWD, false>(p->dtype, ta, tb, tc, gp, sms, st, pair);
@@ -615,24 +615,6 @@ int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void*
   return LCE_OK;
 }
 
-int combine_chunk(const lce_problem* p, const float* row_parts_all, const int64_t* labels, int64_t row0, int64_t rows,
-                  void* workspace, void* stream, const Distill* distill) {
-  int v = validate_problem(p);
-  if (v != LCE_OK) return v;
-  if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
-  if (!row_parts_all || !labels || !workspace) return LCE_ERR_INVALID_ARGUMENT;
-  int sms = 0;
-  if ((v = ensure_device(&sms)) != LCE_OK) return v;
-  const Workspace w = layout_workspace(p, workspace, sms, chunk_buffer_of(p, row0));
-  const long long local0 = row0 % p->chunk_rows;
-  combine_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_parts_all + local0, p->world,
-                                                       reinterpret_cast<const long long*>(labels) + row0, (int)rows,
-                                                       p->chunk_rows, p->ignore_index, p->monitoring, w.lse + local0,
-                                                       w.scalars, w.rescue_groups, w.n_rescue,
-                                                       distill != nullptr ? distill->mass : nullptr);
-  return check_launch();
-}
-
 }  // namespace
 
 extern "C" {
@@ -645,7 +627,19 @@ int lce_forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const v
 
 int lce_combine_chunk(const lce_problem* p, const float* row_parts_all, const int64_t* labels, int64_t row0,
                       int64_t rows, void* workspace, void* stream) {
-  return combine_chunk(p, row_parts_all, labels, row0, rows, workspace, stream, nullptr);
+  int v = validate_problem(p);
+  if (v != LCE_OK) return v;
+  if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
+  if (!row_parts_all || !labels || !workspace) return LCE_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  if ((v = ensure_device(&sms)) != LCE_OK) return v;
+  const Workspace w = layout_workspace(p, workspace, sms, chunk_buffer_of(p, row0));
+  const long long local0 = row0 % p->chunk_rows;
+  combine_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_parts_all + local0, p->world,
+                                                       reinterpret_cast<const long long*>(labels) + row0, (int)rows,
+                                                       p->chunk_rows, p->ignore_index, p->monitoring, w.lse + local0,
+                                                       w.scalars, w.rescue_groups, w.n_rescue);
+  return check_launch();
 }
 
 int lce_parts_bytes(const lce_problem* p, size_t* bytes) {
@@ -1379,7 +1373,7 @@ struct DistillWorkspace {
   long long* labels;   // [n_rows_total] -1: the row counts, kIgnoredRow: it does not
   float* mass;         // [n_rows_total]
   float* plogp;        // [n_rows_total]
-  float* row_parts;    // [ROW_PARTS * chunk_rows]
+  double* row_loss;    // [n_rows_total]
   int* list_idx;       // [chunk_rows, k]
   float* list_q;
   float* list_z;
@@ -1402,7 +1396,7 @@ DistillWorkspace layout_distill(const lce_problem* p, int k, void* base, int sms
   w.labels = reinterpret_cast<long long*>(take(n * sizeof(long long)));
   w.mass = reinterpret_cast<float*>(take(n * sizeof(float)));
   w.plogp = reinterpret_cast<float*>(take(n * sizeof(float)));
-  w.row_parts = reinterpret_cast<float*>(take(ROW_PARTS * rows * sizeof(float)));
+  w.row_loss = reinterpret_cast<double*>(take(n * sizeof(double)));
   w.list_idx = reinterpret_cast<int*>(take(rows * k * sizeof(int)));
   w.list_q = reinterpret_cast<float*>(take(rows * k * sizeof(float)));
   w.list_z = reinterpret_cast<float*>(take(rows * k * sizeof(float)));
@@ -1427,7 +1421,7 @@ int launch_prepare(const lce_problem* p, const TeacherInput& in, const DistillWo
   int padded = 1;
   while (padded < in.k) padded <<= 1;
   int per_block = kPrepareEntries / padded;
-  if (per_block > 32) per_block = 32;
+  if (per_block > kPrepareThreads / 32) per_block = kPrepareThreads / 32;
   const int grid = (int)((rows + per_block - 1) / per_block);
   const int n_tiles = (int)(vocab_pad(p) / BLOCK_N);
   auto launch = [&](auto kernel) {
@@ -1450,13 +1444,14 @@ void launch_distill_dz(const lce_problem* p, const DistillWorkspace& w, const Di
     if (row_reference_mode(p)) {
       distill_finish_kernel<T><<<(int)rows_pad, 256, 0, st>>>(
           reinterpret_cast<const T*>(x) + row0 * x_ld, x_ld, reinterpret_cast<T*>(w.pass.xs), h_pad, (int)p->hidden,
-          slab, v_pad, w.pass.row_base, w.pass.lse, d.mass, d.lists, (int)rows, w.pass.row_coef);
+          slab, v_pad, w.pass.row_base, w.pass.lse, d.lists.mass, d.lists, (int)rows, w.pass.row_coef, w.pass.scalars,
+          w.pass.rescue_groups, w.pass.n_rescue);
       return;
     }
   }
   distill_dz_kernel<T><<<grid_for((rows_pad / 8) * n_vtiles, 1, sms, 16), 256, 0, st>>>(
-      slab, v_pad, w.pass.tile_max, w.pass.lse, d.mass, d.lists, (int)rows_pad, (int)rows, n_vtiles, p->chunk_rows,
-      d.boost);
+      slab, v_pad, w.pass.tile_max, w.pass.lse, d.lists.mass, d.lists, (int)rows_pad, (int)rows, n_vtiles,
+      p->chunk_rows, d.boost);
 }
 
 }  // namespace
@@ -1520,6 +1515,7 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
   d.lists.start_ld = p->chunk_rows;
   d.lists.k = teacher->k;
   d.lists.n_tiles = (int)(vocab_pad(p) / BLOCK_N);
+  d.lists.lse = w.pass.lse;
 
   const int64_t n_chunks = (p->n_rows_total + p->chunk_rows - 1) / p->chunk_rows;
   const bool one_chunk = n_chunks == 1;
@@ -1529,13 +1525,20 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
   for (int64_t ci = 0; ci < n_chunks; ++ci) {
     const int64_t row0 = ci * p->chunk_rows;
     const int64_t rows = std::min<int64_t>(p->chunk_rows, p->n_rows_total - row0);
-    d.mass = w.mass + row0;
+    d.lists.mass = w.mass + row0;
     d.lists.plogp = w.plogp + row0;
+    d.lists.row_loss = w.row_loss + row0;
     if (!one_chunk && (v = launch_prepare(p, in, w, row0, rows, true, st)) != LCE_OK) return v;
-    if ((v = forward_chunk(p, x, x_ld, weight, w_ld, labels, row0, rows, workspace, w.row_parts, stream, &d)) != LCE_OK)
+    // (the rows' own statistics are not exported: there is one shard)
+    if ((v = forward_chunk(p, x, x_ld, weight, w_ld, labels, row0, rows, workspace, nullptr, stream, &d)) != LCE_OK)
       return v;
-    if ((v = combine_chunk(p, w.row_parts, labels, row0, rows, workspace, stream, &d)) != LCE_OK) return v;
-    if (!p->want_grad) continue;
+    if (!p->want_grad) {
+      if (row_reference_mode(p)) {
+        close_rescue_kernel<<<1, 256, 0, st>>>(w.pass.scalars, w.pass.rescue_groups, w.pass.n_rescue, (int)rows);
+        if ((v = check_launch()) != LCE_OK) return v;
+      }
+      continue;
+    }
     switch (p->dtype) {
       case LCE_DTYPE_F16: launch_distill_dz<__half>(p, w, d, x, x_ld, row0, rows, sms, st); break;
       case LCE_DTYPE_BF16: launch_distill_dz<__nv_bfloat16>(p, w, d, x, x_ld, row0, rows, sms, st); break;
@@ -1548,7 +1551,55 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
                                  ci == n_chunks - 1, stream, d.grad_scale)) != LCE_OK)
       return v;
   }
-  distill_finalize_kernel<<<1, 32, 0, st>>>(w.pass.scalars, temperature, loss);
+  distill_finalize_kernel<<<1, 1024, 0, st>>>(w.pass.scalars, w.row_loss, (long long)p->n_rows_total, temperature, loss);
+  return check_launch();
+}
+
+int lce_align_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype, int64_t rows,
+                   int64_t cols, void* stream) {
+  if (dtype != LCE_DTYPE_F16 && dtype != LCE_DTYPE_BF16 && dtype != LCE_DTYPE_F32) return LCE_ERR_INVALID_ARGUMENT;
+  if (!src || !dst || rows <= 0 || cols <= 0 || src_ld < 0) return LCE_ERR_INVALID_ARGUMENT;
+  const int es = elem_size(dtype), per = 16 / es;
+  if (dst_ld < round_up(cols, per)) return LCE_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(src) & (uintptr_t)(es - 1)) != 0 || (reinterpret_cast<uintptr_t>(dst) & 15u) != 0 ||
+      ((dst_ld * es) & 15) != 0)
+    return LCE_ERR_MISALIGNED;
+  const int grid = grid_for(rows * ((cols + per - 1) / per), 256, sm_count_or_default(), 16);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (es == 2)
+    align_rows_kernel<unsigned short><<<grid, 256, 0, st>>>(reinterpret_cast<const unsigned short*>(src), src_ld,
+                                                            reinterpret_cast<unsigned short*>(dst), dst_ld, rows, cols);
+  else
+    align_rows_kernel<uint32_t><<<grid, 256, 0, st>>>(reinterpret_cast<const uint32_t*>(src), src_ld,
+                                                      reinterpret_cast<uint32_t*>(dst), dst_ld, rows, cols);
+  return check_launch();
+}
+
+int lce_grad_scale_pair(void* a, int64_t a_ld, int64_t a_rows, int64_t a_cols, void* b, int64_t b_ld, int64_t b_rows,
+                        int64_t b_cols, int32_t dtype, const float* dev_factor, void* stream) {
+  if (dtype != LCE_DTYPE_F16 && dtype != LCE_DTYPE_BF16 && dtype != LCE_DTYPE_F32) return LCE_ERR_INVALID_ARGUMENT;
+  if (!a || !b || !dev_factor || a_rows <= 0 || a_cols <= 0 || b_rows <= 0 || b_cols <= 0 || a_ld < a_cols ||
+      b_ld < b_cols)
+    return LCE_ERR_INVALID_ARGUMENT;
+  if (a_cols % 8 != 0 || b_cols % 8 != 0) return LCE_ERR_UNSUPPORTED_SHAPE;
+  const int es = elem_size(dtype);
+  if ((reinterpret_cast<uintptr_t>(a) & 15u) != 0 || (reinterpret_cast<uintptr_t>(b) & 15u) != 0 ||
+      ((a_ld * es) & 15) != 0 || ((b_ld * es) & 15) != 0)
+    return LCE_ERR_MISALIGNED;
+  const int sms = sm_count_or_default();
+  // the usual factor is 1 and every block ends at once: few blocks, which walk the matrices if there is work
+  const int first = grid_for(a_rows * (a_cols / 8), 256, sms, 1), second = grid_for(b_rows * (b_cols / 8), 256, sms, 4);
+  cudaStream_t st = (cudaStream_t)stream;
+  auto launch = [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    scale_pair_kernel<T><<<first + second, 256, 0, st>>>(reinterpret_cast<T*>(a), a_ld, a_rows, a_cols,
+                                                         reinterpret_cast<T*>(b), b_ld, b_rows, b_cols, first, dev_factor);
+  };
+  switch (dtype) {
+    case LCE_DTYPE_F16: launch(static_cast<__half*>(nullptr)); break;
+    case LCE_DTYPE_BF16: launch(static_cast<__nv_bfloat16*>(nullptr)); break;
+    default: launch(static_cast<float*>(nullptr));
+  }
   return check_launch();
 }
 

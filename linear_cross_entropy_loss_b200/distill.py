@@ -58,9 +58,11 @@ def _run_pass(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size, want_d
     dx = torch.empty((N, H), dtype=x.dtype, device=dev) if want_dx else None
     dW = dW_res = None
     if want_dW:
-        dW = _aligned_rows_like((H, V), At.dtype, dev)
+        # rows on 32-byte boundaries (16 elements of the 16-bit types): the contraction then writes whole sectors. On 16-byte
+        # ones it goes element by element: 556 against 80 us for 1000 x 50257 in fp16.
+        dW = _aligned_rows_like((H, V), At.dtype, dev, 16)
         if N > N_group and At.dtype != torch.float32:
-            dW_res = _aligned_rows_like((H, V), At.dtype, dev)  # the rounding residual of the sum over the chunks
+            dW_res = _aligned_rows_like((H, V), At.dtype, dev, 16)  # the rounding residual of the sum over the chunks
     teacher = _native.Teacher(
         logits=t.data_ptr(), indices=idx.data_ptr(), lse=None if lse is None else lse.data_ptr(),
         logits_ld=t.stride(0), indices_ld=idx.stride(0), k=k, logits_dtype=_DTYPE_CODE[t.dtype],
@@ -84,13 +86,19 @@ def _operands(x, At):
         A_pad[:H] = At
         A_pad[H:] = 0
         return x_pad, A_pad
-    if not _tma_ready(x):
-        x = x.contiguous()
-    if not _tma_ready(At):
-        copy = _aligned_rows_like(At.shape, At.dtype, At.device)
-        copy.copy_(At)
-        At = copy
-    return x, At
+    return _aligned(x), _aligned(At)
+
+
+def _aligned(m):
+    """m, or a copy of it whose rows start on 16-byte boundaries."""
+    if _tma_ready(m):
+        return m
+    copy = _aligned_rows_like(m.shape, m.dtype, m.device)
+    if m.stride(1) == 1:
+        get_backend().align_rows(m, copy)
+    else:
+        copy.copy_(m)
+    return copy
 
 
 class LinearDistillationImplementation(torch.autograd.Function):
@@ -100,26 +108,34 @@ class LinearDistillationImplementation(torch.autograd.Function):
     def forward(ctx, x_in, At_in, t, idx, lse, temperature, logit_scale, N_chunk_size):
         with _device_guard(x_in):
             H = x_in.shape[-1]
-            x, At = _operands(x_in.reshape(-1, H), At_in)
-            with torch.no_grad():
-                loss, dx, dW = _run_pass(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size,
-                                         bool(ctx.needs_input_grad[0]), bool(ctx.needs_input_grad[1]))
-            if dx is not None:
-                dx = dx[:, :H]
-            if dW is not None:
-                dW = dW[:H]
+            x, At = _operands(x_in if x_in.dim() == 2 else x_in.reshape(-1, H), At_in)
+            loss, dx, dW = _run_pass(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size,
+                                     ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+            if x.shape[1] != H:  # the padding is dropped again
+                dx = None if dx is None else dx[:, :H]
+                dW = None if dW is None else dW[:H]
             ctx.lce_grads = (dx, dW) if dx is not None or dW is not None else None
             ctx.lce_x_shape = x_in.shape
             ctx.lce_x_dtype = x_in.dtype
             return loss
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
         if ctx.lce_grads is None:
             raise RuntimeError("backward called twice, or forward ran without any input requiring grad")
-        with _device_guard(grad_output), torch.no_grad():
-            gx, gA = _scaled_grads(ctx, grad_output)
-        return gx, gA, None, None, None, None, None, None
+        dx, dW = ctx.lce_grads
+        with _device_guard(grad_output):
+            if dx is None or dW is None:
+                dx, dW = _scaled_grads(ctx, grad_output)
+            else:
+                ctx.lce_grads = None
+                factor = grad_output
+                if factor.dtype != torch.float32 or factor.device != dx.device:
+                    factor = factor.to(device=dx.device, dtype=torch.float32)
+                get_backend().grad_scale_pair(dx, dW, factor)
+                dx = dx.view(ctx.lce_x_shape) if dx.is_contiguous() else dx.reshape(ctx.lce_x_shape)
+        return dx, dW, None, None, None, None, None, None
 
 
 def linear_distillation(
@@ -166,8 +182,10 @@ def linear_distillation(
         assert teacher_lse.shape == rows, "teacher_lse must have one entry per row of x"
         assert teacher_lse.is_floating_point(), "teacher_lse must be floating point"
         teacher_lse = teacher_lse.detach().to(torch.float32).reshape(-1).contiguous()
-    given = [t for t in (x, At, teacher_logits, teacher_indices, teacher_lse) if t is not None]
-    assert all(t.device == x.device for t in given), "all tensors must be on one device"
+        assert teacher_lse.device == x.device, "all tensors must be on one device"
+    dev = x.device
+    assert At.device == dev and teacher_logits.device == dev and teacher_indices.device == dev, \
+        "all tensors must be on one device"
     target = _autocast_target(x)
     if target is not None:
         x, At = x.to(target), At.to(target)
@@ -177,14 +195,15 @@ def linear_distillation(
         raise RuntimeError("linear_cross_entropy_loss_b200 runs on CUDA tensors only; there is no CPU fallback")
 
     def lists(t):
-        t = t.detach().reshape(-1, k)
+        t = t.detach()
+        if t.dim() != 2:
+            t = t.reshape(-1, k)
         return t if t.stride(1) == 1 or k == 1 else t.contiguous()
 
     if not torch.is_grad_enabled():
         x, At = x.detach(), At.detach()
-    with torch.autocast(device_type=x.device.type, enabled=False):
-        return LinearDistillationImplementation.apply(
-            x, At, lists(teacher_logits), lists(teacher_indices), teacher_lse, temperature, logit_scale, N_chunk_size)
+    return LinearDistillationImplementation.apply(
+        x, At, lists(teacher_logits), lists(teacher_indices), teacher_lse, temperature, logit_scale, N_chunk_size)
 
 
 class LinearDistillationLoss(LinearCrossEntropyLoss):

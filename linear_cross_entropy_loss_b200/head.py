@@ -30,7 +30,9 @@ def _rows_of(logits: torch.Tensor) -> torch.Tensor:
     """(rows, V) with unit inner stride; leading dimensions merged (a copy only where the strides do not allow it)."""
     assert logits.dim() >= 1 and logits.shape[-1] >= 1, "logits must have at least one column"
     assert logits.dtype in _DTYPE_CODE, f"unsupported dtype {logits.dtype}"
-    rows = logits.detach().reshape(-1, logits.shape[-1])
+    rows = logits.detach()
+    if rows.dim() != 2:
+        rows = rows.reshape(-1, logits.shape[-1])
     return rows if rows.stride(1) == 1 or rows.shape[1] == 1 else rows.contiguous()
 
 
@@ -60,7 +62,9 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     lse = torch.empty(n, dtype=torch.float32, device=dev)
     with _device_guard(rows):
         backend.top_logits(rows, k, float(temperature), values, indices, lse)
-    return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
+    if len(lead) != 1:
+        values, indices, lse = values.view(*lead, k), indices.view(*lead, k), lse.view(lead)
+    return TopLogits(values, indices, lse)
 
 
 def _setting(value, name: str, dtype, n: int, device):
@@ -69,12 +73,12 @@ def _setting(value, name: str, dtype, n: int, device):
         return value, None
     assert value.numel() in (1, n), f"{name} must be a number or have one entry per row"
     assert value.device == device, f"{name} must be on the device of the logits"
-    value = value.detach().reshape(-1)
-    if dtype == torch.int32:
+    if dtype == torch.int32 and value.dtype != torch.int32:
         assert not value.is_floating_point(), f"{name} must hold whole numbers"
-        if value.dtype != torch.int32:
-            value = value.clamp(0, 2**31 - 1)
-    return None, value.to(dtype).expand(n).contiguous()
+        value = value.clamp(0, 2**31 - 1)
+    if value.dtype == dtype and value.dim() == 1 and value.shape[0] == n and value.is_contiguous():
+        return None, value
+    return None, value.detach().reshape(-1).to(dtype).expand(n).contiguous()
 
 
 def sample_logits(
@@ -105,7 +109,8 @@ def sample_logits(
     assert u.dtype in (torch.float32, torch.float64), "u must be float32 or float64"
     assert u.device == dev, "u must be on the device of the logits"
     s = _native.Sampling(u_dtype=_native.DTYPE_F32 if u.dtype == torch.float32 else _native.SAMPLING_U_F64)
-    u = u.detach().reshape(-1).contiguous()
+    if u.dim() != 1 or not u.is_contiguous():
+        u = u.detach().reshape(-1).contiguous()
     s.u = u.data_ptr()
     alive = []  # what the pointers in `s` refer to, until the kernel has been enqueued
     for name, dtype, value in (("temperature", torch.float32, temperature), ("top_k", torch.int32, top_k),
@@ -127,4 +132,4 @@ def sample_logits(
     with _device_guard(rows):
         backend.sample_logits(rows, s, tokens, logprobs)
     lead = logits.shape[:-1]
-    return Sampled(tokens.view(lead), logprobs.view(lead))
+    return Sampled(tokens, logprobs) if len(lead) == 1 else Sampled(tokens.view(lead), logprobs.view(lead))

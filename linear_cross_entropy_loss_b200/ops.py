@@ -39,6 +39,14 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same handle without building a Stream object (2 us of host time per call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
 class NativeBackend:
     """Calls into liblce_b200.so on the current CUDA stream of the tensors' device."""
 
@@ -50,7 +58,7 @@ class NativeBackend:
 
     @staticmethod
     def _stream(t: torch.Tensor) -> int:
-        return torch.cuda.current_stream(t.device).cuda_stream
+        return _raw_stream(t.device.index)
 
     def workspace_bytes(self, prob: Problem) -> int:
         out = ctypes.c_size_t(0)
@@ -199,6 +207,23 @@ class NativeBackend:
                 0 if dW_res is None else dW_res.stride(0), _ptr(loss), self._stream(workspace),
             ),
             "lce_distill_pass",
+        )
+
+    def align_rows(self, src, dst):
+        _native.check(
+            self.lib.lce_align_rows(_ptr(src), src.stride(0), _ptr(dst), dst.stride(0), _DTYPE_CODE[src.dtype],
+                                    src.shape[0], src.shape[1], self._stream(src)),
+            "lce_align_rows",
+        )
+
+    def grad_scale_pair(self, a, b, factor):
+        # whole groups of 8 columns: the padding columns of an aligned-rows buffer go along
+        _native.check(
+            self.lib.lce_grad_scale_pair(
+                _ptr(a), a.stride(0), a.shape[0], -(-a.shape[1] // 8) * 8, _ptr(b), b.stride(0), b.shape[0],
+                -(-b.shape[1] // 8) * 8, _DTYPE_CODE[a.dtype], _ptr(factor), self._stream(a),
+            ),
+            "lce_grad_scale_pair",
         )
 
     def top_logits(self, logits, k, temperature, values, indices, lse):
@@ -587,16 +612,21 @@ def run_pass(x, y, At, ignore_index, z_regularization, logit_scale, N_chunk_size
     return out5, dx, dW, workspace
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
 def _device_guard(t: torch.Tensor):
     """Makes the tensor's GPU current (needed for devices other than 0, as in reference ops.py:680)."""
-    return torch.cuda.device(t.device) if t.is_cuda else contextlib.nullcontext()
+    if not t.is_cuda or t.device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(t.device)
 
 
-def _aligned_rows_like(shape, dtype, device):
+def _aligned_rows_like(shape, dtype, device, unit=8):
     """An uninitialised (rows, cols) tensor whose rows start on 16-byte boundaries: a view of a buffer that is a few
     columns wider when cols is not a multiple of 8 (vocabulary sizes such as 50257)."""
     rows, cols = shape
-    ld = -(-cols // 8) * 8  # whole groups of 8 elements: 16 bytes for 16-bit types, 32 for fp32 (vector accesses)
+    ld = -(-cols // unit) * unit  # whole groups of 8 elements: 16 bytes for 16-bit types, 32 for fp32 (vector accesses)
     buf = torch.empty((rows, ld), dtype=dtype, device=device)
     return buf if ld == cols else buf[:, :cols]
 

@@ -329,3 +329,16 @@ def test_student_samples_teacher_lists_student_learns():
     bx, bw = gradient_bounds(ref, torch.bfloat16)
     assert ((h.grad.double().cpu() - ref["dx"]).abs() <= bx).all()
     assert ((student.weight.grad.double().cpu() - ref["dW"]).abs() <= bw).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols,ld,offset", [(1, 1, 1, 0), (3, 7, 7, 1), (5, 50257, 50257, 0), (64, 1003, 1010, 3), (9, 64, 64, 5)])
+def test_rows_are_moved_to_boundaries(dtype, rows, cols, ld, offset):
+    from linear_cross_entropy_loss_b200.distill import _aligned
+
+    g = torch.Generator().manual_seed(cols)
+    flat = torch.randn(rows * ld + offset, generator=g).to(dtype).cuda()
+    src = flat[offset:].view(rows, ld)[:, :cols]
+    got = _aligned(src)
+    assert torch.equal(got, src) and got.data_ptr() % 16 == 0
+    assert rows == 1 or got.stride(0) * got.element_size() % 16 == 0

@@ -224,3 +224,20 @@ def test_distill_workspace(lib):
 
 def test_teacher_structure_has_the_layout_of_the_header(tmp_path):
     check_layout(tmp_path, "lce_teacher", _native.Teacher, [("LCE_TEACHER_MAX", _native.TEACHER_MAX)])
+
+
+@pytest.mark.parametrize("kw,code", [(dict(src=None), -1), (dict(dst=None), -1), (dict(rows=0), -1), (dict(cols=0), -1),
+                                     (dict(src_ld=-1), -1), (dict(dst_ld=96), -1), (dict(dtype=5), -1), (dict(src=17), -3),
+                                     (dict(dst=24), -3), (dict(dst_ld=108), -3)])
+def test_align_rows_abi_refuses(lib, kw, code):
+    a = dict(src=18, src_ld=101, dst=32, dst_ld=104, dtype=1, rows=4, cols=101)
+    a.update(kw)
+    assert lib.lce_align_rows(a["src"], a["src_ld"], a["dst"], a["dst_ld"], a["dtype"], a["rows"], a["cols"], None) == code
+
+
+@pytest.mark.parametrize("kw,code", [(dict(a=None), -1), (dict(b=None), -1), (dict(f=None), -1), (dict(rows=0), -1),
+                                     (dict(cols=12), -2), (dict(ld=8), -1), (dict(dtype=4), -1), (dict(a=24), -3), (dict(ld=20), -3)])
+def test_grad_scale_pair_abi_refuses(lib, kw, code):
+    a = dict(a=32, b=64, f=16, rows=4, cols=16, ld=16, dtype=1)
+    a.update(kw)
+    assert lib.lce_grad_scale_pair(a["a"], a["ld"], a["rows"], a["cols"], a["b"], 16, 4, 16, a["dtype"], a["f"], None) == code
