@@ -75,12 +75,12 @@ int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
 }
 
 // Blocks that share a row of sample_row_kernel, and the vectors of 16 bytes that each keeps in shared memory (0: too long a
-// row, it is read again for each sweep). A block keeps up to 64 KiB, so that two are on an SM; few rows are split further, down to 8 KiB; up
+// row, it is read again for each sweep). A block keeps up to 65 KiB, so that two are on an SM; few rows are split further, down to 8 KiB; up
 // to 192 KiB where eight blocks are not enough.
 void row_layout(int64_t rows, int64_t vocab, int es, int* parts, int* cache_vectors) {
   const int64_t bytes = vocab * es + 32;
   int n = 1;
-  while (n < kRowParts && bytes > n * (64ll << 10)) n *= 2;
+  while (n < kRowParts && bytes > n * (65ll << 10)) n *= 2;
   while (n < kRowParts && rows * n * 2 <= 2ll * sm_count() && bytes > n * (16ll << 10)) n *= 2;
   const int64_t vectors = (bytes + 15) / 16;
   const int64_t each = (vectors + n - 1) / n;

@@ -198,29 +198,27 @@ constexpr int kRowList = 2048;
 constexpr int kRowPieces = 64;  // of a warp's stretch: kept weights are added up for each
 constexpr int kRowParts = 8;
 
-// Everything up to and including (key, index) in the order is inside.
+// A stretch of the order that starts at its top: logits above `value`, and equal ones with an index below `end`.
 struct RowCut {
-  uint32_t key;
-  uint32_t index;
+  float value;
+  uint32_t end;
 };
-constexpr uint32_t kNoIndexLimit = 0xffffffffu;
-__device__ __forceinline__ bool inside(const RowCut& c, uint32_t key, uint32_t index) {
-  return key > c.key || (key == c.key && index <= c.index);
+constexpr uint32_t kNoEnd = 0xffffffffu;
+__device__ __forceinline__ bool inside(const RowCut& c, float l, uint32_t index) {
+  return l > c.value || (l == c.value && index < c.end);  // never a NaN
 }
 
 struct RowShared {
   union {
-    struct {
-      uint32_t lo[kRowBins], hi[kRowBins];  // a 64-bit sum in two words
-    } bins;
-    unsigned long long list[kRowList];      // the elements of one bin, order_pair(key, index)
+    unsigned long long bins[kRowBins];
+    unsigned long long list[kRowList];  // the elements of one bin, order_pair(key, index)
   };
   unsigned long long pieces[kRowWarps * kRowPieces];
   unsigned long long reduce[32];
   float reduce_f[32];
   double table[32];
   // written by the blocks of the cluster, each into its own place
-  float part_max[kRowParts], part_min[kRowParts];
+  float part_max[kRowParts];
   unsigned long long part_sum[kRowParts];
   uint32_t part_least[kRowParts], part_most[kRowParts], part_listed[kRowParts];
   // written by one block into all
@@ -268,13 +266,7 @@ struct RowStretch {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // f(step, first element's index, the elements) for this lane's vector of a step; elements outside the row are -inf.
-  template <typename F>
-  __device__ __forceinline__ void at_step(int step, F f) const {
-    const int v = begin + step * 32 + int(threadIdx.x & 31);
-    if (v >= end) return;
-    const uint4 raw = cache != nullptr ? cache[step * 32] : load(v);
-    float l[kPer];
+  static __device__ __forceinline__ void unpack(const uint4& raw, float (&l)[kPer]) {
     if constexpr (sizeof(T) == 4) {
       l[0] = __uint_as_float(raw.x); l[1] = __uint_as_float(raw.y);
       l[2] = __uint_as_float(raw.z); l[3] = __uint_as_float(raw.w);
@@ -285,16 +277,34 @@ struct RowStretch {
       halves(raw.z, l[4], l[5], tag);
       halves(raw.w, l[6], l[7], tag);
     }
+  }
+  // f(first element's index, the elements) for this lane's vector of a step; elements outside the row are -inf.
+  template <typename F>
+  __device__ __forceinline__ void at_step(int step, F f) const {
+    const int v = begin + step * 32 + int(threadIdx.x & 31);
+    if (v >= end) return;
+    float l[kPer];
+    unpack(cache != nullptr ? cache[step * 32] : load(v), l);
     f(uint32_t(v * kPer - lead), l);
   }
-  template <typename F>
-  __device__ __forceinline__ void sweep(F f) const {
-    for (int step = 0; step < steps; ++step)
-      at_step(step, [&](uint32_t index, float(&l)[kPer]) {
+  // f(index, logit) for the elements of a step with test(index, logit). Few of many: a lane takes its next one while
+  // others take theirs, so a step costs as many rounds as one lane has elements, not one for each place.
+  template <typename Test, typename F>
+  __device__ __forceinline__ void some_at_step(int step, Test test, F f) const {
+    at_step(step, [&](uint32_t index, float(&l)[kPer]) {
+      uint32_t hits = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (l[i] > -INFINITY) f(index + i, l[i]);  // neither -inf nor NaN
-      });
+      for (int i = 0; i < kPer; ++i) hits |= test(index + i, l[i]) ? 1u << i : 0u;
+      while (hits != 0) {
+        const int at = __ffs(hits) - 1;
+        hits &= hits - 1;
+        float value = l[0];
+#pragma unroll
+        for (int i = 1; i < kPer; ++i)
+          if (at == i) value = l[i];
+        f(index + at, value);
+      }
+    });
   }
 };
 
@@ -305,42 +315,66 @@ struct RowCluster {
   __device__ __forceinline__ RowShared& of(int part) const { return *group.map_shared_rank(&s, part); }
 };
 
+// The smallest logit whose weight_steps are at least `least` (<= 0), found among all floats up to the largest logit by all lanes of
+// a warp: what a comparison of logits has to use for the comparison of the steps. weight_steps is monotonic.
+__device__ __forceinline__ float logit_from_steps(const RowWeights& w, float largest, double least) {
+  if (w.only_largest) return largest;
+  uint32_t left = kKeyNegInf + 1, right = order_key(largest);
+  while (left < right) {
+    const uint32_t width = (right - left) / 32 + 1;
+    const uint32_t at = left + min(width * (threadIdx.x & 31), right - left);
+    const uint32_t yes = __ballot_sync(0xffffffffu, weight_steps(w, key_to_float(at)) >= least);
+    const uint32_t none = yes != 0 ? __ffs(yes) - 1 : 32u;  // lanes below the border
+    if (none < 32) right = left + min(width * none, right - left);
+    if (none > 0) left = min(left + width * (none - 1) + 1, right);
+  }
+  return key_to_float(right);
+}
+
 struct Crossing {
   uint32_t bin;
   unsigned long long before;  // what lies in the bins ahead of it
   unsigned long long total;
 };
 
-// Sums amount(index, logit) by bin(logit) over the row (elements with bin >= kRowBins are left out) and finds the bin in
-// which target(total) is reached, bin 0 first.
-template <typename T, typename Amount, typename Bin, typename Target>
-__device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStretch<T>& x, Amount amount, Bin bin, Target target) {
+// Sums amount(logit) by bin(logit) over the elements of the row that `active` selects and finds the bin in which target(total) is
+// reached, bin 0 first. The 64-bit sums are kept in two words, the carry passed on by the one who causes it.
+template <typename T, typename Amount, typename Bin, typename Active, typename Target>
+__device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStretch<T>& x, Amount amount, Bin bin,
+                                             Active active, Target target) {
   RowShared& s = c.s;
   __syncthreads();
-  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) s.bins.lo[i] = s.bins.hi[i] = 0;
+  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) s.bins[i] = 0;
   __syncthreads();
-  x.sweep([&](uint32_t index, float l) {
-    const uint32_t b = bin(l);
-    if (b >= uint32_t(kRowBins)) return;
-    const unsigned long long a = amount(index, l);
-    if (a == 0) return;
-    const uint32_t low = uint32_t(a);
-    const uint32_t was = atomicAdd(&s.bins.lo[b], low);
-    const uint32_t high = uint32_t(a >> 32) + (was + low < was ? 1u : 0u);  // the carry goes along
-    if (high != 0) atomicAdd(&s.bins.hi[b], high);
-  });
+  uint32_t* const words = reinterpret_cast<uint32_t*>(s.bins);
+  for (int step = 0; step < x.steps; ++step)
+    x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+#pragma unroll
+      for (int i = 0; i < RowStretch<T>::kPer; ++i) {
+        if (!active(index + i, l[i])) continue;
+        const unsigned long long a = amount(l[i]);
+        uint32_t* const at = words + 2 * bin(l[i]);
+        const uint32_t low = uint32_t(a);
+        const uint32_t was = atomicAdd(at, low);
+        const uint32_t high = uint32_t(a >> 32) + (was + low < was ? 1u : 0u);
+        if (high != 0) atomicAdd(at + 1, high);
+      }
+    });
   c.group.sync();
-  // each block adds up its share of the bins over all blocks; bins_each consecutive ones per thread
+  // each block adds up its share of the bins over all blocks, consecutive ones per thread
   const int share = kRowBins / c.parts;
   const int each = share >= kRowThreads ? share / kRowThreads : 1;
   const int first = c.rank * share + each * int(threadIdx.x);
   unsigned long long sum[kRowBins / kRowThreads] = {}, mine = 0;
   if (each * int(threadIdx.x) < share) {
-    for (int part = 0; part < c.parts; ++part) {
-      const RowShared& other = c.of(part);
 #pragma unroll
-      for (int i = 0; i < kRowBins / kRowThreads; ++i)
-        if (i < each) sum[i] += ((unsigned long long)other.bins.hi[first + i] << 32) + other.bins.lo[first + i];
+    for (int part = 0; part < kRowParts; ++part) {
+      if (part < c.parts) {
+        const RowShared& other = c.of(part);
+#pragma unroll
+        for (int i = 0; i < kRowBins / kRowThreads; ++i)
+          if (i < each) sum[i] += other.bins[first + i];
+      }
     }
 #pragma unroll
     for (int i = 0; i < kRowBins / kRowThreads; ++i) mine += sum[i];
@@ -372,25 +406,27 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
 }
 
 // The place in the order at which the amounts reach `target`, given that this happens among the elements that `active`
-// selects and that `before` lies ahead of them. weight(index, logit): their amounts, equal for equal logits.
+// selects and that `before` lies ahead of them.
 template <typename T, typename Amount, typename Active>
 __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStretch<T>& x, unsigned long long before,
                                              unsigned long long target, Amount amount, Active active) {
   RowShared& s = c.s;
-  uint32_t from = 0, to = 0xffffffffu;  // keys that still matter
+  float from = -INFINITY, to = INFINITY;  // logits that still matter
   for (;;) {
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     uint32_t least = 0xffffffffu, most = 0;
-    x.sweep([&](uint32_t index, float l) {
-      const uint32_t key = order_key(l);
-      if (key < from || key > to || !active(index, l)) return;
-      least = min(least, key);
-      most = max(most, key);
-      const unsigned int at = atomicAdd(&s.listed, 1u);
-      if (at < unsigned(kRowList)) s.list[at] = order_pair(key, index);
-    });
+    for (int step = 0; step < x.steps; ++step)
+      x.some_at_step(
+          step, [&](uint32_t index, float l) { return l >= from && l <= to && active(index, l); },
+          [&](uint32_t index, float l) {
+            const uint32_t key = order_key(l);
+            least = min(least, key);
+            most = max(most, key);
+            const unsigned int at = atomicAdd(&s.listed, 1u);
+            if (at < unsigned(kRowList)) s.list[at] = order_pair(key, index);
+          });
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
     uint32_t* scratch = reinterpret_cast<uint32_t*>(s.reduce);
@@ -399,15 +435,15 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
       scratch[32 + (threadIdx.x >> 5)] = most;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < kRowWarps; ++i) {
-        least = min(least, scratch[i]);
-        most = max(most, scratch[32 + i]);
-      }
-      for (int part = 0; part < c.parts; ++part) {
-        c.of(part).part_least[c.rank] = least;
-        c.of(part).part_most[c.rank] = most;
-        c.of(part).part_listed[c.rank] = s.listed;
+    if (threadIdx.x < 32) {
+      const int i = int(threadIdx.x) < kRowWarps ? int(threadIdx.x) : 0;
+      least = __reduce_min_sync(0xffffffffu, scratch[i]);
+      most = __reduce_max_sync(0xffffffffu, scratch[32 + i]);
+      if (int(threadIdx.x) < c.parts) {
+        RowShared& other = c.of(threadIdx.x);
+        other.part_least[c.rank] = least;
+        other.part_most[c.rank] = most;
+        other.part_listed[c.rank] = s.listed;
       }
     }
     c.group.sync();
@@ -437,12 +473,12 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
         for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
           const int i = i0 + int(threadIdx.x);
           unsigned long long a = 0;
-          if (i < int(n)) a = amount(pair_index(s.list[i]), key_to_float(pair_key(s.list[i])));
+          if (i < int(n)) a = amount(key_to_float(pair_key(s.list[i])));
           unsigned long long sum;
           const unsigned long long place = seen + block_prefix(a, s.reduce, &sum);
           if (a != 0 && place < target && target <= place + a)
             for (int part = 0; part < c.parts; ++part)
-              c.of(part).found_cut = RowCut{pair_key(s.list[i]), pair_index(s.list[i])};
+              c.of(part).found_cut = RowCut{key_to_float(pair_key(s.list[i])), pair_index(s.list[i]) + 1};
           seen += sum;
           if (seen >= target) break;
         }
@@ -452,11 +488,16 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
     }
     if (least == most) {
       // one value: the m-th of its places
-      const unsigned long long each = amount(kNoIndexLimit, key_to_float(least));
-      unsigned long long m = (target - before + each - 1) / each;
-      auto is_one = [&](uint32_t index, float l) { return order_key(l) == least && active(index, l); };
+      const float value = key_to_float(least);
+      const unsigned long long each = amount(value);
+      const unsigned long long m = (target - before + each - 1) / each;
+      auto is_one = [&](uint32_t index, float l) { return l == value && active(index, l); };
       unsigned long long mine = 0;
-      x.sweep([&](uint32_t index, float l) { mine += is_one(index, l); });
+      for (int step = 0; step < x.steps; ++step)
+        x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+#pragma unroll
+          for (int i = 0; i < RowStretch<T>::kPer; ++i) mine += is_one(index + i, l[i]);
+        });
       // in index order: lanes of a step, steps, warps, blocks
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -468,22 +509,22 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
       for (int part = 0; part < c.rank; ++part) ahead += s.part_sum[part];
       if (ahead < m && m <= ahead + mine) {
         for (int step = 0; step < x.steps; ++step) {
-          unsigned long long here = 0;
+          unsigned int here = 0;
           x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
-            for (int i = 0; i < RowStretch<T>::kPer; ++i) here += l[i] > -INFINITY && is_one(index + i, l[i]);
+#pragma unroll
+            for (int i = 0; i < RowStretch<T>::kPer; ++i) here += is_one(index + i, l[i]);
           });
-          unsigned long long inc = here;
+          unsigned int inc = here;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long other = __shfl_up_sync(0xffffffffu, inc, o);
+            const unsigned int other = __shfl_up_sync(0xffffffffu, inc, o);
             if (int(threadIdx.x & 31) >= o) inc += other;
           }
           unsigned long long at = ahead + inc - here;
           if (at < m && m <= at + here)
-            x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
-              for (int i = 0; i < RowStretch<T>::kPer; ++i)
-                if (l[i] > -INFINITY && is_one(index + i, l[i]) && ++at == m)
-                  for (int part = 0; part < c.parts; ++part) c.of(part).found_cut = RowCut{least, index + i};
+            x.some_at_step(step, is_one, [&](uint32_t index, float) {
+              if (++at == m)
+                for (int part = 0; part < c.parts; ++part) c.of(part).found_cut = RowCut{value, index + 1};
             });
           ahead += __shfl_sync(0xffffffffu, inc, 31);
         }
@@ -491,21 +532,20 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
       c.group.sync();
       return s.found_cut;
     }
-    // too many of several values: a finer histogram over their keys (a fraction of 2048 of the range at least)
+    // too many of several values: a finer histogram over their keys
     int shift = 0;
     while (((most - least) >> shift) >= uint32_t(kRowBins)) ++shift;
-    const uint32_t a = least, b = most;
+    const float low = key_to_float(least), high = key_to_float(most);
+    const uint32_t top_key = most;
     const Crossing at = find_bin(
-        c, x, [&](uint32_t index, float l) { return active(index, l) ? amount(index, l) : 0ull; },
-        [&](float l) {
-          const uint32_t key = order_key(l);
-          return key >= a && key <= b ? (b - key) >> shift : uint32_t(kRowBins);
-        },
+        c, x, amount, [&](float l) { return (top_key - order_key(l)) >> shift; },
+        [&](uint32_t index, float l) { return l >= low && l <= high && active(index, l); },
         [&](unsigned long long) { return target - before; });
     before += at.before;
-    to = b - (at.bin << shift);
+    const uint32_t to_key = most - (at.bin << shift);
     const uint32_t down = (1u << shift) - 1u;
-    from = to - a > down ? to - down : a;
+    to = key_to_float(to_key);
+    from = key_to_float(to_key - least > down ? to_key - down : least);
   }
 }
 
@@ -520,12 +560,13 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   if (by_list(p, set)) return;  // the whole cluster
   RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kPer = RowStretch<T>::kPer;
 
   RowStretch<T> x;
   x.row = logits + r * ld;
   x.vocab = vocab;
   x.lead = int((reinterpret_cast<uintptr_t>(x.row) & 15u) / sizeof(T));
-  const int vectors = int(((long long)vocab + x.lead + RowStretch<T>::kPer - 1) / RowStretch<T>::kPer);
+  const int vectors = int(((long long)vocab + x.lead + kPer - 1) / kPer);
   const int per_block = (vectors + parts - 1) / parts;
   const int per_warp = (per_block + kRowThreads - 1) / kRowThreads * 32;
   const int block_begin = min(c.rank * per_block, vectors), block_end = min(block_begin + per_block, vectors);
@@ -539,8 +580,8 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     for (int step = 0; step < x.steps; ++step) {
       const int v = x.begin + step * 32 + lane;
       if (v >= x.end) break;
-      const long long e = (long long)v * RowStretch<T>::kPer - x.lead;
-      if (e >= 0 && e + RowStretch<T>::kPer <= (long long)vocab) copy_async16(cache + step * 32, x.row + e);
+      const long long e = (long long)v * kPer - x.lead;
+      if (e >= 0 && e + kPer <= (long long)vocab) copy_async16(cache + step * 32, x.row + e);
       else cache[step * 32] = x.load(v);
     }
     copy_async_wait();  // a lane reads back what it has copied itself
@@ -548,76 +589,79 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   }
   if (threadIdx.x < 32) s.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
 
-  // ---- the largest logit, and the smallest that may be drawn
-  float top = -INFINITY, low = INFINITY;
-  x.sweep([&](uint32_t, float l) {
-    top = fmaxf(top, l);
-    low = fminf(low, l);
-  });
+  // ---- the largest logit
+  float top = -INFINITY;
+  for (int step = 0; step < x.steps; ++step)
+    x.at_step(step, [&](uint32_t, float(&l)[kPer]) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) top = fmaxf(top, l[i]);  // passes a NaN over
+    });
   top = block_max(top, s.reduce_f);
-  low = -block_max(-low, s.reduce_f);
-  if (int(threadIdx.x) < parts) {
-    c.of(threadIdx.x).part_max[c.rank] = top;
-    c.of(threadIdx.x).part_min[c.rank] = low;
-  }
+  if (int(threadIdx.x) < parts) c.of(threadIdx.x).part_max[c.rank] = top;
   c.group.sync();
-  for (int part = 0; part < parts; ++part) {
-    top = fmaxf(top, s.part_max[part]);
-    low = fminf(low, s.part_min[part]);
-  }
+  for (int part = 0; part < parts; ++part) top = fmaxf(top, s.part_max[part]);
   if (!(top > -INFINITY)) {
     if (c.rank == 0 && threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
     return;  // the whole cluster; nothing of it is read any more
   }
   const RowWeights w = row_weights(p, set, top, s.table);
-  auto weight = [&](float l) { return row_weight(w, l); };
+  auto weight = [&](float l) { return w.only_largest ? 1ull << 32 : weight_of_steps(w, weight_steps(w, l)); };
 
-  // ---- the cuts. First bins: equal steps of the logit below the largest, down to where weights round to nothing (what
-  // is below shares the last bin).
-  const float reach = float(46.0 * 0.69314718055994531 * set.temperature);
-  const bool all_in_reach = top - low <= reach;
-  const float range = fminf(top - low, reach);
-  const float per_bin = w.only_largest ? 1.f : (range > 0.f ? float(kRowBins) / range : 0.f);
-  auto bin = [&](float l) {
-    return l == top ? 0u : uint32_t(min(kRowBins - 1, __float2int_rz((top - l) * per_bin)));
+  // ---- the cuts, among the logits that have any weight. First bins: equal steps of the logit below the largest.
+  const float weighty = logit_from_steps(w, top, kNoWeight);
+  RowCut cut{weighty, kNoEnd};
+  const float per_bin = w.only_largest ? 1.f : float(double(kRowBins) / (46.5 * 0.69314718055994531 * set.temperature));
+  auto place = [&](float l) { return l == top ? 0.f : (top - l) * per_bin; };
+  auto bin = [&](float l) { return uint32_t(min(kRowBins - 1, __float2int_rz(place(l)))); };
+  auto in_bin = [&](uint32_t b, float l) {
+    const float v = place(l);
+    return v >= float(b) && (v < float(b + 1) || b == uint32_t(kRowBins - 1));
   };
-  RowCut cut{0u, kNoIndexLimit};
   if (set.top_k > 0 && set.top_k < (long long)vocab) {
     const unsigned long long k = (unsigned long long)set.top_k;
-    auto one = [](uint32_t, float) { return 1ull; };
-    const Crossing at = find_bin(c, x, one, bin, [&](unsigned long long total) { return total < k ? total : k; });
-    // a cut among weights of nothing changes nothing
-    if (at.total > k && (all_in_reach || at.bin + 1 < uint32_t(kRowBins)))
-      cut = find_place(c, x, at.before, k, one, [&](uint32_t, float l) { return bin(l) == at.bin; });
+    auto one = [](float) { return 1ull; };
+    auto all = [&](uint32_t, float l) { return l >= weighty; };
+    const Crossing at = find_bin(c, x, one, bin, all, [&](unsigned long long total) { return total < k ? total : k; });
+    if (at.total > k)
+      cut = find_place(c, x, at.before, k, one, [&](uint32_t, float l) { return l >= weighty && in_bin(at.bin, l); });
   }
   if (set.top_p < 1.0) {
     const RowCut outer = cut;
-    auto amount = [&](uint32_t index, float l) { return inside(outer, order_key(l), index) ? weight(l) : 0ull; };
     unsigned long long target = 0;
-    const Crossing at = find_bin(c, x, amount, bin, [&](unsigned long long total) {
-      target = mass_target(set.top_p, total);
-      return target;
-    });
-    cut = find_place(c, x, at.before, target, [&](uint32_t, float l) { return weight(l); },
-                     [&](uint32_t index, float l) { return bin(l) == at.bin && inside(outer, order_key(l), index); });
+    const Crossing at = find_bin(
+        c, x, weight, bin, [&](uint32_t index, float l) { return inside(outer, l, index); },
+        [&](unsigned long long total) {
+          target = mass_target(set.top_p, total);
+          return target;
+        });
+    cut = find_place(c, x, at.before, target, weight,
+                     [&](uint32_t index, float l) { return in_bin(at.bin, l) && inside(outer, l, index); });
+  }
+  const bool few = cut.value > weighty || set.lowest > -INFINITY;
+  if (set.lowest > -INFINITY) {
+    const float lowest = logit_from_steps(w, top, set.lowest);
+    if (lowest > cut.value) cut = RowCut{lowest, kNoEnd};
   }
 
   // ---- the kept weights, piece by piece
-  auto kept = [&](uint32_t index, float l) {
-    if (!(l > -INFINITY) || !inside(cut, order_key(l), index)) return 0ull;
-    if (!w.only_largest && !(weight_steps(w, l) >= set.lowest)) return 0ull;
-    return weight(l);
+  auto kept = [&](uint32_t index, float l) { return inside(cut, l, index); };
+  auto kept_at_step = [&](int step) {
+    unsigned long long sum = 0;
+    if (few)
+      x.some_at_step(step, kept, [&](uint32_t, float l) { sum += weight(l); });
+    else
+      x.at_step(step, [&](uint32_t index, float(&l)[kPer]) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += kept(index + i, l[i]) ? weight(l[i]) : 0ull;
+      });
+    return sum;
   };
   __syncthreads();
   for (int i = threadIdx.x; i < kRowWarps * kRowPieces; i += kRowThreads) s.pieces[i] = 0;
   __syncthreads();
   for (int step0 = 0; step0 < x.steps; step0 += x.per_piece) {
     unsigned long long mine = 0;
-    for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step)
-      x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
-#pragma unroll
-        for (int i = 0; i < RowStretch<T>::kPer; ++i) mine += kept(index + i, l[i]);
-      });
+    for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step) mine += kept_at_step(step);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) s.pieces[warp * kRowPieces + step0 / x.per_piece] = mine;
@@ -653,11 +697,7 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const int step0 = int(s.piece) % kRowPieces * x.per_piece;
   before = s.piece_before;
   for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step) {
-    unsigned long long here = 0;
-    x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
-#pragma unroll
-      for (int i = 0; i < RowStretch<T>::kPer; ++i) here += kept(index + i, l[i]);
-    });
+    const unsigned long long here = kept_at_step(step);
     unsigned long long inc = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -666,15 +706,13 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     }
     unsigned long long at = before + inc - here;
     if (at <= goal && goal < at + here)
-      x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
-        for (int i = 0; i < RowStretch<T>::kPer; ++i) {
-          const unsigned long long a = kept(index + i, l[i]);
-          if (a != 0 && at <= goal && goal < at + a) {
-            tokens[r] = index + i;
-            logprobs[r] = log_share(p, set, w, l[i], a, total);
-          }
-          at += a;
+      x.some_at_step(step, kept, [&](uint32_t index, float l) {
+        const unsigned long long a = weight(l);
+        if (at <= goal && goal < at + a) {
+          tokens[r] = index;
+          logprobs[r] = log_share(p, set, w, l, a, total);
         }
+        at += a;
       });
     before += __shfl_sync(0xffffffffu, inc, 31);
   }

@@ -138,21 +138,27 @@ constexpr double kStepLn2 = 0.021660849392498290;  // ln(2) / 32
 __device__ __forceinline__ double weight_steps(const RowWeights& w, float logit) {
   return (double(logit) - w.largest) * w.steps;
 }
-__device__ __forceinline__ unsigned long long row_weight(const RowWeights& w, float logit) {
-  if (w.only_largest) return double(logit) == w.largest ? 1ull << 32 : 0ull;
-  const double t = weight_steps(w, logit);
-  if (!(t > -32.0 * (kWeightBits + 2))) return 0ull;  // rounds to nothing; also -inf and NaN
-  const double shifted = t + 6755399441055744.0;      // 1.5 * 2^52: the integer part ends up in the low word
+// Steps below which a weight rounds to nothing.
+constexpr double kNoWeight = -32.0 * (kWeightBits + 2);
+// The weight of `steps` in [kNoWeight, 0].
+__device__ __forceinline__ unsigned long long weight_of_steps(const RowWeights& w, double steps) {
+  const double shifted = steps + 6755399441055744.0;  // 1.5 * 2^52: the integer part ends up in the low word
   const int n = __double2loint(shifted);
-  const double x = (t - (shifted - 6755399441055744.0)) * kStepLn2;
-  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(x, p, 1.0 / 6.0);
-  p = fma(x, p, 0.5);
-  p = fma(x, p, 1.0);
-  p = fma(x, p, 1.0);
+  const double y = steps - (shifted - 6755399441055744.0);  // 2^(y / 32), |y| <= 1/2, by its series in y ln(2) / 32
+  constexpr double c = kStepLn2;
+  double p = fma(y, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+  p = fma(y, p, c * c * c / 6.0);
+  p = fma(y, p, c * c / 2.0);
+  p = fma(y, p, c);
+  p = fma(y, p, 1.0);
   p *= w.table[n & 31];
   p = __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
   return (unsigned long long)(__double_as_longlong(p + w.to_int) - __double_as_longlong(w.to_int));
+}
+__device__ __forceinline__ unsigned long long row_weight(const RowWeights& w, float logit) {
+  if (w.only_largest) return double(logit) == w.largest ? 1ull << 32 : 0ull;
+  const double steps = weight_steps(w, logit);
+  return steps >= kNoWeight ? weight_of_steps(w, steps) : 0ull;  // also 0 for -inf and NaN
 }
 
 }  // namespace lce
