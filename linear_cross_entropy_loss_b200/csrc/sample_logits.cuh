@@ -42,7 +42,7 @@ __device__ __forceinline__ RowSettings row_settings(const SampleParams& p, long 
   s.top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   s.top_p = p.top_p ? double(p.top_p[r]) : p.top_p_all;
   const double min_p = p.min_p ? double(p.min_p[r]) : p.min_p_all;
-  s.lowest = min_p > 0.0 ? 32.0 * log2(fmin(min_p, 1.0)) : -INFINITY;
+  s.lowest = min_p > 0.0 ? kSteps * log2(fmin(min_p, 1.0)) : -INFINITY;
   s.u = p.u_is_double ? reinterpret_cast<const double*>(p.u)[r] : double(reinterpret_cast<const float*>(p.u)[r]);
   s.u = s.u > 0.0 ? fmin(s.u, 1.0) : 0.0;
   s.greedy = !(s.temperature > 0.0);
@@ -62,7 +62,7 @@ __device__ __forceinline__ RowWeights row_weights(const SampleParams& p, const R
   RowWeights w;
   w.largest = largest;
   w.only_largest = largest == INFINITY;
-  w.steps = fmin(46.166241308446828 / s.temperature, 1e300);  // 32 log2(e) / T
+  w.steps = fmin(1.0 / (kStepLn2 * s.temperature), 1e300);
   w.to_int = exp2(double(52 - p.weight_bits));
   w.table = table;
   return w;
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kTopThreads, 4)
 sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int parts, const SampleParams p,
                    long long* __restrict__ tokens, float* __restrict__ logprobs) {
   __shared__ TopShared s;
-  __shared__ double table[32];
+  __shared__ double table[kSteps];
   __shared__ unsigned long long reduce[32];
   const long long r = blockIdx.x / parts;
   const int part = int(blockIdx.x % parts);
@@ -107,7 +107,7 @@ sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, i
   const int share = (row.groups + parts - 1) / parts;
   const int v0 = min(part * share, row.groups), v1 = min(v0 + share, row.groups);
   float ref, sum;
-  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  if (threadIdx.x < kSteps) table[threadIdx.x] = exp2(double(threadIdx.x) / kSteps);
   stream_top<T, false, Nan::kNever>(s, row, v0, v1, k, 1.f, ref, sum);
   merge_lists(s, k, parts);
   if (part != 0) return;
@@ -205,18 +205,21 @@ struct RowCut {
 };
 constexpr uint32_t kNoEnd = 0xffffffffu;
 __device__ __forceinline__ bool inside(const RowCut& c, float l, uint32_t index) {
-  return l > c.value || (l == c.value && index < c.end);  // never a NaN
+  if (!(l >= c.value)) return false;  // also a NaN
+  return c.end == kNoEnd || l > c.value || index < c.end;
 }
 
 struct RowShared {
   union {
-    unsigned long long bins[kRowBins];
+    struct {
+      uint32_t low[kRowBins], high[kRowBins];  // a 64-bit sum in two words
+    } bins;
     unsigned long long list[kRowList];  // the elements of one bin, order_pair(key, index)
   };
   unsigned long long pieces[kRowWarps * kRowPieces];
   unsigned long long reduce[32];
   float reduce_f[32];
-  double table[32];
+  double table[kSteps];
   // written by the blocks of the cluster, each into its own place
   float part_max[kRowParts];
   unsigned long long part_sum[kRowParts];
@@ -252,6 +255,7 @@ struct RowStretch {
   int steps;       // of 32 vectors
   int per_piece;   // steps of a piece
   uint4* cache;    // this lane's vector of step 0, or null: the row is read from global memory each time
+  const T* flat;   // element e of this block's stretch at flat[e], in the cache or in the row
 
   __device__ __forceinline__ uint4 load(int v) const {
     const long long e = (long long)v * kPer - lead;
@@ -278,6 +282,35 @@ struct RowStretch {
       halves(raw.w, l[6], l[7], tag);
     }
   }
+  // The largest of this lane's elements, -inf where there is none (a NaN is none).
+  __device__ __forceinline__ float largest() const {
+    constexpr uint32_t none = sizeof(T) == 4 ? RowGroups<T>::kNegInf : RowGroups<T>::kNegInf * 0x10001u;
+    uint4 m = make_uint4(none, none, none, none);
+    for (int step = 0; step < steps; ++step) {
+      const int v = begin + step * 32 + int(threadIdx.x & 31);
+      if (v >= end) break;
+      const uint4 raw = cache != nullptr ? cache[step * 32] : load(v);
+      m.x = larger_of_word(m.x, raw.x);
+      m.y = larger_of_word(m.y, raw.y);
+      m.z = larger_of_word(m.z, raw.z);
+      m.w = larger_of_word(m.w, raw.w);
+    }
+    float l[kPer];
+    unpack(m, l);
+    float r = l[0];
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) r = fmaxf(r, l[i]);
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t larger_of_word(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    } else {
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2 r = __hmax2(*reinterpret_cast<T2*>(&a), *reinterpret_cast<T2*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&r);
+    }
+  }
   // f(first element's index, the elements) for this lane's vector of a step; elements outside the row are -inf.
   template <typename F>
   __device__ __forceinline__ void at_step(int step, F f) const {
@@ -287,14 +320,14 @@ struct RowStretch {
     unpack(cache != nullptr ? cache[step * 32] : load(v), l);
     f(uint32_t(v * kPer - lead), l);
   }
-  // f(index, logit) for the elements of a step with test(index, logit). Few of many: a lane takes its next one while
-  // others take theirs, so a step costs as many rounds as one lane has elements, not one for each place.
+  // f(index, logit) for the elements of a step with test(logit). Few of many: a lane takes its next one while others
+  // take theirs, so a step costs as many rounds as one lane has elements, not one for each place.
   template <typename Test, typename F>
   __device__ __forceinline__ void some_at_step(int step, Test test, F f) const {
     at_step(step, [&](uint32_t index, float(&l)[kPer]) {
       uint32_t hits = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) hits |= test(index + i, l[i]) ? 1u << i : 0u;
+      for (int i = 0; i < kPer; ++i) hits |= test(l[i]) ? 1u << i : 0u;
       while (hits != 0) {
         const int at = __ffs(hits) - 1;
         hits &= hits - 1;
@@ -312,23 +345,39 @@ struct RowCluster {
   cooperative_groups::cluster_group group;
   int rank, parts;
   RowShared& s;
+  float top;  // the row's largest logit
   __device__ __forceinline__ RowShared& of(int part) const { return *group.map_shared_rank(&s, part); }
 };
 
-// The smallest logit whose weight_steps are at least `least` (<= 0), found among all floats up to the largest logit by all lanes of
-// a warp: what a comparison of logits has to use for the comparison of the steps. weight_steps is monotonic.
-__device__ __forceinline__ float logit_from_steps(const RowWeights& w, float largest, double least) {
-  if (w.only_largest) return largest;
+// The smallest float up to `largest` for which holds(float) is true; it is true for `largest` and, once true, for all
+// larger ones. All lanes of a warp take part: they try the floats around the estimate, or, where the border is not
+// among them, cut the whole range into 32 parts at a time.
+template <typename Holds>
+__device__ __forceinline__ float border_of(float estimate, float largest, Holds holds) {
+  const int lane = int(threadIdx.x & 31);
   uint32_t left = kKeyNegInf + 1, right = order_key(largest);
+  {
+    const uint32_t mid = min(max(order_key(estimate), left + 16), right);
+    const uint32_t at = min(mid - 16 + uint32_t(lane), right);
+    const uint32_t yes = __ballot_sync(0xffffffffu, holds(key_to_float(at)));
+    if (yes != 0 && (yes & 1u) == 0) return key_to_float(min(mid - 16 + uint32_t(__ffs(yes) - 1), right));
+  }
   while (left < right) {
     const uint32_t width = (right - left) / 32 + 1;
-    const uint32_t at = left + min(width * (threadIdx.x & 31), right - left);
-    const uint32_t yes = __ballot_sync(0xffffffffu, weight_steps(w, key_to_float(at)) >= least);
+    const uint32_t at = left + min(width * uint32_t(lane), right - left);
+    const uint32_t yes = __ballot_sync(0xffffffffu, holds(key_to_float(at)));
     const uint32_t none = yes != 0 ? __ffs(yes) - 1 : 32u;  // lanes below the border
     if (none < 32) right = left + min(width * none, right - left);
     if (none > 0) left = min(left + width * (none - 1) + 1, right);
   }
   return key_to_float(right);
+}
+// The smallest logit whose weight_steps are at least `least` (<= 0): what a comparison of logits has to use for the
+// comparison of the steps.
+__device__ __forceinline__ float logit_from_steps(const RowWeights& w, double inv_steps, float largest, double least) {
+  if (w.only_largest) return largest;
+  return border_of(float(w.largest + least * inv_steps), largest,
+                   [&](float l) { return weight_steps(w, l) >= least; });
 }
 
 struct Crossing {
@@ -344,20 +393,25 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
                                              Active active, Target target) {
   RowShared& s = c.s;
   __syncthreads();
-  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) s.bins[i] = 0;
+  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) s.bins.low[i] = s.bins.high[i] = 0;
   __syncthreads();
-  uint32_t* const words = reinterpret_cast<uint32_t*>(s.bins);
   for (int step = 0; step < x.steps; ++step)
     x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
 #pragma unroll
       for (int i = 0; i < RowStretch<T>::kPer; ++i) {
-        if (!active(index + i, l[i])) continue;
-        const unsigned long long a = amount(l[i]);
-        uint32_t* const at = words + 2 * bin(l[i]);
+        // (a weight is taken for every place, of the largest logit where there is nothing to add: the chains of
+        // a vector's elements then run side by side)
+        const bool is = active(index + i, l[i]);
+        const float safe = is ? l[i] : c.top;
+        const unsigned long long a = amount(safe);
+        const uint32_t at = bin(safe);
         const uint32_t low = uint32_t(a);
-        const uint32_t was = atomicAdd(at, low);
-        const uint32_t high = uint32_t(a >> 32) + (was + low < was ? 1u : 0u);
-        if (high != 0) atomicAdd(at + 1, high);
+        uint32_t high = uint32_t(a >> 32);
+        if (is) {
+          const uint32_t was = atomicAdd(&s.bins.low[at], low);
+          high += was + low < was ? 1u : 0u;
+          if (high != 0) atomicAdd(&s.bins.high[at], high);
+        }
       }
     });
   c.group.sync();
@@ -373,7 +427,7 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
         const RowShared& other = c.of(part);
 #pragma unroll
         for (int i = 0; i < kRowBins / kRowThreads; ++i)
-          if (i < each) sum[i] += other.bins[first + i];
+          if (i < each) sum[i] += ((unsigned long long)other.bins.high[first + i] << 32) + other.bins.low[first + i];
       }
     }
 #pragma unroll
@@ -405,13 +459,20 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
   return found;
 }
 
-// The place in the order at which the amounts reach `target`, given that this happens among the elements that `active`
-// selects and that `before` lies ahead of them.
-template <typename T, typename Amount, typename Active>
+// The logits of a bin.
+struct RowBin {
+  float from, below;  // below: NaN where it goes up to +inf
+  __device__ __forceinline__ bool has(float l) const { return l >= from && !(l >= below); }
+};
+
+// The place in the order at which the amounts reach `target`, given that this happens among the elements of `bin` inside
+// `outer` and that `before` lies ahead of them.
+template <typename T, typename Amount>
 __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStretch<T>& x, unsigned long long before,
-                                             unsigned long long target, Amount amount, Active active) {
+                                             unsigned long long target, Amount amount, const RowBin bin,
+                                             const RowCut outer) {
   RowShared& s = c.s;
-  float from = -INFINITY, to = INFINITY;  // logits that still matter
+  float from = bin.from, to = INFINITY;  // logits that still matter
   for (;;) {
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;
@@ -419,8 +480,9 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
     uint32_t least = 0xffffffffu, most = 0;
     for (int step = 0; step < x.steps; ++step)
       x.some_at_step(
-          step, [&](uint32_t index, float l) { return l >= from && l <= to && active(index, l); },
+          step, [&](float l) { return l >= from && !(l >= bin.below); },
           [&](uint32_t index, float l) {
+            if (l > to || !inside(outer, l, index)) return;
             const uint32_t key = order_key(l);
             least = min(least, key);
             most = max(most, key);
@@ -456,31 +518,49 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
       most = max(most, s.part_most[part]);
     }
     if (n <= unsigned(kRowList)) {
-      // few enough: the first block takes them all, sorts them and adds their amounts up
+      // few enough: the first block takes them all, in any order
       if (c.rank == 0) {
-        unsigned int at = s.listed;
-        for (int part = 1; part < c.parts; ++part) {
-          const RowShared& other = c.of(part);
-          const unsigned int more = s.part_listed[part];
-          for (unsigned int i = threadIdx.x; i < more; i += kRowThreads) s.list[at + i] = other.list[i];
-          at += more;
+        const unsigned int own = s.listed;
+        for (unsigned int i = own + threadIdx.x; i < n; i += kRowThreads) {
+          unsigned int at = i - own;
+          int part = 1;
+          while (at >= s.part_listed[part]) at -= s.part_listed[part++];
+          s.list[i] = c.of(part).list[at];
         }
-        int padded = 2;
-        while (padded < int(n)) padded <<= 1;
-        for (int i = int(n) + int(threadIdx.x); i < padded; i += kRowThreads) s.list[i] = 0;
-        block_sort_descending(s.list, padded);
-        unsigned long long seen = before;
-        for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
-          const int i = i0 + int(threadIdx.x);
-          unsigned long long a = 0;
-          if (i < int(n)) a = amount(key_to_float(pair_key(s.list[i])));
-          unsigned long long sum;
-          const unsigned long long place = seen + block_prefix(a, s.reduce, &sum);
-          if (a != 0 && place < target && target <= place + a)
-            for (int part = 0; part < c.parts; ++part)
-              c.of(part).found_cut = RowCut{key_to_float(pair_key(s.list[i])), pair_index(s.list[i]) + 1};
-          seen += sum;
-          if (seen >= target) break;
+        auto found = [&](unsigned long long e) {
+          for (int part = 0; part < c.parts; ++part)
+            c.of(part).found_cut = RowCut{key_to_float(pair_key(e)), pair_index(e) + 1};
+        };
+        if (n <= unsigned(kRowWarps * kRowPieces) / 8) {
+          // every element's place is the sum of the amounts ahead of it
+          unsigned long long mine = 0, a = 0, place = before;
+          __syncthreads();
+          if (threadIdx.x < n) {
+            mine = s.list[threadIdx.x];
+            a = amount(key_to_float(pair_key(mine)));
+            s.pieces[threadIdx.x] = a;
+          }
+          __syncthreads();
+          if (threadIdx.x < n) {
+            for (unsigned int i = 0; i < n; ++i) place += s.list[i] > mine ? s.pieces[i] : 0ull;
+            if (a != 0 && place < target && target <= place + a) found(mine);
+          }
+        } else {
+          int padded = 2;
+          while (padded < int(n)) padded <<= 1;
+          for (int i = int(n) + int(threadIdx.x); i < padded; i += kRowThreads) s.list[i] = 0;
+          block_sort_descending(s.list, padded);
+          unsigned long long seen = before;
+          for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
+            const int i = i0 + int(threadIdx.x);
+            unsigned long long a = 0;
+            if (i < int(n)) a = amount(key_to_float(pair_key(s.list[i])));
+            unsigned long long sum;
+            const unsigned long long place = seen + block_prefix(a, s.reduce, &sum);
+            if (a != 0 && place < target && target <= place + a) found(s.list[i]);
+            seen += sum;
+            if (seen >= target) break;
+          }
         }
       }
       c.group.sync();
@@ -491,7 +571,7 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
       const float value = key_to_float(least);
       const unsigned long long each = amount(value);
       const unsigned long long m = (target - before + each - 1) / each;
-      auto is_one = [&](uint32_t index, float l) { return l == value && active(index, l); };
+      auto is_one = [&](uint32_t index, float l) { return l == value && inside(outer, l, index); };
       unsigned long long mine = 0;
       for (int step = 0; step < x.steps; ++step)
         x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
@@ -522,8 +602,8 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
           }
           unsigned long long at = ahead + inc - here;
           if (at < m && m <= at + here)
-            x.some_at_step(step, is_one, [&](uint32_t index, float) {
-              if (++at == m)
+            x.some_at_step(step, [&](float l) { return l == value; }, [&](uint32_t index, float l) {
+              if (is_one(index, l) && ++at == m)
                 for (int part = 0; part < c.parts; ++part) c.of(part).found_cut = RowCut{value, index + 1};
             });
           ahead += __shfl_sync(0xffffffffu, inc, 31);
@@ -539,7 +619,7 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
     const uint32_t top_key = most;
     const Crossing at = find_bin(
         c, x, amount, [&](float l) { return (top_key - order_key(l)) >> shift; },
-        [&](uint32_t index, float l) { return l >= low && l <= high && active(index, l); },
+        [&](uint32_t index, float l) { return l >= low && l <= high && inside(outer, l, index); },
         [&](unsigned long long) { return target - before; });
     before += at.before;
     const uint32_t to_key = most - (at.bin << shift);
@@ -558,7 +638,7 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const long long r = blockIdx.x / parts;
   const RowSettings set = row_settings(p, r);
   if (by_list(p, set)) return;  // the whole cluster
-  RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s};
+  RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s, -INFINITY};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPer = RowStretch<T>::kPer;
 
@@ -575,8 +655,11 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   x.steps = (x.end - x.begin + 31) / 32;
   x.per_piece = (per_warp / 32 + kRowPieces - 1) / kRowPieces;
   x.cache = nullptr;
+  x.flat = x.row;
   if (cache_vectors > 0) {
-    uint4* cache = reinterpret_cast<uint4*>(dynamic + (sizeof(RowShared) + 15) / 16 * 16) + (x.begin - block_begin) + lane;
+    uint4* const block_cache = reinterpret_cast<uint4*>(dynamic + (sizeof(RowShared) + 15) / 16 * 16);
+    uint4* const cache = block_cache + (x.begin - block_begin) + lane;
+    x.flat = reinterpret_cast<const T*>(block_cache) + (x.lead - (long long)block_begin * kPer);
     for (int step = 0; step < x.steps; ++step) {
       const int v = x.begin + step * 32 + lane;
       if (v >= x.end) break;
@@ -587,19 +670,15 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     copy_async_wait();  // a lane reads back what it has copied itself
     x.cache = cache;
   }
-  if (threadIdx.x < 32) s.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  if (threadIdx.x < kSteps) s.table[threadIdx.x] = exp2(double(threadIdx.x) / kSteps);
 
   // ---- the largest logit
-  float top = -INFINITY;
-  for (int step = 0; step < x.steps; ++step)
-    x.at_step(step, [&](uint32_t, float(&l)[kPer]) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) top = fmaxf(top, l[i]);  // passes a NaN over
-    });
+  float top = x.largest();  // passes NaN over
   top = block_max(top, s.reduce_f);
   if (int(threadIdx.x) < parts) c.of(threadIdx.x).part_max[c.rank] = top;
   c.group.sync();
   for (int part = 0; part < parts; ++part) top = fmaxf(top, s.part_max[part]);
+  c.top = top;
   if (!(top > -INFINITY)) {
     if (c.rank == 0 && threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
     return;  // the whole cluster; nothing of it is read any more
@@ -608,22 +687,25 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   auto weight = [&](float l) { return w.only_largest ? 1ull << 32 : weight_of_steps(w, weight_steps(w, l)); };
 
   // ---- the cuts, among the logits that have any weight. First bins: equal steps of the logit below the largest.
-  const float weighty = logit_from_steps(w, top, kNoWeight);
+  const double inv_steps = set.temperature * kStepLn2;
+  const float weighty = logit_from_steps(w, inv_steps, top, kNoWeight);
   RowCut cut{weighty, kNoEnd};
-  const float per_bin = w.only_largest ? 1.f : float(double(kRowBins) / (46.5 * 0.69314718055994531 * set.temperature));
+  const float per_bin = w.only_largest ? 1.f : float(double(kRowBins) / ((kWeightBits + 2.5) * kLn2 * set.temperature));
   auto place = [&](float l) { return l == top ? 0.f : (top - l) * per_bin; };
   auto bin = [&](float l) { return uint32_t(min(kRowBins - 1, __float2int_rz(place(l)))); };
-  auto in_bin = [&](uint32_t b, float l) {
-    const float v = place(l);
-    return v >= float(b) && (v < float(b + 1) || b == uint32_t(kRowBins - 1));
+  // a bin goes from the smallest logit that lies ahead of the next bin up to, and without, its own border
+  auto logits_of = [&](uint32_t b) {
+    auto border = [&](uint32_t first) {
+      return border_of(top - float(first) / per_bin, top, [&](float l) { return place(l) < float(first); });
+    };
+    return RowBin{border(b + 1), b > 0 ? border(b) : __uint_as_float(0x7fc00000u)};
   };
   if (set.top_k > 0 && set.top_k < (long long)vocab) {
     const unsigned long long k = (unsigned long long)set.top_k;
     auto one = [](float) { return 1ull; };
     auto all = [&](uint32_t, float l) { return l >= weighty; };
     const Crossing at = find_bin(c, x, one, bin, all, [&](unsigned long long total) { return total < k ? total : k; });
-    if (at.total > k)
-      cut = find_place(c, x, at.before, k, one, [&](uint32_t, float l) { return l >= weighty && in_bin(at.bin, l); });
+    if (at.total > k) cut = find_place(c, x, at.before, k, one, logits_of(at.bin), cut);
   }
   if (set.top_p < 1.0) {
     const RowCut outer = cut;
@@ -634,37 +716,82 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
           target = mass_target(set.top_p, total);
           return target;
         });
-    cut = find_place(c, x, at.before, target, weight,
-                     [&](uint32_t index, float l) { return in_bin(at.bin, l) && inside(outer, l, index); });
+    cut = find_place(c, x, at.before, target, weight, logits_of(at.bin), outer);
   }
   const bool few = cut.value > weighty || set.lowest > -INFINITY;
   if (set.lowest > -INFINITY) {
-    const float lowest = logit_from_steps(w, top, set.lowest);
+    const float lowest = logit_from_steps(w, inv_steps, top, set.lowest);
     if (lowest > cut.value) cut = RowCut{lowest, kNoEnd};
   }
 
-  // ---- the kept weights, piece by piece
+  // ---- the kept weights, piece by piece in index order. Where a cut leaves few, a warp first moves them together
+  // (up to kCompact of them), so that a piece is 32 kept elements, one per lane.
   auto kept = [&](uint32_t index, float l) { return inside(cut, l, index); };
   auto kept_at_step = [&](int step) {
     unsigned long long sum = 0;
-    if (few)
-      x.some_at_step(step, kept, [&](uint32_t, float l) { sum += weight(l); });
-    else
-      x.at_step(step, [&](uint32_t index, float(&l)[kPer]) {
+    x.at_step(step, [&](uint32_t index, float(&l)[kPer]) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += kept(index + i, l[i]) ? weight(l[i]) : 0ull;
-      });
+      for (int i = 0; i < kPer; ++i) {
+        const bool is = kept(index + i, l[i]);
+        const unsigned long long a = weight(is ? l[i] : top);
+        sum += is ? a : 0ull;
+      }
+    });
     return sum;
   };
+  constexpr int kCompact = 2 * kRowList / kRowWarps;
+  uint32_t* const together = reinterpret_cast<uint32_t*>(s.list) + warp * kCompact;  // their indices, ascending
+  int n_kept = few ? 0 : kCompact + 1;
   __syncthreads();
   for (int i = threadIdx.x; i < kRowWarps * kRowPieces; i += kRowThreads) s.pieces[i] = 0;
   __syncthreads();
-  for (int step0 = 0; step0 < x.steps; step0 += x.per_piece) {
+  for (int step = 0; step < x.steps && n_kept <= kCompact; ++step) {
+    uint32_t hits = 0, first = 0;
+    x.at_step(step, [&](uint32_t index, float(&l)[kPer]) {
+      first = index;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) hits |= l[i] >= cut.value ? 1u << i : 0u;
+      if (cut.end != kNoEnd) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (l[i] == cut.value && index + i >= cut.end) hits &= ~(1u << i);
+      }
+    });
+    if (!__any_sync(0xffffffffu, hits != 0)) continue;
+    int inc = __popc(hits);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += other;
+    }
+    int at = n_kept + inc - __popc(hits);
+    n_kept += __shfl_sync(0xffffffffu, inc, 31);
+    if (n_kept > kCompact) break;
+    while (hits != 0) {
+      together[at++] = first + uint32_t(__ffs(hits) - 1);
+      hits &= hits - 1;
+    }
+  }
+  const bool compact = n_kept <= kCompact;
+  __syncwarp();
+  auto weight_together = [&](int i, float* l) {
+    const bool is = i < n_kept;
+    *l = is ? logit_to_float(x.flat[together[i]]) : top;
+    const unsigned long long a = weight(*l);
+    return is ? a : 0ull;
+  };
+  float logit;
+  const int pieces = compact ? (n_kept + 31) / 32 : (x.steps + x.per_piece - 1) / x.per_piece;
+  for (int piece = 0; piece < pieces; ++piece) {
     unsigned long long mine = 0;
-    for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step) mine += kept_at_step(step);
+    if (compact)
+      mine = weight_together(piece * 32 + lane, &logit);
+    else
+      for (int step = piece * x.per_piece; step < min((piece + 1) * x.per_piece, x.steps); ++step)
+        mine += kept_at_step(step);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) s.pieces[warp * kRowPieces + step0 / x.per_piece] = mine;
+    if (lane == 0) s.pieces[warp * kRowPieces + piece] = mine;
   }
   __syncthreads();
   constexpr int kEach = kRowWarps * kRowPieces / kRowThreads;
@@ -694,27 +821,40 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   }
   __syncthreads();
   if (warp != int(s.piece) / kRowPieces) return;
-  const int step0 = int(s.piece) % kRowPieces * x.per_piece;
+  const int piece = int(s.piece) % kRowPieces;
   before = s.piece_before;
-  for (int step = step0; step < min(step0 + x.per_piece, x.steps); ++step) {
-    const unsigned long long here = kept_at_step(step);
+  auto drawn = [&](uint32_t index, float l, unsigned long long a) {
+    tokens[r] = index;
+    logprobs[r] = log_share(p, set, w, l, a, total);
+  };
+  auto lanes_before = [&](unsigned long long here, unsigned long long* all) {
     unsigned long long inc = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long other = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += other;
     }
-    unsigned long long at = before + inc - here;
+    *all = __shfl_sync(0xffffffffu, inc, 31);
+    return inc - here;
+  };
+  unsigned long long all;
+  if (compact) {
+    const unsigned long long a = weight_together(piece * 32 + lane, &logit);
+    const unsigned long long at = before + lanes_before(a, &all);
+    if (a != 0 && at <= goal && goal < at + a) drawn(together[piece * 32 + lane], logit, a);
+    return;
+  }
+  for (int step = piece * x.per_piece; step < min((piece + 1) * x.per_piece, x.steps); ++step) {
+    const unsigned long long here = kept_at_step(step);
+    unsigned long long at = before + lanes_before(here, &all);
     if (at <= goal && goal < at + here)
-      x.some_at_step(step, kept, [&](uint32_t index, float l) {
+      x.some_at_step(step, [&](float l) { return l >= cut.value; }, [&](uint32_t index, float l) {
+        if (!kept(index, l)) return;
         const unsigned long long a = weight(l);
-        if (at <= goal && goal < at + a) {
-          tokens[r] = index;
-          logprobs[r] = log_share(p, set, w, l, a, total);
-        }
+        if (at <= goal && goal < at + a) drawn(index, l, a);
         at += a;
       });
-    before += __shfl_sync(0xffffffffu, inc, 31);
+    before += all;
   }
 }
 

@@ -122,37 +122,38 @@ __device__ __forceinline__ void block_sort_descending(unsigned long long* a, int
 // w = exp((l - max) / T) as an integer: w * 2^bits rounded to the nearest. Integers add up to the same sum in any
 // order, so the sums of a row do not depend on how it is split over threads and blocks, and a token's border is where
 // 64-bit arithmetic puts it: the rounding of one weight is 2^-(bits + 1) of the largest one (bits = 44 for up to
-// 2^18 columns), that of the exponential below 2^-47. A sum of 32-bit floats would be off by 1e-7 of the total, which is
-// as wide as the share of a token in the tail of a vocabulary.
-//   exp(d / T) = 2^(n / 32) (1 + x + x^2 / 2 + ...),  n = round(32 d log2(e) / T),  |x| <= ln(2) / 64
+// 2^18 columns), the exponential is off by at most 2.3e-12 of itself. A sum of 32-bit floats would be off by 1e-7 of the
+// total, which is as wide as the share of a token in the tail of a vocabulary.
+//   exp(d / T) = 2^(n / 128) (1 + x + x^2 / 2 + x^3 / 6),  n = round(128 d log2(e) / T),  |x| <= ln(2) / 256
 struct RowWeights {
   double largest;        // the row's largest logit
-  double steps;          // 32 log2(e) / T: logit difference -> n
+  double steps;          // kSteps log2(e) / T: logit difference -> n
   double to_int;         // 2^(52 - bits): adding it leaves w * 2^bits in the low bits of the sum
-  const double* table;   // shared memory: 2^(j / 32), j = 0 .. 31
+  const double* table;   // shared memory: 2^(j / kSteps), j = 0 .. kSteps - 1
   bool only_largest;     // the largest logit is +inf: it alone has weight
 };
 constexpr int kWeightBits = 44;
-constexpr double kStepLn2 = 0.021660849392498290;  // ln(2) / 32
+constexpr int kSteps = 128;  // a power of two
+constexpr double kLn2 = 0.69314718055994531, kStepLn2 = kLn2 / kSteps;
 
 __device__ __forceinline__ double weight_steps(const RowWeights& w, float logit) {
   return (double(logit) - w.largest) * w.steps;
 }
 // Steps below which a weight rounds to nothing.
-constexpr double kNoWeight = -32.0 * (kWeightBits + 2);
+constexpr double kNoWeight = -double(kSteps) * (kWeightBits + 2);
 // The weight of `steps` in [kNoWeight, 0].
 __device__ __forceinline__ unsigned long long weight_of_steps(const RowWeights& w, double steps) {
   const double shifted = steps + 6755399441055744.0;  // 1.5 * 2^52: the integer part ends up in the low word
   const int n = __double2loint(shifted);
-  const double y = steps - (shifted - 6755399441055744.0);  // 2^(y / 32), |y| <= 1/2, by its series in y ln(2) / 32
+  const double y = steps - (shifted - 6755399441055744.0);  // |y| <= 1/2; the series is in y ln(2) / kSteps
   constexpr double c = kStepLn2;
-  double p = fma(y, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
-  p = fma(y, p, c * c * c / 6.0);
-  p = fma(y, p, c * c / 2.0);
+  double p = fma(y, c * c * c / 6.0, c * c / 2.0);
   p = fma(y, p, c);
   p = fma(y, p, 1.0);
-  p *= w.table[n & 31];
-  p = __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+  p *= w.table[n & (kSteps - 1)];
+  constexpr int kShift = 20 - 7;  // n / kSteps into the exponent
+  static_assert(kSteps == 1 << 7, "kShift goes with it");
+  p = __hiloint2double(__double2hiint(p) + ((n & ~(kSteps - 1)) << kShift), __double2loint(p));
   return (unsigned long long)(__double_as_longlong(p + w.to_int) - __double_as_longlong(w.to_int));
 }
 __device__ __forceinline__ unsigned long long row_weight(const RowWeights& w, float logit) {
