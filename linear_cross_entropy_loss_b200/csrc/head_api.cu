@@ -76,7 +76,9 @@ int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
 
 // Blocks that share a row of sample_row_kernel, and the vectors of 16 bytes that each keeps in shared memory (0: too long a
 // row, it is read again for each sweep). A block keeps up to 65 KiB, so that two are on an SM; few rows are split further, down to 8 KiB; up
-// to 192 KiB where eight blocks are not enough.
+// to 176 KiB where eight blocks are not enough.
+constexpr int64_t kRowCacheMax = 176 << 10;
+static_assert((sizeof(RowShared) + 15) / 16 * 16 + kRowCacheMax <= 232448, "dynamic shared memory limit of sm_100");
 void row_layout(int64_t rows, int64_t vocab, int es, int* parts, int* cache_vectors) {
   const int64_t bytes = vocab * es + 32;
   int n = 1;
@@ -85,7 +87,7 @@ void row_layout(int64_t rows, int64_t vocab, int es, int* parts, int* cache_vect
   const int64_t vectors = (bytes + 15) / 16;
   const int64_t each = (vectors + n - 1) / n;
   *parts = n;
-  *cache_vectors = each * 16 <= (192ll << 10) ? (int)each : 0;
+  *cache_vectors = each * 16 <= kRowCacheMax ? (int)each : 0;
 }
 
 // Dynamic shared memory above 48 KiB has to be allowed for each kernel, once per device.
@@ -129,7 +131,7 @@ int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, 
   int parts = 1, cache = 0;
   row_layout(rows, vocab, (int)sizeof(T), &parts, &cache);
   const size_t fixed = (sizeof(RowShared) + 15) / 16 * 16;
-  if ((v = allow_smem(sample_row_kernel<T>, fixed + (192u << 10))) != LCE_OK) return v;
+  if ((v = allow_smem(sample_row_kernel<T>, fixed + kRowCacheMax)) != LCE_OK) return v;
   return launch_clusters(sample_row_kernel<T>, rows * parts, kRowThreads, fixed + (size_t)cache * 16, parts, st, logits,
                          (long long)ld, (uint32_t)vocab, parts, cache, p, tokens, logprobs);
 }

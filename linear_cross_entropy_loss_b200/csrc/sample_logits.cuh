@@ -63,7 +63,7 @@ __device__ __forceinline__ RowWeights row_weights(const SampleParams& p, const R
   w.largest = largest;
   w.only_largest = largest == INFINITY;
   w.steps = fmin(1.0 / (kStepLn2 * s.temperature), 1e300);
-  w.to_int = exp2(double(52 - p.weight_bits));
+  w.to_int = __hiloint2double((1023 + 52 - p.weight_bits) << 20, 0);  // 2^(52 - bits)
   w.table = table;
   return w;
 }
@@ -197,6 +197,8 @@ constexpr int kRowBins = 2048;
 constexpr int kRowList = 2048;
 constexpr int kRowPieces = 64;  // of a warp's stretch: kept weights are added up for each
 constexpr int kRowParts = 8;
+constexpr int kRowCoarse = kRowBins / 32;
+constexpr int kRowCompact = 2 * kRowList / kRowWarps;
 
 // A stretch of the order that starts at its top: logits above `value`, and equal ones with an index below `end`.
 struct RowCut {
@@ -214,8 +216,10 @@ struct RowShared {
     struct {
       uint32_t low[kRowBins], high[kRowBins];  // a 64-bit sum in two words
     } bins;
-    unsigned long long list[kRowList];  // the elements of one bin, order_pair(key, index)
+    unsigned long long gathered[kRowList];          // all blocks' lists
+    uint32_t together[kRowWarps][kRowCompact];      // indices of what a warp keeps, ascending
   };
+  unsigned long long list[kRowList];  // this block's elements of one bin, order_pair(key, index)
   unsigned long long pieces[kRowWarps * kRowPieces];
   unsigned long long reduce[32];
   float reduce_f[32];
@@ -224,10 +228,13 @@ struct RowShared {
   float part_max[kRowParts];
   unsigned long long part_sum[kRowParts];
   uint32_t part_least[kRowParts], part_most[kRowParts], part_listed[kRowParts];
+  unsigned long long part_coarse[kRowParts][kRowCoarse];  // sums over 32 bins
   // written by one block into all
-  unsigned long long found_before;
-  uint32_t found_bin;
   RowCut found_cut;
+  // this block's own
+  unsigned long long coarse[kRowCoarse];
+  unsigned long long found_before, found_total;
+  uint32_t found_bin;
   unsigned int listed;
   uint32_t piece;
   unsigned long long piece_before;
@@ -397,63 +404,95 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
   __syncthreads();
   for (int step = 0; step < x.steps; ++step)
     x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
+      // Four elements side by side, without branches: where there is nothing to add, nothing is added to a bin of the
+      // lane's own. The answer of the first word's addition (a carry) is only looked at when all four are on their way.
 #pragma unroll
-      for (int i = 0; i < RowStretch<T>::kPer; ++i) {
-        // (a weight is taken for every place, of the largest logit where there is nothing to add: the chains of
-        // a vector's elements then run side by side)
-        const bool is = active(index + i, l[i]);
-        const float safe = is ? l[i] : c.top;
-        const unsigned long long a = amount(safe);
-        const uint32_t at = bin(safe);
-        const uint32_t low = uint32_t(a);
-        uint32_t high = uint32_t(a >> 32);
-        if (is) {
-          const uint32_t was = atomicAdd(&s.bins.low[at], low);
-          high += was + low < was ? 1u : 0u;
-          if (high != 0) atomicAdd(&s.bins.high[at], high);
+      for (int i0 = 0; i0 < RowStretch<T>::kPer; i0 += 4) {
+        uint32_t at[4], low[4], high[4], was[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool is = active(index + i0 + i, l[i0 + i]);
+          const float safe = is ? l[i0 + i] : c.top;
+          const unsigned long long a = amount(safe);
+          at[i] = is ? bin(safe) : uint32_t(threadIdx.x & 31);
+          low[i] = is ? uint32_t(a) : 0u;
+          high[i] = is ? uint32_t(a >> 32) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) was[i] = atomicAdd(&s.bins.low[at[i]], low[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          high[i] += was[i] + low[i] < was[i] ? 1u : 0u;
+          if (high[i] != 0) atomicAdd(&s.bins.high[at[i]], high[i]);
         }
       }
     });
+  __syncthreads();
+  // Sums over 32 bins go to all blocks; behind the barrier every block finds the 32 bins in question by itself, reads
+  // those of all blocks and finds the bin. (Reading and adding up all bins instead, a share per block, took two more barriers
+  // and 9,000 cycles against 3,000.)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kRowCoarse / kRowWarps; ++i) {
+    const int g = i * kRowWarps + warp, b = g * 32 + lane;
+    unsigned long long v = ((unsigned long long)s.bins.high[b] << 32) + s.bins.low[b];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane < c.parts) c.of(lane).part_coarse[c.rank][g] = v;
+  }
   c.group.sync();
-  // each block adds up its share of the bins over all blocks, consecutive ones per thread
-  const int share = kRowBins / c.parts;
-  const int each = share >= kRowThreads ? share / kRowThreads : 1;
-  const int first = c.rank * share + each * int(threadIdx.x);
-  unsigned long long sum[kRowBins / kRowThreads] = {}, mine = 0;
-  if (each * int(threadIdx.x) < share) {
+  if (threadIdx.x < kRowCoarse) {
+    unsigned long long v = 0;
+    for (int part = 0; part < c.parts; ++part) v += s.part_coarse[part][threadIdx.x];
+    s.coarse[threadIdx.x] = v;
+  }
+  __syncthreads();
+  auto prefix = [&](unsigned long long v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long other = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += other;
+    }
+    return v;
+  };
+  unsigned long long goal = 0;
+  if (warp == 0) {
+    static_assert(kRowCoarse == 64, "two per lane");
+    const unsigned long long v0 = s.coarse[2 * lane], v1 = s.coarse[2 * lane + 1];
+    const unsigned long long end = prefix(v0 + v1);
+    const unsigned long long total = __shfl_sync(0xffffffffu, end, 31);
+    goal = target(total);
+    const unsigned long long before0 = end - v1 - v0, before1 = end - v1;
+    if (before0 < goal && goal <= before1) {
+      s.found_bin = 2 * lane;
+      s.found_before = before0;
+    } else if (before1 < goal && goal <= end) {
+      s.found_bin = 2 * lane + 1;
+      s.found_before = before1;
+    }
+    if (lane == 0) s.found_total = total;
+  }
+  __syncthreads();
+  Crossing found;
+  found.total = s.found_total;
+  const uint32_t group = s.found_bin;
+  if (warp == 0) {
+    unsigned long long v = 0;
 #pragma unroll
     for (int part = 0; part < kRowParts; ++part) {
       if (part < c.parts) {
         const RowShared& other = c.of(part);
-#pragma unroll
-        for (int i = 0; i < kRowBins / kRowThreads; ++i)
-          if (i < each) sum[i] += ((unsigned long long)other.bins.high[first + i] << 32) + other.bins.low[first + i];
+        v += ((unsigned long long)other.bins.high[group * 32 + lane] << 32) + other.bins.low[group * 32 + lane];
       }
     }
-#pragma unroll
-    for (int i = 0; i < kRowBins / kRowThreads; ++i) mine += sum[i];
+    const unsigned long long end = s.found_before + prefix(v);
+    __syncwarp();
+    if (end - v < goal && goal <= end) {
+      s.found_bin = group * 32 + lane;
+      s.found_before = end - v;
+    }
   }
-  unsigned long long block_total;
-  unsigned long long before = block_prefix(mine, s.reduce, &block_total);
-  if (int(threadIdx.x) < c.parts) c.of(threadIdx.x).part_sum[c.rank] = block_total;
-  c.group.sync();
-  Crossing found;
-  found.total = 0;
-  for (int part = 0; part < c.parts; ++part) {
-    if (part < c.rank) before += s.part_sum[part];
-    found.total += s.part_sum[part];
-  }
-  const unsigned long long goal = target(found.total);
-#pragma unroll
-  for (int i = 0; i < kRowBins / kRowThreads; ++i) {
-    if (sum[i] != 0 && before < goal && goal <= before + sum[i])
-      for (int part = 0; part < c.parts; ++part) {
-        c.of(part).found_bin = uint32_t(first + i);
-        c.of(part).found_before = before;
-      }
-    before += sum[i];
-  }
-  c.group.sync();
+  __syncthreads();
   found.bin = s.found_bin;
   found.before = s.found_before;
   return found;
@@ -518,52 +557,50 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
       most = max(most, s.part_most[part]);
     }
     if (n <= unsigned(kRowList)) {
-      // few enough: the first block takes them all, in any order
-      if (c.rank == 0) {
-        const unsigned int own = s.listed;
-        for (unsigned int i = own + threadIdx.x; i < n; i += kRowThreads) {
-          unsigned int at = i - own;
-          int part = 1;
-          while (at >= s.part_listed[part]) at -= s.part_listed[part++];
-          s.list[i] = c.of(part).list[at];
+      // few enough: every block takes them all, in any order, and finds the place by itself
+      for (unsigned int i = threadIdx.x; i < n; i += kRowThreads) {
+        unsigned int at = i;
+        int part = 0;
+        while (at >= s.part_listed[part]) at -= s.part_listed[part++];
+        s.gathered[i] = c.of(part).list[at];
+      }
+      auto found = [&](unsigned long long e) {
+        s.found_cut = RowCut{key_to_float(pair_key(e)), pair_index(e) + 1};
+      };
+      constexpr int kShare = 4;  // threads per element
+      __syncthreads();
+      if (n <= kRowThreads / kShare) {
+        // every element's place is the sum of the amounts ahead of it
+        if (threadIdx.x < n) s.pieces[threadIdx.x] = amount(key_to_float(pair_key(s.gathered[threadIdx.x])));
+        __syncthreads();
+        const unsigned int i = threadIdx.x / kShare;
+        unsigned long long mine = 0, place = 0;
+        if (i < n) {
+          mine = s.gathered[i];
+          for (unsigned int j = threadIdx.x % kShare; j < n; j += kShare) place += s.gathered[j] > mine ? s.pieces[j] : 0ull;
         }
-        auto found = [&](unsigned long long e) {
-          for (int part = 0; part < c.parts; ++part)
-            c.of(part).found_cut = RowCut{key_to_float(pair_key(e)), pair_index(e) + 1};
-        };
-        if (n <= unsigned(kRowWarps * kRowPieces) / 8) {
-          // every element's place is the sum of the amounts ahead of it
-          unsigned long long mine = 0, a = 0, place = before;
-          __syncthreads();
-          if (threadIdx.x < n) {
-            mine = s.list[threadIdx.x];
-            a = amount(key_to_float(pair_key(mine)));
-            s.pieces[threadIdx.x] = a;
-          }
-          __syncthreads();
-          if (threadIdx.x < n) {
-            for (unsigned int i = 0; i < n; ++i) place += s.list[i] > mine ? s.pieces[i] : 0ull;
-            if (a != 0 && place < target && target <= place + a) found(mine);
-          }
-        } else {
-          int padded = 2;
-          while (padded < int(n)) padded <<= 1;
-          for (int i = int(n) + int(threadIdx.x); i < padded; i += kRowThreads) s.list[i] = 0;
-          block_sort_descending(s.list, padded);
-          unsigned long long seen = before;
-          for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
-            const int i = i0 + int(threadIdx.x);
-            unsigned long long a = 0;
-            if (i < int(n)) a = amount(key_to_float(pair_key(s.list[i])));
-            unsigned long long sum;
-            const unsigned long long place = seen + block_prefix(a, s.reduce, &sum);
-            if (a != 0 && place < target && target <= place + a) found(s.list[i]);
-            seen += sum;
-            if (seen >= target) break;
-          }
+#pragma unroll
+        for (int o = 1; o < kShare; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+        place += before;
+        if (i < n && threadIdx.x % kShare == 0 && place < target && target <= place + s.pieces[i]) found(mine);
+      } else {
+        int padded = 2;
+        while (padded < int(n)) padded <<= 1;
+        for (int i = int(n) + int(threadIdx.x); i < padded; i += kRowThreads) s.gathered[i] = 0;
+        block_sort_descending(s.gathered, padded);
+        unsigned long long seen = before;
+        for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
+          const int i = i0 + int(threadIdx.x);
+          unsigned long long a = 0;
+          if (i < int(n)) a = amount(key_to_float(pair_key(s.gathered[i])));
+          unsigned long long sum;
+          const unsigned long long place = seen + block_prefix(a, s.reduce, &sum);
+          if (a != 0 && place < target && target <= place + a) found(s.gathered[i]);
+          seen += sum;
+          if (seen >= target) break;
         }
       }
-      c.group.sync();
+      __syncthreads();
       return s.found_cut;
     }
     if (least == most) {
@@ -709,14 +746,10 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   }
   if (set.top_p < 1.0) {
     const RowCut outer = cut;
-    unsigned long long target = 0;
     const Crossing at = find_bin(
         c, x, weight, bin, [&](uint32_t index, float l) { return inside(outer, l, index); },
-        [&](unsigned long long total) {
-          target = mass_target(set.top_p, total);
-          return target;
-        });
-    cut = find_place(c, x, at.before, target, weight, logits_of(at.bin), outer);
+        [&](unsigned long long total) { return mass_target(set.top_p, total); });
+    cut = find_place(c, x, at.before, mass_target(set.top_p, at.total), weight, logits_of(at.bin), outer);
   }
   const bool few = cut.value > weighty || set.lowest > -INFINITY;
   if (set.lowest > -INFINITY) {
@@ -739,8 +772,8 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     });
     return sum;
   };
-  constexpr int kCompact = 2 * kRowList / kRowWarps;
-  uint32_t* const together = reinterpret_cast<uint32_t*>(s.list) + warp * kCompact;  // their indices, ascending
+  constexpr int kCompact = kRowCompact;
+  uint32_t* const together = s.together[warp];
   int n_kept = few ? 0 : kCompact + 1;
   __syncthreads();
   for (int i = threadIdx.x; i < kRowWarps * kRowPieces; i += kRowThreads) s.pieces[i] = 0;
