@@ -214,7 +214,7 @@ __device__ __forceinline__ bool inside(const RowCut& c, float l, uint32_t index)
 struct RowShared {
   union {
     struct {
-      uint32_t low[kRowBins], high[kRowBins];  // a 64-bit sum in two words
+      uint32_t low[kRowBins + 32], high[kRowBins + 32];  // a 64-bit sum in two words; 32 more for what is left out
     } bins;
     unsigned long long gathered[kRowList];          // all blocks' lists
     uint32_t together[kRowWarps][kRowCompact];      // indices of what a warp keeps, ascending
@@ -352,7 +352,6 @@ struct RowCluster {
   cooperative_groups::cluster_group group;
   int rank, parts;
   RowShared& s;
-  float top;  // the row's largest logit
   __device__ __forceinline__ RowShared& of(int part) const { return *group.map_shared_rank(&s, part); }
 };
 
@@ -404,19 +403,18 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
   __syncthreads();
   for (int step = 0; step < x.steps; ++step)
     x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
-      // Four elements side by side, without branches: where there is nothing to add, nothing is added to a bin of the
-      // lane's own. The answer of the first word's addition (a carry) is only looked at when all four are on their way.
+      // Four elements side by side, without branches: what is not active goes, whatever its amount comes out as, to a
+      // word of the lane's own. The answer of the first word's addition (a carry) is only looked at when all four are on
+      // their way.
 #pragma unroll
       for (int i0 = 0; i0 < RowStretch<T>::kPer; i0 += 4) {
         uint32_t at[4], low[4], high[4], was[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool is = active(index + i0 + i, l[i0 + i]);
-          const float safe = is ? l[i0 + i] : c.top;
-          const unsigned long long a = amount(safe);
-          at[i] = is ? bin(safe) : uint32_t(threadIdx.x & 31);
-          low[i] = is ? uint32_t(a) : 0u;
-          high[i] = is ? uint32_t(a >> 32) : 0u;
+          const unsigned long long a = amount(l[i0 + i]);
+          at[i] = active(index + i0 + i, l[i0 + i]) ? bin(l[i0 + i]) : uint32_t(kRowBins) + (threadIdx.x & 31);
+          low[i] = uint32_t(a);
+          high[i] = uint32_t(a >> 32);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) was[i] = atomicAdd(&s.bins.low[at[i]], low[i]);
@@ -675,7 +673,7 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const long long r = blockIdx.x / parts;
   const RowSettings set = row_settings(p, r);
   if (by_list(p, set)) return;  // the whole cluster
-  RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s, -INFINITY};
+  RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPer = RowStretch<T>::kPer;
 
@@ -715,7 +713,6 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   if (int(threadIdx.x) < parts) c.of(threadIdx.x).part_max[c.rank] = top;
   c.group.sync();
   for (int part = 0; part < parts; ++part) top = fmaxf(top, s.part_max[part]);
-  c.top = top;
   if (!(top > -INFINITY)) {
     if (c.rank == 0 && threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
     return;  // the whole cluster; nothing of it is read any more
@@ -727,11 +724,13 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const double inv_steps = set.temperature * kStepLn2;
   const float weighty = logit_from_steps(w, inv_steps, top, kNoWeight);
   RowCut cut{weighty, kNoEnd};
-  const float per_bin = w.only_largest ? 1.f : float(double(kRowBins) / ((kWeightBits + 2.5) * kLn2 * set.temperature));
-  auto place = [&](float l) { return l == top ? 0.f : (top - l) * per_bin; };
-  auto bin = [&](float l) { return uint32_t(min(kRowBins - 1, __float2int_rz(place(l)))); };
+  // (the last bins lie below `weighty`, so no logit with weight falls behind them)
+  const float per_bin = fminf(float(double(kRowBins) / ((kWeightBits + 2.5) * kLn2 * set.temperature)), 1e30f);
+  auto place = [&](float l) { return (top - l) * per_bin; };
+  auto bin = [&](float l) { return uint32_t(__float2int_rz(place(l))); };  // +inf next to +inf: NaN, which becomes 0
   // a bin goes from the smallest logit that lies ahead of the next bin up to, and without, its own border
   auto logits_of = [&](uint32_t b) {
+    if (w.only_largest) return RowBin{top, __uint_as_float(0x7fc00000u)};
     auto border = [&](uint32_t first) {
       return border_of(top - float(first) / per_bin, top, [&](float l) { return place(l) < float(first); });
     };
