@@ -32,6 +32,22 @@ int sm_count() {
   return n;
 }
 
+// Dynamic shared memory above 48 KiB has to be allowed for each kernel, once per device.
+template <auto kKernel>
+int allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};  // one bit per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return LCE_ERR_CUDA;
+  if (dev < 0 || dev >= 64) return LCE_ERR_UNSUPPORTED_DEVICE;
+  if ((done.load(std::memory_order_relaxed) >> dev) & 1u) return LCE_OK;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return LCE_ERR_CUDA;
+  }
+  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return LCE_OK;
+}
+
 // One launch of `blocks` blocks in clusters of `parts`.
 template <typename... Args, typename... Given>
 int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size_t smem, int parts, cudaStream_t st,
@@ -55,13 +71,13 @@ int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size
   return check_launch();
 }
 
-// Blocks that share a row: doubled while the blocks of all rows fit the GPU at once (four of kTopThreads on an SM), a part
+// Blocks that share a row: doubled while the blocks of all rows fit the GPU at once (three of kTopThreads on an SM), a part
 // keeps a whole batch, and the lists of all parts fit one.
 template <typename T>
 int top_parts(int64_t rows, int64_t vocab, int k) {
   const int64_t batch = (int64_t)kTopBatch * (32 / (int)sizeof(T));
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 4ll * sm_count() && vocab >= batch * parts && k * parts * 2 <= kTopList) parts *= 2;
+  while (parts < kTopParts && rows * parts * 2 <= 3ll * sm_count() && vocab >= batch * parts && k * parts * 2 <= kTopList) parts *= 2;
   return parts;
 }
 
@@ -69,7 +85,9 @@ template <typename T>
 int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int k, float inv_t, void* values,
                int64_t* indices, float* lse, cudaStream_t st) {
   const int parts = top_parts<T>(rows, vocab, k);
-  return launch_clusters(top_logits_kernel<T>, rows * parts, kTopThreads, 0, parts, st,
+  const int v = allow_smem<&top_logits_kernel<T>>(sizeof(TopShared));
+  if (v != LCE_OK) return v;
+  return launch_clusters(top_logits_kernel<T>, rows * parts, kTopThreads, sizeof(TopShared), parts, st,
                          reinterpret_cast<const T*>(logits), (long long)ld, (uint32_t)vocab, k, parts, inv_t,
                          reinterpret_cast<T*>(values), reinterpret_cast<long long*>(indices), lse);
 }
@@ -90,22 +108,6 @@ void row_layout(int64_t rows, int64_t vocab, int es, int* parts, int* cache_vect
   *cache_vectors = each * 16 <= kRowCacheMax ? (int)each : 0;
 }
 
-// Dynamic shared memory above 48 KiB has to be allowed for each kernel, once per device.
-template <typename K>
-int allow_smem(K kernel, size_t bytes) {
-  static std::atomic<uint64_t> done{0};  // one bit per device; one counter per kernel type
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return LCE_ERR_CUDA;
-  if (dev < 0 || dev >= 64) return LCE_ERR_UNSUPPORTED_DEVICE;
-  if ((done.load(std::memory_order_relaxed) >> dev) & 1u) return LCE_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
-    cudaGetLastError();
-    return LCE_ERR_CUDA;
-  }
-  done.fetch_or(1ull << dev, std::memory_order_relaxed);
-  return LCE_OK;
-}
-
 template <typename T>
 int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, SampleParams p, int64_t* tokens_,
                   float* logprobs, cudaStream_t st) {
@@ -124,14 +126,17 @@ int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, 
   const bool others = each || ((p.temperature != nullptr || p.temperature_all > 0.0) &&
                                !(p.top_k_all >= 1 && p.top_k_all <= p.list_limit));
   int v;
-  if (lists && (v = launch_clusters(sample_list_kernel<T>, rows * list_parts, kTopThreads, 0, list_parts, st, logits,
-                                    (long long)ld, (uint32_t)vocab, list_parts, p, tokens, logprobs)) != LCE_OK)
-    return v;
+  if (lists) {
+    if ((v = allow_smem<&sample_list_kernel<T>>(sizeof(TopShared))) != LCE_OK) return v;
+    if ((v = launch_clusters(sample_list_kernel<T>, rows * list_parts, kTopThreads, sizeof(TopShared), list_parts, st,
+                             logits, (long long)ld, (uint32_t)vocab, list_parts, p, tokens, logprobs)) != LCE_OK)
+      return v;
+  }
   if (!others) return LCE_OK;
   int parts = 1, cache = 0;
   row_layout(rows, vocab, (int)sizeof(T), &parts, &cache);
   const size_t fixed = (sizeof(RowShared) + 15) / 16 * 16;
-  if ((v = allow_smem(sample_row_kernel<T>, fixed + kRowCacheMax)) != LCE_OK) return v;
+  if ((v = allow_smem<&sample_row_kernel<T>>(fixed + kRowCacheMax)) != LCE_OK) return v;
   return launch_clusters(sample_row_kernel<T>, rows * parts, kRowThreads, fixed + (size_t)cache * 16, parts, st, logits,
                          (long long)ld, (uint32_t)vocab, parts, cache, p, tokens, logprobs);
 }

@@ -14,7 +14,7 @@
 // 4. Rank: the logits of the listed groups are read again and those that reach the bound sorted.
 //
 // A row with more groups than the shared array takes goes through 1 to 3 in segments. A row may also be split over
-// the blocks of a cluster; the first block then takes the others' lists.
+// the blocks of a cluster, which share their first bounds and hand their lists to the first block.
 #pragma once
 
 #include "ptx.cuh"
@@ -33,23 +33,26 @@ constexpr int kTopChunk = 4 * kTopThreads;                 // groups looked at b
 constexpr int kTopSegmentBytes = 16384;                    // shared array of the maxima
 constexpr int kTopList = 2048;                             // groups in the list
 constexpr int kTopFull = kTopList - kTopChunk;             // most of them before a chunk: the chunk fits
-constexpr int kTopElements = 2 * kTopMax;                  // logits of the last step: what is kept, and as many more
-constexpr int kSearchSteps = 33;  // of bound_for: a step leaves a fifth of the range, or one key less
+constexpr int kTopParts = 8;
+constexpr int kSearchBins = kTopThreads;
+static_assert(kTopSegmentBytes >= kTopList * 8, "rank_list borrows the array of the maxima");
 static_assert(kTopFull >= kTopMax, "the list keeps k groups and takes a chunk");
 
 struct TopShared {
-  unsigned long long list[kTopList];         // order_pair(largest logit, group)
-  union {
-    unsigned long long elements[kTopElements]; // order_pair(logit, index); after the last segment
-    uint4 maxima[kTopSegmentBytes / 16];       // the segment's groups: their maxima in the type of the logits
-  };
-  unsigned int counters[2 * kSearchSteps + 1];
+  unsigned long long list[kTopList];    // order_pair(largest logit, group); later, of a row in parts, the elements
+  unsigned long long other[kTopList];   // the elements, order_pair(logit, index); of a row in parts first all parts' lists
+  uint4 maxima[kTopSegmentBytes / 16];  // the segment's groups: their maxima in the type of the logits
+  unsigned int bins[kSearchBins];
   unsigned int range[2];
+  unsigned int found[3];     // bin, keys above it, keys in it
   unsigned int count;        // entries of `list`
-  unsigned int n_elements;   // entries of `elements`
+  unsigned int n_other;      // entries of `other`
+  unsigned int place;
   unsigned long long bound;  // keys from here on enter (2^32: none)
   float scratch[32];
-  float part_ref, part_sum;  // log-sum-exp of this block's part
+  // written by all blocks of the cluster, each into its own place
+  uint32_t part_bound[kTopParts];
+  float part_ref[kTopParts], part_sum[kTopParts];  // log-sum-exp of a part
 };
 
 struct Group {
@@ -110,7 +113,9 @@ struct RowGroups {
   __device__ __forceinline__ bool exists(int e) const { return e >= 0 && uint32_t(e) < vocab; }
   __device__ __forceinline__ Group load(int v) const {
     const int e = first_of(v);
-    if (e >= 0 && uint32_t(e + kPer) <= vocab) return load_stream(row + e);
+    return e >= 0 && uint32_t(e + kPer) <= vocab ? load_stream(row + e) : load_edge(e);
+  }
+  __device__ __noinline__ Group load_edge(int e) const {
     Group g = {};
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -200,62 +205,72 @@ __device__ __forceinline__ unsigned long long add_exponentials(unsigned long lon
   return sum2;
 }
 
-// A key that at least k of the block's entries reach, and (unless many are equal) at most k + slack. The range of the keys
-// is cut into five parts at a time (a step costs a barrier and a trip through shared memory, whatever it counts).
-// least / most: over this thread's entries; count_from(key): how many of this thread's entries are >= key. With
-// fewer than k entries: 0.
-template <typename CountFrom>
-__device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, uint32_t least, uint32_t most,
-                                              CountFrom count_from) {
-  if (threadIdx.x < 2 * kSearchSteps + 1) s.counters[threadIdx.x] = 0;
+// A key that at least k of the block's keys reach, and (unless many are equal) at most k + slack. least / most: over this
+// thread's keys; each(f): f(key) for this thread's keys, 0 for one that does not exist. 0 when there are fewer than k.
+// A histogram of 256 bins over the range of the keys; where the bin in question holds too many, one over that bin.
+template <typename Each>
+__device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, uint32_t least, uint32_t most, Each each) {
+  const int lane = int(threadIdx.x & 31);
+  __syncthreads();
   if (threadIdx.x == 0) {
     s.range[0] = 0xffffffffu;
     s.range[1] = 0;
   }
+  s.bins[threadIdx.x] = 0;
   __syncthreads();
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
-  const unsigned int all = __reduce_add_sync(0xffffffffu, (unsigned int)count_from(0u));
-  if ((threadIdx.x & 31) == 0) {
+  if (lane == 0) {
     atomicMin(&s.range[0], least);
     atomicMax(&s.range[1], most);
-    atomicAdd(&s.counters[2 * kSearchSteps], all);
   }
   __syncthreads();
-  if (int(s.counters[2 * kSearchSteps]) < k) return 0u;
-  uint32_t lo = s.range[0];                                      // k or more from here on
-  unsigned long long above = (unsigned long long)s.range[1] + 1;  // fewer than k from here on
-  for (int step = 0; above - lo > 1; ++step) {
-    const unsigned long long width = above - lo;
-    uint32_t at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) at[i] = uint32_t(lo + width * (i + 1) / 5);
-    // two counts in a word: none is above 2^16
-    unsigned int low = (unsigned int)count_from(at[0]) | (unsigned int)count_from(at[1]) << 16;
-    unsigned int high = (unsigned int)count_from(at[2]) | (unsigned int)count_from(at[3]) << 16;
-    low = __reduce_add_sync(0xffffffffu, low);
-    high = __reduce_add_sync(0xffffffffu, high);
-    if ((threadIdx.x & 31) == 0) {
-      atomicAdd(&s.counters[2 * step], low);
-      if (high != 0) atomicAdd(&s.counters[2 * step + 1], high);
-    }
+  uint32_t lo = max(s.range[0], 1u), hi = s.range[1];
+  unsigned int above = 0;  // keys above hi
+  for (;;) {
+    if (hi < lo) return 0u;  // no key at all
+    const int shift = max(0, 24 - __clz(hi - lo));  // (hi - lo) >> shift < 256
+    each([&](uint32_t key) {
+      if (key >= lo && key <= hi) atomicAdd(&s.bins[(key - lo) >> shift], 1u);
+    });
     __syncthreads();
-    low = s.counters[2 * step];
-    high = s.counters[2 * step + 1];
-    const int total[4] = {int(low & 0xffffu), int(low >> 16), int(high & 0xffffu), int(high >> 16)};
-    bool near = false;
+    if (threadIdx.x < 32) {
+      // lane l has the bins from 255 - 8 l downwards
+      unsigned int c[8], mine = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (total[i] >= k) {
-        if (at[i] > lo) lo = at[i];
-        near = total[i] <= k + slack;
-      } else if (at[i] < above) {
-        above = at[i];
+      for (int i = 0; i < 8; ++i) {
+        c[i] = s.bins[kSearchBins - 1 - 8 * lane - i];
+        mine += c[i];
+      }
+      unsigned int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned int before = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += before;
+      }
+      unsigned int seen = above + inc - mine;
+      if (lane == 31 && above + inc < unsigned(k)) s.found[2] = 0xffffffffu;  // fewer than k
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (seen < unsigned(k) && seen + c[i] >= unsigned(k)) {
+          s.found[0] = kSearchBins - 1 - 8 * lane - i;
+          s.found[1] = seen;
+          s.found[2] = c[i];
+        }
+        seen += c[i];
       }
     }
-    if (near) break;
+    __syncthreads();
+    const unsigned int in_bin = s.found[2];
+    if (in_bin == 0xffffffffu) return 0u;
+    above = s.found[1];
+    lo += s.found[0] << shift;
+    if (above + in_bin <= unsigned(k + slack) || shift == 0) return lo;
+    const uint32_t width = (1u << shift) - 1u;
+    hi = hi - lo > width ? lo + width : hi;
+    s.bins[threadIdx.x] = 0;
+    __syncthreads();
   }
-  return lo;
 }
 
 // Keeps the entries of a list for which stay(entry) holds, in place: chunk by chunk, each read before any place up to
@@ -273,17 +288,6 @@ __device__ __forceinline__ void filter_list(unsigned long long* list, unsigned i
   __syncthreads();
 }
 
-// Sorts a list of n entries (room for the next power of two of them) and keeps the first k.
-__device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int& count, int n, int k) {
-  __syncthreads();
-  int padded = 2;
-  while (padded < n) padded <<= 1;
-  for (int i = n + threadIdx.x; i < padded; i += kTopThreads) list[i] = 0;
-  block_sort_descending(list, padded);
-  if (threadIdx.x == 0) count = min(n, k);
-  __syncthreads();
-}
-
 // Leaves at least the k first entries of a list, and at most `most_left` (k <= most_left) of them. Returns a key that
 // all of them reach; what comes behind them in the order has a smaller one, or the same.
 __device__ __noinline__ uint32_t cut_list(TopShared& s, unsigned long long* list, unsigned int& count, int k, int most_left) {
@@ -295,14 +299,15 @@ __device__ __noinline__ uint32_t cut_list(TopShared& s, unsigned long long* list
     least = min(least, key);
     most = max(most, key);
   }
-  const uint32_t from = bound_for(s, k, min(k / 4 + 16, most_left - k), least, most, [&](uint32_t key) {
-    int c = 0;
-    for (int i = threadIdx.x; i < n; i += kTopThreads) c += pair_key(list[i]) >= key;
-    return c;
+  const uint32_t from = bound_for(s, k, min(k / 4 + 16, most_left - k), least, most, [&](auto f) {
+    for (int i = threadIdx.x; i < n; i += kTopThreads) f(pair_key(list[i]));
   });
   filter_list(list, count, n, [&](unsigned long long e) { return pair_key(e) >= from; });
   if (int(count) <= most_left) return from;
-  sort_list(list, count, int(count), k);  // too many equal ones to tell apart by their keys
+  // too many equal ones to tell apart by their keys
+  block_sort_descending<kTopThreads>(list, int(count));
+  if (threadIdx.x == 0) count = k;
+  __syncthreads();
   return pair_key(list[k - 1]);
 }
 
@@ -312,11 +317,100 @@ __device__ __forceinline__ float bound_value(unsigned long long bound) {
   return bound <= 0xffffffffull ? key_to_float(uint32_t(bound)) : __uint_as_float(0x7fc00000u);
 }
 
+// bound_for four keys of each thread (0: no key), and for the maxima of a segment.
+__device__ __noinline__ uint32_t bound_of_four(TopShared& s, int k, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  static_assert(2 * kTopUnroll == 4, "four running maxima");
+  auto or_none = [](uint32_t key) { return key != 0 ? key : 0xffffffffu; };
+  return bound_for(s, k, k / 4 + 4, min(min(or_none(a), or_none(b)), min(or_none(c), or_none(d))),
+                   max(max(a, b), max(c, d)), [&](auto f) {
+                     f(a);
+                     f(b);
+                     f(c);
+                     f(d);
+                   });
+}
+template <typename T, Nan kNan>
+__device__ __noinline__ uint32_t bound_of_segment(TopShared& s, int k, int groups) {
+  const T* const maxima = reinterpret_cast<const T*>(s.maxima);
+  uint32_t least = 0xffffffffu, most = 0;
+  for (int i = threadIdx.x; i < groups; i += kTopThreads) {
+    const uint32_t key = search_key<kNan>(logit_to_float(maxima[i]));
+    least = min(least, key);
+    most = max(most, key);
+  }
+  return bound_for(s, k, 64, least, most, [&](auto f) {
+    for (int i = threadIdx.x; i < groups; i += kTopThreads) f(search_key<kNan>(logit_to_float(maxima[i])));
+  });
+}
+
+// The groups [seg, end) of the segment whose maxima lie in shared memory: those that reach the bound go to the list.
+// (A function of its own, like the search: the registers of the stream are free here.)
+template <typename T, Nan kNan>
+__device__ __noinline__ void collect_segment(TopShared& s, int seg, int end, bool first_segment, int k, int limit) {
+  const T* const maxima = reinterpret_cast<const T*>(s.maxima);
+  // 16 bytes of maxima at a time: one comparison of their largest with the bound decides for all
+  constexpr int kAtOnce = 16 / int(sizeof(T));
+  auto collect = [&](int at, int stop) {  // this thread's places `at`, at + kTopThreads * kAtOnce, .. below `stop`
+    const unsigned long long bound_key = s.bound;
+    const float bound = bound_value(bound_key);
+    bool full = false;
+    for (; at < stop; at += kTopThreads * kAtOnce) {
+      const uint4 raw = s.maxima[at / kAtOnce];
+      Group one = RowGroups<T>::nothing();
+      one.w[0] = raw.x; one.w[1] = raw.y; one.w[2] = raw.z; one.w[3] = raw.w;
+      if (largest<kNan>(one, static_cast<const T*>(nullptr)) < bound) continue;
+      float top[kAtOnce];
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(one.w[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) halves(one.w[i], top[2 * i], top[2 * i + 1], static_cast<const T*>(nullptr));
+      }
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)
+        hits |= !(top[i] < bound) && search_key<kNan>(top[i]) >= bound_key && seg + at + i < end ? 1u << i : 0u;
+      if (hits == 0) continue;
+      unsigned int place = atomicAdd(&s.count, (unsigned int)__popc(hits));
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (!(hits & (1u << i))) continue;
+        if (place < unsigned(kTopList)) s.list[place] = order_pair(search_key<kNan>(top[i]), uint32_t(seg + at + i));
+        full |= place >= unsigned(limit);
+        ++place;
+      }
+    }
+    return full;
+  };
+  auto cut = [&]() {
+    const uint32_t least_left = cut_list(s, s.list, s.count, k, limit);
+    if (threadIdx.x == 0) s.bound = (unsigned long long)least_left + 1;
+    __syncthreads();
+  };
+  // all at once: with a good bound few groups enter
+  const int mine = kAtOnce * int(threadIdx.x);
+  if (!__syncthreads_or(collect(mine, end - seg))) return;
+  const bool lost = s.count > unsigned(kTopList);
+  __syncthreads();
+  if (!lost) {
+    cut();
+    return;
+  }
+  // again, a chunk at a time, cutting the list whenever it is full
+  filter_list(s.list, s.count, kTopList,
+              [&](unsigned long long e) { return !first_segment && pair_index(e) < uint32_t(seg); });
+  for (int c = 0; c < end - seg; c += kTopChunk) {
+    const int from = c + mine, stop = min(c + kTopChunk, end - seg);
+    if (__syncthreads_or(collect(from, stop))) cut();
+  }
+}
+
 // Groups [v0, v1) of the row into the list, which then has the k first of them among its entries (all of them if there
 // are fewer than k). kSum: the thread's share of sum_j 2^(l_j * log2_scale - ref) goes to (ref, sum).
 template <typename T, bool kSum, Nan kNan>
-__device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row, int v0, int v1, int k, float log2_scale,
-                                           float& ref, float& sum) {
+__device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row, int v0, int v1, int parts, int k,
+                                           float log2_scale, float& ref, float& sum) {
   constexpr int kSegment = kTopSegmentBytes / int(sizeof(T));  // groups
   static_assert(kSegment % kTopChunk == 0 && kSegment % (2 * kTopBatch) == 0, "segments are whole chunks");
   const T* tag = nullptr;
@@ -325,6 +419,7 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
   __syncthreads();
   if (threadIdx.x == 0) {
     s.count = 0;
+    s.n_other = 0;
     s.bound = 0;
   }
   auto fetch = [&](int vb, Group(&to)[kTopUnroll]) {
@@ -342,10 +437,10 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
   };
   ref = -INFINITY;
   sum = 0.f;
-  Group cur[kTopUnroll], nxt[kTopUnroll];
-  fetch(v0, cur);
   for (int seg = v0; seg < v1; seg += kSegment) {
     const int end = min(seg + kSegment, v1);
+    Group cur[kTopUnroll], nxt[kTopUnroll];
+    fetch(seg, cur);
     float run[2 * kTopUnroll];
 #pragma unroll
     for (int i = 0; i < 2 * kTopUnroll; ++i) run[i] = -INFINITY;
@@ -376,157 +471,193 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
       }
     };
     for (int vb = seg; vb < end; vb += 2 * kTopBatch) {
-      if (vb + kTopBatch < v1) fetch(vb + kTopBatch, nxt);
+      if (vb + kTopBatch < end) fetch(vb + kTopBatch, nxt);
       take(vb, cur, run);
-      if (vb + 2 * kTopBatch < v1) fetch(vb + 2 * kTopBatch, cur);
+      if (vb + 2 * kTopBatch < end) fetch(vb + 2 * kTopBatch, cur);
       if (vb + kTopBatch < end) take(vb + kTopBatch, nxt, run + kTopUnroll);
     }
     __syncthreads();
-    // the first bound; with more wanted than half the running maxima they say too little, and the groups' own are searched
-    uint32_t from;
-    if (k <= kTopThreads * kTopUnroll) {
-      uint32_t key[2 * kTopUnroll], least = 0xffffffffu, most = 0;
+    // The first bound. A row in parts needs k groups from all of them: each part finds a share of k among its first
+    // segment, and the lowest of the parts' bounds is one that k groups reach. Where one part lies far above the others its
+    // list runs full and is cut.
+    if (parts == 1 || seg == v0) {
+      const int want = (k + parts - 1) / parts;
+      uint32_t from;
+      if (want <= kTopThreads * kTopUnroll) {
+        uint32_t key[2 * kTopUnroll];
 #pragma unroll
-      for (int i = 0; i < 2 * kTopUnroll; ++i) {
-        key[i] = seg + i * kTopThreads + int(threadIdx.x) < end ? search_key<kNan>(run[i]) : 0u;  // 0: no group
-        least = min(least, key[i]);
-        most = max(most, key[i]);
+        for (int i = 0; i < 2 * kTopUnroll; ++i)
+          key[i] = seg + i * kTopThreads + int(threadIdx.x) < end ? search_key<kNan>(run[i]) : 0u;  // 0: no group
+        from = bound_of_four(s, want, key[0], key[1], key[2], key[3]);
+      } else {
+        // more than half of the running maxima are wanted: they say too little, and the groups' own are searched
+        from = bound_of_segment<T, kNan>(s, want, end - seg);
       }
-      from = bound_for(s, k, k / 4 + 4, least, most, [&](uint32_t b) {
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < 2 * kTopUnroll; ++i) c += key[i] >= b;
-        return c;
-      });
-    } else {
-      uint32_t least = 0xffffffffu, most = 0;
-      for (int i = threadIdx.x; i < end - seg; i += kTopThreads) {
-        const uint32_t key = search_key<kNan>(logit_to_float(maxima[i]));
-        least = min(least, key);
-        most = max(most, key);
+      if (parts > 1) {  // every part comes here once: it has groups
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        if (int(threadIdx.x) < parts) cluster.map_shared_rank(&s, threadIdx.x)->part_bound[cluster.block_rank()] = from;
+        cluster.sync();
+        for (int part = 0; part < parts; ++part) from = min(from, s.part_bound[part]);
       }
-      from = bound_for(s, k, 64, least, most, [&](uint32_t b) {
-        int c = 0;
-        for (int i = threadIdx.x; i < end - seg; i += kTopThreads) c += search_key<kNan>(logit_to_float(maxima[i])) >= b;
-        return c;
-      });
-    }
-    if (threadIdx.x == 0) s.bound = max(s.bound, (unsigned long long)from);
-    __syncthreads();
-    float bound = bound_value(s.bound);
-    for (int c = seg; c < end; c += kTopChunk) {
-      bool full = false;
-      T four[4];
-      const int at = c - seg + 4 * int(threadIdx.x);
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(four) = reinterpret_cast<const uint4*>(maxima)[at / 4];
-      else *reinterpret_cast<uint2*>(four) = reinterpret_cast<const uint2*>(maxima)[at / 4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float top = logit_to_float(four[i]);
-        if (!(top < bound) && seg + at + i < end) {
-          const uint32_t key = search_key<kNan>(top);
-          if (key >= s.bound) {
-            const unsigned int place = atomicAdd(&s.count, 1u);
-            s.list[place] = order_pair(key, uint32_t(seg + at + i));
-            full |= place >= unsigned(limit);
-          }
-        }
-      }
-      if (__syncthreads_or(full)) {
-        const uint32_t least = cut_list(s, s.list, s.count, k, limit);
-        if (threadIdx.x == 0) s.bound = (unsigned long long)least + 1;
-        __syncthreads();
-        bound = bound_value(s.bound);
-      }
-    }
-  }
-  __syncthreads();
-}
-
-// Takes the other blocks' lists (and shares of the sum) into the first block, whose list then has the row's k first groups
-// among its entries. k * parts <= kTopList. The other blocks return with their part done.
-__device__ __forceinline__ void merge_lists(TopShared& s, int k, int parts) {
-  if (parts > 1) {
-    if (s.count > unsigned(kTopList / parts)) cut_list(s, s.list, s.count, k, kTopList / parts);
-    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-    cluster.sync();
-    if (cluster.block_rank() == 0) {
-      unsigned int at = s.count;
-      for (int part = 1; part < parts; ++part) {
-        const TopShared* other = cluster.map_shared_rank(&s, part);
-        const unsigned int n = other->count;
-        for (unsigned int i = threadIdx.x; i < n; i += kTopThreads) s.list[at + i] = other->list[i];
-        at += n;
-      }
+      if (threadIdx.x == 0) s.bound = max(s.bound, (unsigned long long)from);
       __syncthreads();
-      if (threadIdx.x == 0) {
-        s.count = at;
-        float m = s.part_ref;
-        for (int part = 1; part < parts; ++part) m = fmaxf(m, cluster.map_shared_rank(&s, part)->part_ref);
-        float sum = 0.f;
-        for (int part = 0; part < parts; ++part) {
-          const TopShared* other = cluster.map_shared_rank(&s, part);
-          if (other->part_ref > -INFINITY) sum += other->part_sum * fast_exp2(other->part_ref - m);
-        }
-        s.part_ref = m;
-        s.part_sum = sum;
-      }
     }
-    cluster.sync();
-    if (cluster.block_rank() != 0) return;
+    collect_segment<T, kNan>(s, seg, end, seg == v0, k, limit);
   }
   __syncthreads();
-  if (s.count > unsigned(k + k / 4 + 32)) cut_list(s, s.list, s.count, k, min(2 * k + 64, kTopFull));
 }
 
-// The listed groups' logits again: s.elements then holds the k first logits of the row (all of them if there are fewer),
-// sorted, s.n_elements of them.
-template <Nan kNan, typename T>
-__device__ __forceinline__ void rank_elements(TopShared& s, const RowGroups<T>& row, int k) {
-  constexpr int kPer = RowGroups<T>::kPer;
+// The list that has the row's k first groups among its entries, and their number; of a row in parts in the first block, the others
+// return with 0. `free_list`: room for the elements.
+struct TopGroups {
+  unsigned long long* list;
+  unsigned long long* free_list;
+  int n;
+};
+__device__ __forceinline__ TopGroups merge_lists(TopShared& s, int k, int parts) {
   __syncthreads();
-  const int n = int(s.count);
+  if (parts == 1) {
+    if (s.count > unsigned(2 * k + 64)) cut_list(s, s.list, s.count, k, 2 * k + 64);
+    return TopGroups{s.list, s.other, int(s.count)};
+  }
+  // every part hands over what it has, up to its share of the room; behind the barrier nobody looks at the others again
+  if (s.count > unsigned(kTopList / parts)) cut_list(s, s.list, s.count, k, kTopList / parts);
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  TopShared* first = cluster.map_shared_rank(&s, 0);
+  if (threadIdx.x == 0) s.place = atomicAdd(&first->n_other, s.count);
+  __syncthreads();
+  for (unsigned int i = threadIdx.x; i < s.count; i += kTopThreads) first->other[s.place + i] = s.list[i];
+  cluster.sync();
+  if (cluster.block_rank() != 0) return TopGroups{nullptr, nullptr, 0};
+  if (s.n_other > unsigned(2 * k + 64)) cut_list(s, s.other, s.n_other, k, 2 * k + 64);
+  return TopGroups{s.other, s.list, int(s.n_other)};
+}
+
+// Sorts a list of m <= kTopList entries, largest first, into its own place. `spare`: room for as many.
+__device__ __noinline__ void rank_list(TopShared& s, unsigned long long* list, unsigned long long* spare, int m) {
+  constexpr int kEach = kTopList / kTopThreads;
+  __syncthreads();
+  if (m <= kTopThreads / 2) {
+    // few: every entry's place is the number of entries ahead of it
+    const unsigned long long mine = int(threadIdx.x) < m ? list[threadIdx.x] : 0;
+    int place = 0;
+    for (int i = 0; i < m; ++i) place += list[i] > mine;
+    __syncthreads();
+    if (int(threadIdx.x) < m) list[place] = mine;
+    __syncthreads();
+    return;
+  }
+  // Entries go to 256 bins over the range of the keys; an entry's place is the number of those in bins ahead and of those of its own bin
+  // ahead of it, of which there are few.
   if (threadIdx.x == 0) {
-    s.n_elements = 0;
+    s.range[0] = 0xffffffffu;
+    s.range[1] = 0;
+  }
+  s.bins[threadIdx.x] = 0;
+  __syncthreads();
+  uint32_t least = 0xffffffffu, most = 0;
+  for (int i = threadIdx.x; i < m; i += kTopThreads) {
+    least = min(least, pair_key(list[i]));
+    most = max(most, pair_key(list[i]));
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMin(&s.range[0], least);
+    atomicMax(&s.range[1], most);
+  }
+  __syncthreads();
+  const uint32_t hi = s.range[1];
+  const int shift = max(0, 24 - __clz(hi - s.range[0]));
+  unsigned int at[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = i * kTopThreads + int(threadIdx.x);
+    at[i] = j < m ? atomicAdd(&s.bins[(hi - pair_key(list[j])) >> shift], 1u) : 0u;
+  }
+  __syncthreads();
+  const unsigned int mine = s.bins[threadIdx.x];
+  if (__syncthreads_or(mine > 64u)) {  // many equal ones
+    block_sort_descending<kTopThreads>(list, m);
+    return;
+  }
+  unsigned int total;
+  const unsigned int begin = block_prefix(mine, reinterpret_cast<unsigned int*>(s.scratch), &total);
+  s.bins[threadIdx.x] = begin;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = i * kTopThreads + int(threadIdx.x);
+    if (j < m) spare[s.bins[(hi - pair_key(list[j])) >> shift] + at[i]] = list[j];
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < m; j += kTopThreads) {
+    const unsigned long long e = spare[j];
+    const uint32_t b = (hi - pair_key(e)) >> shift;
+    const int first = int(s.bins[b]), end = b + 1 < uint32_t(kSearchBins) ? int(s.bins[b + 1]) : m;
+    int place = first;
+    for (int i = first; i < end; ++i) place += spare[i] > e;
+    list[place] = e;
+  }
+  __syncthreads();
+}
+
+// The listed groups' logits again: the k first logits of the row (all of them if there are fewer), sorted, in g.free_list;
+// returns how many.
+template <Nan kNan, typename T>
+__device__ __forceinline__ int rank_elements(TopShared& s, const RowGroups<T>& row, const TopGroups& g, int k) {
+  constexpr int kPer = RowGroups<T>::kPer, kPart = kPer / 4;  // logits of a thread: a quarter of a group
+  unsigned long long* const elements = g.free_list;
+  unsigned int& count = s.place;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    count = 0;
     s.range[0] = 0xffffffffu;
   }
   __syncthreads();
   uint32_t least = 0xffffffffu;
-  for (int i = threadIdx.x; i < n; i += kTopThreads) least = min(least, pair_key(s.list[i]));
+  for (int i = threadIdx.x; i < g.n; i += kTopThreads) least = min(least, pair_key(g.list[i]));
   least = __reduce_min_sync(0xffffffffu, least);
   if ((threadIdx.x & 31) == 0) atomicMin(&s.range[0], least);
   __syncthreads();
-  uint32_t from = n >= k ? s.range[0] : 0u;  // n logits reach it
-  int m = 0;
-  for (int i0 = 0; i0 < n * kPer; i0 += kTopMax) {
+  uint32_t from = g.n >= k ? s.range[0] : 0u;  // g.n logits reach it
+  auto expand = [&](int i0, int i1) {  // groups
+    for (int i = 4 * i0 + int(threadIdx.x); i < 4 * i1; i += kTopThreads) {
+      const int e = row.first_of(int(pair_index(g.list[i / 4]))) + i % 4 * kPart;
+      T l[kPart];
+      if (e >= 0 && uint32_t(e + kPart) <= row.vocab) {
+        *reinterpret_cast<uint2*>(l) = __ldg(reinterpret_cast<const uint2*>(row.row + e));
+      } else {
 #pragma unroll
-    for (int j = 0; j < kTopMax / kTopThreads; ++j) {
-      const int i = i0 + j * kTopThreads + int(threadIdx.x);
-      if (i < n * kPer) {
-        const int e = row.first_of(int(pair_index(s.list[i / kPer]))) + i % kPer;
-        if (row.exists(e)) {
-          const uint32_t key = search_key<kNan>(logit_to_float(row.row[e]));
-          if (key >= from) s.elements[atomicAdd(&s.n_elements, 1u)] = order_pair(key, uint32_t(e));
+        for (int j = 0; j < kPart; ++j) l[j] = row.exists(e + j) ? row.row[e + j] : T(-INFINITY);
+      }
+#pragma unroll
+      for (int j = 0; j < kPart; ++j) {
+        const uint32_t key = search_key<kNan>(logit_to_float(l[j]));
+        if (key >= from && row.exists(e + j)) {
+          const unsigned int place = atomicAdd(&count, 1u);
+          if (place < unsigned(kTopList)) elements[place] = order_pair(key, uint32_t(e + j));
         }
       }
     }
     __syncthreads();
-    m = int(s.n_elements);
+    const int m = int(count);
     __syncthreads();
-    if (m > kTopMax && i0 + kTopMax < n * kPer) from = cut_list(s, s.elements, s.n_elements, k, kTopMax);
+    return m;
+  };
+  int m = expand(0, g.n);
+  if (m > kTopList) {
+    // too many equal ones: again, few groups at a time, keeping the first k
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    m = 0;
+    for (int i = 0; i < g.n; i += kTopMax / kPer) {
+      if (m > kTopMax) from = cut_list(s, elements, count, k, kTopMax);
+      m = expand(i, min(i + kTopMax / kPer, g.n));
+    }
   }
-  if (m <= kTopThreads) {
-    // few: every entry's place is the number of entries ahead of it
-    const unsigned long long mine = int(threadIdx.x) < m ? s.elements[threadIdx.x] : 0;
-    int place = 0;
-    for (int i = 0; i < m; ++i) place += s.elements[i] > mine;
-    __syncthreads();
-    if (int(threadIdx.x) < m) s.elements[place] = mine;
-    if (threadIdx.x == 0) s.n_elements = min(m, k);
-    __syncthreads();
-  } else {
-    sort_list(s.elements, s.n_elements, m, k);
-  }
+  rank_list(s, elements, reinterpret_cast<unsigned long long*>(s.maxima), m);
+  return min(m, k);
 }
 
 }  // namespace lce

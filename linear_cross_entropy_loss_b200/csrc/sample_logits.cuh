@@ -92,10 +92,11 @@ __device__ __forceinline__ void draw_nothing(long long r, long long* tokens, flo
 // rows with a short list
 // ---------------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(kTopThreads, 4)
+__global__ void __launch_bounds__(kTopThreads, 3)
 sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int parts, const SampleParams p,
                    long long* __restrict__ tokens, float* __restrict__ logprobs) {
-  __shared__ TopShared s;
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  TopShared& s = *reinterpret_cast<TopShared*>(dynamic);
   __shared__ double table[kSteps];
   __shared__ unsigned long long reduce[32];
   const long long r = blockIdx.x / parts;
@@ -104,17 +105,15 @@ sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, i
   if (!by_list(p, set)) return;  // the whole cluster
   const int k = int(min((long long)vocab, set.top_k));
   const RowGroups<T> row(logits + r * ld, vocab);
-  const int share = (row.groups + parts - 1) / parts;
-  const int v0 = min(part * share, row.groups), v1 = min(v0 + share, row.groups);
+  const int v0 = int((long long)row.groups * part / parts), v1 = int((long long)row.groups * (part + 1) / parts);
   float ref, sum;
   if (threadIdx.x < kSteps) table[threadIdx.x] = exp2(double(threadIdx.x) / kSteps);
-  stream_top<T, false, Nan::kNever>(s, row, v0, v1, k, 1.f, ref, sum);
-  merge_lists(s, k, parts);
+  stream_top<T, false, Nan::kNever>(s, row, v0, v1, parts, k, 1.f, ref, sum);
+  const TopGroups g = merge_lists(s, k, parts);
   if (part != 0) return;
-  rank_elements<Nan::kNever>(s, row, k);
-
-  const int n = int(s.n_elements);
-  const uint32_t first = pair_key(s.elements[0]);
+  const int n = rank_elements<Nan::kNever>(s, row, g, k);
+  const unsigned long long* const elements = g.free_list;
+  const uint32_t first = pair_key(elements[0]);
   if (first == kKeyNegInf) {
     if (threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
     return;
@@ -126,21 +125,21 @@ sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, i
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int rank = kEach * int(threadIdx.x) + i;
-    mine[i] = rank < n ? row_weight(w, key_to_float(pair_key(s.elements[rank]))) : 0ull;
+    mine[i] = rank < n ? row_weight(w, key_to_float(pair_key(elements[rank]))) : 0ull;
     sum4 += mine[i];
   }
   unsigned long long mass;
   unsigned long long before = block_prefix(sum4, reduce, &mass);
   const unsigned long long target = set.top_p < 1.0 ? mass_target(set.top_p, mass) : mass;
-  unsigned long long* weights = s.list;            // by rank; 0 where a token is not kept
-  unsigned long long* by_index = s.list + kTopMax;
+  unsigned long long* weights = g.list;            // by rank; 0 where a token is not kept
+  unsigned long long* by_index = g.list + kTopMax;
   sum4 = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int rank = kEach * int(threadIdx.x) + i;
     bool keep = before < target;
     if (rank < n && !w.only_largest)
-      keep = keep && weight_steps(w, key_to_float(pair_key(s.elements[rank]))) >= set.lowest;
+      keep = keep && weight_steps(w, key_to_float(pair_key(elements[rank]))) >= set.lowest;
     before += mine[i];
     if (!keep) mine[i] = 0;
     weights[rank] = mine[i];
@@ -156,18 +155,18 @@ sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, i
   if (kept <= kTopThreads) {
     const int i = int(threadIdx.x);
     if (i < kept) {
-      const uint32_t index = pair_index(s.elements[i]);
+      const uint32_t index = pair_index(elements[i]);
       unsigned long long at = 0;
-      for (int j = 0; j < kept; ++j) at += pair_index(s.elements[j]) < index ? weights[j] : 0ull;
+      for (int j = 0; j < kept; ++j) at += pair_index(elements[j]) < index ? weights[j] : 0ull;
       if (at <= goal && goal < at + weights[i]) {
         tokens[r] = index;
-        logprobs[r] = log_share(p, set, w, key_to_float(pair_key(s.elements[i])), weights[i], total);
+        logprobs[r] = log_share(p, set, w, key_to_float(pair_key(elements[i])), weights[i], total);
       }
     }
   } else {
-    for (int i = threadIdx.x; i < kTopMax; i += kTopThreads)
-      by_index[i] = i < kept ? order_pair(0xffffffffu - pair_index(s.elements[i]), uint32_t(i)) : 0ull;
-    block_sort_descending(by_index, kTopMax);
+    for (int i = threadIdx.x; i < kept; i += kTopThreads)
+      by_index[i] = order_pair(0xffffffffu - pair_index(elements[i]), uint32_t(i));
+    block_sort_descending<kTopThreads>(by_index, kept);
     sum4 = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -179,7 +178,7 @@ sample_list_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, i
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       if (mine[i] != 0 && before <= goal && goal < before + mine[i]) {
-        const unsigned long long e = s.elements[pair_index(by_index[kEach * int(threadIdx.x) + i])];
+        const unsigned long long e = elements[pair_index(by_index[kEach * int(threadIdx.x) + i])];
         tokens[r] = pair_index(e);
         logprobs[r] = log_share(p, set, w, key_to_float(pair_key(e)), mine[i], total);
       }
@@ -582,10 +581,7 @@ __device__ __forceinline__ RowCut find_place(const RowCluster& c, const RowStret
         place += before;
         if (i < n && threadIdx.x % kShare == 0 && place < target && target <= place + s.pieces[i]) found(mine);
       } else {
-        int padded = 2;
-        while (padded < int(n)) padded <<= 1;
-        for (int i = int(n) + int(threadIdx.x); i < padded; i += kRowThreads) s.gathered[i] = 0;
-        block_sort_descending(s.gathered, padded);
+        block_sort_descending<kRowThreads>(s.gathered, int(n));
         unsigned long long seen = before;
         for (int i0 = 0; i0 < int(n); i0 += kRowThreads) {
           const int i = i0 + int(threadIdx.x);

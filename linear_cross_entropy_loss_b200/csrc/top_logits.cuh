@@ -7,39 +7,44 @@
 namespace lce {
 
 template <typename T>
-__global__ void __launch_bounds__(kTopThreads, 4)
+__global__ void __launch_bounds__(kTopThreads, 3)
 top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int k, int parts, float inv_temperature,
                   T* __restrict__ values, long long* __restrict__ indices, float* __restrict__ lse) {
-  __shared__ TopShared s;
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  TopShared& s = *reinterpret_cast<TopShared*>(dynamic);
   const long long r = blockIdx.x / parts;
   const int part = int(blockIdx.x % parts);
   const RowGroups<T> row(logits + r * ld, vocab);
-  const int share = (row.groups + parts - 1) / parts;
-  const int v0 = min(part * share, row.groups), v1 = min(v0 + share, row.groups);
+  const int v0 = int((long long)row.groups * part / parts), v1 = int((long long)row.groups * (part + 1) / parts);
   const float log2_scale = inv_temperature * 1.4426950408889634f;
   float ref, sum;
-  stream_top<T, true, Nan::kFirst>(s, row, v0, v1, k, log2_scale, ref, sum);
+  stream_top<T, true, Nan::kFirst>(s, row, v0, v1, parts, k, log2_scale, ref, sum);
   const float m = block_max(ref, s.scratch);
   sum = block_sum(ref > -INFINITY ? sum * fast_exp2(ref - m) : 0.f, s.scratch);
   if (threadIdx.x == 0) {
-    s.part_ref = m;
-    s.part_sum = sum;
+    TopShared* first = parts > 1 ? cooperative_groups::this_cluster().map_shared_rank(&s, 0) : &s;
+    first->part_ref[part] = m;
+    first->part_sum[part] = sum;
   }
-  merge_lists(s, k, parts);
+  const TopGroups g = merge_lists(s, k, parts);
   if (part != 0) return;
-  rank_elements<Nan::kFirst>(s, row, k);
-  for (int i = threadIdx.x; i < k; i += kTopThreads) {
-    const unsigned long long e = s.elements[i];
+  const int n = rank_elements<Nan::kFirst>(s, row, g, k);
+  for (int i = threadIdx.x; i < n; i += kTopThreads) {
+    const unsigned long long e = g.free_list[i];
     values[r * k + i] = T(key_to_float(pair_key(e)));
     indices[r * k + i] = pair_index(e);
   }
   if (threadIdx.x == 0) {
+    float top = s.part_ref[0], total = 0.f;
+    for (int i = 1; i < parts; ++i) top = fmaxf(top, s.part_ref[i]);
+    for (int i = 0; i < parts; ++i)
+      if (s.part_ref[i] > -INFINITY) total += s.part_sum[i] * fast_exp2(s.part_ref[i] - top);
     // The sum is over 2^(l * log2_scale), whose exponents are right to the rounding of log2_scale; at the largest
     // logit, which carries the sum, that rounding is put back.
-    const uint32_t first = pair_key(s.elements[0]);
+    const uint32_t first = pair_key(g.free_list[0]);
     const double largest = double(key_to_float(first));
-    const double put_back = largest * (double(inv_temperature) - double(log2_scale) * 0.69314718055994531);
-    float v = float((double(s.part_ref) + double(log2f(s.part_sum))) * 0.69314718055994531 + put_back);
+    const double put_back = largest * (double(inv_temperature) - double(log2_scale) * kLn2);
+    float v = float((double(top) + double(log2f(total))) * kLn2 + put_back);
     if (first >= kKeyPosInf || first == kKeyNegInf) v = key_to_float(first);  // +inf, NaN; nothing but -inf
     lse[r] = v;
   }

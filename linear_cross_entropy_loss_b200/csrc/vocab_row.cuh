@@ -96,24 +96,73 @@ __device__ __forceinline__ T block_prefix(T v, T* scratch /*[32]*/, T* total) {
   return before + inc - v;
 }
 
-// Sorts n (a power of two) numbers in shared memory, largest first.
-__device__ __forceinline__ void block_sort_descending(unsigned long long* a, int n) {
-  for (int size = 2; size <= n; size <<= 1) {
+// Sorts kThreads * kEach numbers in shared memory, largest first (a bitonic network). Thread t holds the places t * kEach ..:
+// strides below kEach stay in its registers, strides below 32 * kEach go through shuffles, and only the few longer ones
+// through shared memory. (All 55 steps of 1024 numbers through shared memory took 21,000 cycles.)
+template <int kThreads, int kEach>
+__device__ __forceinline__ void block_sort_each(unsigned long long* a) {
+  unsigned long long v[kEach];
+  const int first = int(threadIdx.x) * kEach;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) v[i] = a[first + i];
+  for (int size = 2; size <= kThreads * kEach; size <<= 1) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < (n >> 1); i += blockDim.x) {
-        const int lo = ((i & ~(stride - 1)) << 1) | (i & (stride - 1));
-        const int hi = lo | stride;
-        const unsigned long long x = a[lo], y = a[hi];
-        const bool descending = (lo & size) == 0;
-        if ((x < y) == descending) {
-          a[lo] = y;
-          a[hi] = x;
+      if (stride >= 32 * kEach) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) a[first + i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int at = first + i;
+          const unsigned long long other = a[at ^ stride];
+          const bool larger = ((at & size) == 0) == ((at & stride) == 0);  // this place gets the larger of the two
+          v[i] = (other > v[i]) == larger ? other : v[i];
+        }
+      } else if (stride >= kEach) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int at = first + i;
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, v[i], stride / kEach);
+          const bool larger = ((at & size) == 0) == ((at & stride) == 0);
+          v[i] = (other > v[i]) == larger ? other : v[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+          for (int j = 1; j < kEach; j <<= 1) {
+            if (j == stride && (i & j) == 0) {
+              const unsigned long long x = v[i], y = v[i | j];
+              const bool down = ((first + i) & size) == 0;
+              v[i] = (x < y) == down ? y : x;
+              v[i | j] = (x < y) == down ? x : y;
+            }
+          }
         }
       }
     }
   }
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) a[first + i] = v[i];
+  __syncthreads();
+}
+// Sorts the first n numbers of an array that has room for kThreads times a power of two of them (up to 2048 in all),
+// largest first.
+template <int kThreads>
+__device__ __noinline__ void block_sort_descending(unsigned long long* a, int n) {
+  __syncthreads();
+  int each = 1;
+  while (each * kThreads < n) each <<= 1;
+  for (int i = n + int(threadIdx.x); i < each * kThreads; i += kThreads) a[i] = 0;
+  switch (each) {
+    case 1: block_sort_each<kThreads, 1>(a); break;
+    case 2: block_sort_each<kThreads, 2>(a); break;
+    case 4: block_sort_each<kThreads, 4>(a); break;
+    default: block_sort_each<kThreads, 2048 / kThreads>(a);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
