@@ -2,7 +2,8 @@
 
 Same public names as ``linear_cross_entropy`` (the reference package, __init__.py:1):
 ``LinearCrossEntropyLoss``, ``linear_cross_entropy``, ``fwd_configs``, ``bwd_configs``. Beside them, on the same heads:
-``LinearDistillationLoss``, ``linear_distillation``, ``top_logits`` and ``sample_logits``.
+``LinearDistillationLoss``, ``linear_distillation``, ``top_logits`` and ``sample_logits``, the last two also from
+the head's input (``linear_top_logits``, ``linear_sample``, ``linear_logits``).
 """
 from .ops import (  # noqa: F401
     LinearCrossEntropyLoss,
@@ -14,7 +15,16 @@ from .ops import (  # noqa: F401
 )
 
 from .distill import LinearDistillationLoss, linear_distillation  # noqa: F401
-from .head import Sampled, TopLogits, sample_logits, top_logits  # noqa: F401
+from .head import (  # noqa: F401
+    Sampled,
+    TopLogits,
+    linear_logits,
+    linear_sample,
+    linear_top_logits,
+    sample_logits,
+    top_logits,
+)
 
 __all__ = ["LinearCrossEntropyLoss", "linear_cross_entropy", "fwd_configs", "bwd_configs", "set_autocast_policy",
-           "LinearDistillationLoss", "linear_distillation", "top_logits", "TopLogits", "sample_logits", "Sampled"]
+           "LinearDistillationLoss", "linear_distillation", "top_logits", "TopLogits", "sample_logits", "Sampled",
+           "linear_logits", "linear_top_logits", "linear_sample"]

@@ -222,6 +222,8 @@ SIGNATURES = {
     ),
     "lce_align_rows": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp]),
     "lce_grad_scale_pair": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
+    "lce_linear_logits": (
+        ctypes.c_int, [_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _i64, _vp, _vp]),
     "lce_top_logits": (
         ctypes.c_int, [_i32, _vp, _i64, _i64, _i64, _i32, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "lce_sample_logits": (

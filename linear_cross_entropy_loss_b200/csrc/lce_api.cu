@@ -1555,6 +1555,46 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
   return check_launch();
 }
 
+int lce_linear_logits(int32_t dtype, const void* x, int64_t x_ld, const void* weight, int64_t w_ld, int64_t rows,
+                      int64_t hidden, int64_t vocab, float scale, float* out, int64_t out_ld, int32_t* dev_status,
+                      void* stream) {
+  if (dtype != LCE_DTYPE_F16 && dtype != LCE_DTYPE_BF16 && dtype != LCE_DTYPE_F32) return LCE_ERR_INVALID_ARGUMENT;
+  if (!x || !weight || !out || !dev_status || rows <= 0 || hidden <= 0 || vocab <= 0) return LCE_ERR_INVALID_ARGUMENT;
+  if (x_ld < hidden || w_ld < vocab || out_ld < vocab || !(scale > 0.f)) return LCE_ERR_INVALID_ARGUMENT;
+  if (hidden % 8 != 0) return LCE_ERR_UNSUPPORTED_SHAPE;
+  if (rows > (1ll << 30) || hidden > (1ll << 30) || vocab > (1ll << 30)) return LCE_ERR_TOO_LARGE;
+  // (what make_tmap checks, before any device is touched)
+  const long long es = elem_size(dtype);
+  const uintptr_t addresses =
+      reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out);
+  if ((addresses & 15u) != 0 || ((x_ld * es | w_ld * es | out_ld * 4) & 15) != 0) return LCE_ERR_MISALIGNED;
+  int sms = 0;
+  int v = ensure_device(&sms);
+  if (v != LCE_OK) return v;
+  const long long rows_pad = round_up(rows, BLOCK_M), v_pad = round_up(vocab, BLOCK_N);
+  const bool pair = use_pair_kernel(rows_pad / BLOCK_M, sms);
+  CUtensorMap ta, tb, tc;
+  if ((v = make_operand_tmap(&ta, dtype, false, x, hidden, rows, x_ld, BLOCK_M)) != LCE_OK) return v;
+  if ((v = make_operand_tmap(&tb, dtype, true, weight, vocab, hidden, w_ld, rows_of_b_tile(pair))) != LCE_OK) return v;
+  // the map of the output has exactly its rows and columns: TMA drops what a tile has beyond them
+  if ((v = make_store_tmap(&tc, LCE_DTYPE_F32, out, vocab, rows, out_ld)) != LCE_OK) return v;
+  GemmParams gp;
+  memset(&gp, 0, sizeof(gp));
+  gp.m_tiles = (int)(rows_pad / BLOCK_M);
+  gp.n_tiles = (int)(v_pad / BLOCK_N);
+  gp.splits = 1;
+  gp.k_blocks = (int)((hidden * es + 127) / 128);
+  gp.out = out;
+  gp.out_ld = out_ld;
+  gp.out_rows = (int)rows;
+  gp.out_cols = (int)vocab;
+  gp.out_vector_ok = 1;
+  gp.out_scale = scale;
+  gp.out_tma = 1;
+  gp.status = dev_status;
+  return launch_gemm_dtype<false, true, EPI_F32, false>(dtype, ta, tb, tc, gp, sms, (cudaStream_t)stream, pair);
+}
+
 int lce_align_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype, int64_t rows,
                    int64_t cols, void* stream) {
   if (dtype != LCE_DTYPE_F16 && dtype != LCE_DTYPE_BF16 && dtype != LCE_DTYPE_F32) return LCE_ERR_INVALID_ARGUMENT;

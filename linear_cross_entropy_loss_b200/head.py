@@ -2,8 +2,10 @@
 
 ``top_logits`` lists the k largest logits of each row with the row's log-sum-exp -- the form in which a teacher's
 distribution is kept for :func:`linear_distillation`. ``sample_logits`` draws one token per row from given random
-numbers. Both read each logit once and run as one kernel launch in ``liblce_b200.so``, on the current stream of the
-logits' device; like the loss they have no CPU fallback. The reference project has no counterpart of either.
+numbers. Both read the logits once, in ``liblce_b200.so``, on the current stream of the logits' device; like the loss they
+have no CPU fallback. ``linear_logits``, ``linear_top_logits`` and ``linear_sample`` start from the head's input and
+weight instead and take their logits from the contraction of the loss. The reference project has no counterpart of any of
+them.
 """
 from __future__ import annotations
 
@@ -65,6 +67,84 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     if len(lead) != 1:
         values, indices, lse = values.view(*lead, k), indices.view(*lead, k), lse.view(lead)
     return TopLogits(values, indices, lse)
+
+
+def _head_operands(x: torch.Tensor, At: torch.Tensor):
+    """x as (rows, H) and At, as the kernels read them."""
+    from .distill import _operands
+    from .ops import _autocast_target
+
+    assert x.dim() >= 1 and At.dim() == 2 and At.shape[0] == x.shape[-1], "x and the weight disagree on the hidden size"
+    assert At.shape[0] >= 1 and At.shape[1] >= 1
+    assert x.device == At.device, "all tensors must be on one device"
+    x, At = x.detach(), At.detach()
+    target = _autocast_target(x)
+    if target is not None:
+        x, At = x.to(target), At.to(target)
+    assert x.dtype == At.dtype, "x and the weight must have the same dtype"
+    assert x.dtype in _DTYPE_CODE, f"unsupported dtype {x.dtype}"
+    _require_cuda(get_backend(), x)
+    x = x.reshape(-1, x.shape[-1])
+    if x.shape[0] == 0:
+        return x, At
+    with _device_guard(x):
+        return _operands(x, At)
+
+
+def _logit_rows(x, At, scale: float) -> torch.Tensor:
+    """(rows, V) float32 logits, rows on 16-byte boundaries."""
+    V = At.shape[1]
+    out = torch.empty((x.shape[0], -(-V // 4) * 4), dtype=torch.float32, device=x.device)
+    if x.shape[0] > 0:
+        status = torch.zeros(1, dtype=torch.int32, device=x.device)
+        with _device_guard(x):
+            get_backend().linear_logits(x, At, float(scale), out, status)
+    return out if out.shape[1] == V else out[:, :V]
+
+
+def linear_logits(x: torch.Tensor, At: torch.Tensor, logit_scale: float = 1.0) -> torch.Tensor:
+    """``logit_scale * (x @ At)`` in float32, (..., V), from the tensor-core contraction of the loss (products accumulated in
+    fp32; float32 inputs are multiplied as TF32). Not differentiable: the losses never need the logits themselves."""
+    assert logit_scale > 0
+    rows, A = _head_operands(x, At)
+    return _logit_rows(rows, A, logit_scale).reshape(*x.shape[:-1], At.shape[1])
+
+
+def linear_top_logits(x: torch.Tensor, At: torch.Tensor, k: int, temperature: float = 1.0, logit_scale: float = 1.0,
+                      N_chunk_size: int = 4096) -> TopLogits:
+    """:func:`top_logits` of ``logit_scale * (x @ At)``, N_chunk_size rows of logits at a time: a teacher's head."""
+    assert logit_scale > 0 and int(N_chunk_size) >= 1
+    rows, A = _head_operands(x, At)
+    lead, k = x.shape[:-1], int(k)
+    parts = [top_logits(_logit_rows(c, A, logit_scale), k, temperature) for c in rows.split(int(N_chunk_size))]
+    values, indices, lse = parts[0] if len(parts) == 1 else (torch.cat(t) for t in zip(*parts))
+    return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
+
+
+def linear_sample(x: torch.Tensor, At: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  logit_scale: float = 1.0, N_chunk_size: int = 4096) -> Sampled:
+    """:func:`sample_logits` of ``logit_scale * (x @ At)``, N_chunk_size rows of logits at a time: a head that answers."""
+    assert logit_scale > 0 and int(N_chunk_size) >= 1
+    rows, A = _head_operands(x, At)
+    lead, n = x.shape[:-1], rows.shape[0]
+    assert u.shape == lead, "u must have one entry per row of x"
+    u = u.reshape(-1)
+
+    def per_row(v, name):
+        if not isinstance(v, torch.Tensor):
+            return v
+        assert v.numel() in (1, n), f"{name} must be a number or have one entry per row"
+        return v.reshape(-1).expand(n)
+
+    settings = [per_row(v, name) for v, name in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"),
+                                                 (min_p, "min_p"))]
+    parts = []
+    for r in range(0, max(n, 1), int(N_chunk_size)):
+        here = slice(r, r + int(N_chunk_size))
+        parts.append(sample_logits(_logit_rows(rows[here], A, logit_scale), u[here],
+                                   *(v[here] if isinstance(v, torch.Tensor) else v for v in settings)))
+    tokens, logprobs = parts[0] if len(parts) == 1 else (torch.cat(t) for t in zip(*parts))
+    return Sampled(tokens.view(lead), logprobs.view(lead))
 
 
 def _setting(value, name: str, dtype, n: int, device):

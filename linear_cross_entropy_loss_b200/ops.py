@@ -226,6 +226,15 @@ class NativeBackend:
             "lce_grad_scale_pair",
         )
 
+    def linear_logits(self, x, At, scale, out, status):
+        _native.check(
+            self.lib.lce_linear_logits(
+                _DTYPE_CODE[x.dtype], _ptr(x), x.stride(0), _ptr(At), At.stride(0), x.shape[0], x.shape[1], At.shape[1],
+                scale, _ptr(out), out.stride(0), _ptr(status), self._stream(x),
+            ),
+            "lce_linear_logits",
+        )
+
     def top_logits(self, logits, k, temperature, values, indices, lse):
         _native.check(
             self.lib.lce_top_logits(
@@ -875,6 +884,30 @@ class LinearCrossEntropyLoss(torch.nn.Linear):
                 "z_value": z_reg,
             }
         return loss
+
+    @torch.no_grad()
+    def logits(self, x):
+        """``logit_scale * (x @ weight)`` as (..., out_features) float32, from the contraction that the loss is made of
+        (fp32 accumulation, no rounding to the input type)."""
+        from .head import linear_logits
+
+        return linear_logits(x, self.weight, self.logit_scale)
+
+    @torch.no_grad()
+    def top_logits(self, x, k: int, temperature: float = 1.0):
+        """The k largest logits of each row of x with the row's log-sum-exp (:func:`top_logits`): what a teacher's head
+        hands to :func:`linear_distillation`. ``N_chunk_size`` rows of logits exist at a time."""
+        from .head import linear_top_logits
+
+        return linear_top_logits(x, self.weight, k, temperature, self.logit_scale, self.N_chunk_size)
+
+    @torch.no_grad()
+    def sample(self, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One token of each row of x, drawn with the random numbers u (:func:`sample_logits`). ``N_chunk_size`` rows of
+        logits exist at a time."""
+        from .head import linear_sample
+
+        return linear_sample(x, self.weight, u, temperature, top_k, top_p, min_p, self.logit_scale, self.N_chunk_size)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias=False"

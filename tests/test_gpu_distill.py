@@ -7,7 +7,7 @@ import torch
 
 from distill_util import gradient_bounds, loss_bound, reference
 from linear_cross_entropy_loss_b200 import (LinearCrossEntropyLoss, LinearDistillationLoss, linear_cross_entropy,
-                                            linear_distillation, sample_logits, top_logits)
+                                            linear_distillation, linear_logits, sample_logits, top_logits)
 
 pytestmark = pytest.mark.gpu
 
@@ -342,3 +342,62 @@ def test_rows_are_moved_to_boundaries(dtype, rows, cols, ld, offset):
     got = _aligned(src)
     assert torch.equal(got, src) and got.data_ptr() % 16 == 0
     assert rows == 1 or got.stride(0) * got.element_size() % 16 == 0
+
+
+# ---------------------------------------------------------------------------------------------------- the head itself
+def grid_head(N, H, V, dtype, seed):
+    """x and At on grids on which every sum of products is exact in fp32 in any order: multiples of 2^-3 below 4 and of
+    2^-7 below 1/2 give multiples of 2^-10 below 2 H < 2^13."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(N, H, generator=g) * 8).round().clamp(-31, 31) / 8
+    At = (torch.randn(H, V, generator=g) * 16).round().clamp(-63, 63) / 128
+    return x.to(dtype), At.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("N,H,V", [(1, 64, 256), (3, 60, 1001), (130, 128, 5003), (300, 256, 2048)])
+def test_logits_of_a_head(dtype, N, H, V):
+    x, At = grid_head(N, H, V, dtype, N)
+    got = linear_logits(x.cuda(), At.cuda(), 0.5)
+    assert got.dtype == torch.float32 and got.shape == (N, V)
+    assert torch.equal(got.double().cpu(), 0.5 * (x.double() @ At.double()))
+
+
+@pytest.mark.parametrize("N,chunk", [(1, 4096), (50, 4096), (300, 128)])
+def test_head_lists_and_draws_like_its_logits(N, chunk):
+    x, At = grid_head(N, 64, 3001, torch.bfloat16, 7)
+    x, At = x.cuda(), At.cuda()
+    head = LinearCrossEntropyLoss(64, 3001, device="cuda", dtype=torch.bfloat16, logit_scale=0.5, N_chunk_size=chunk)
+    with torch.no_grad():
+        head.weight.copy_(At)
+    logits = head.logits(x)
+    assert torch.equal(logits, (0.5 * (x.double() @ At.double())).float())
+    got, want = head.top_logits(x, 20, temperature=1.5), top_logits(logits, 20, temperature=1.5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got.values.requires_grad
+    u = torch.rand(N, generator=torch.Generator().manual_seed(1)).cuda()
+    T = (0.5 + torch.rand(N, generator=torch.Generator().manual_seed(2))).cuda()
+    for kw in (dict(temperature=T, top_k=30, top_p=0.9), dict(top_p=0.8), dict(temperature=T[:1])):
+        got, want = head.sample(x, u, **kw), sample_logits(logits, u, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = head.sample(x.view(1, N, 64), u.view(1, N), top_k=5)
+    assert got.tokens.shape == (1, N) and got.logprobs.shape == (1, N)
+    assert head.top_logits(x[:0], 3).values.shape == (0, 3) and head.sample(x[:0], u[:0]).tokens.shape == (0,)
+
+
+def test_a_distillation_step_with_two_heads():
+    """The student draws, the teacher lists, the student learns: one step through the modules, against the definition."""
+    torch.manual_seed(1)
+    H, V, B = 64, 2000, 96
+    teacher = LinearCrossEntropyLoss(H, V, device="cuda", dtype=torch.bfloat16)
+    student = LinearDistillationLoss(H, V, device="cuda", dtype=torch.bfloat16, temperature=1.5, N_chunk_size=128)
+    x = torch.randn(B, H, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    tokens, logprobs = student.sample(x, torch.rand(B, device="cuda"), top_p=0.95)
+    assert ((tokens >= 0) & (tokens < V)).all() and (logprobs <= 0).all()
+    lists = teacher.top_logits(x, 16, temperature=1.5)
+    loss = student(x, lists.values, lists.indices, lists.lse)
+    loss.backward()
+    ref = reference(x.detach().cpu(), student.weight.detach().cpu(), lists.values.cpu(), lists.indices.cpu(), 1.5, 1.0, lists.lse.cpu())
+    assert abs(loss.item() - ref["loss"]) <= loss_bound(ref, 1.5, B)
+    bx, bw = gradient_bounds(ref, torch.bfloat16)
+    assert ((x.grad.double().cpu() - ref["dx"]).abs() <= bx).all()
+    assert ((student.weight.grad.double().cpu() - ref["dW"]).abs() <= bw).all()

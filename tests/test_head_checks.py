@@ -4,7 +4,8 @@ import ctypes
 import pytest
 import torch
 
-from linear_cross_entropy_loss_b200 import LinearDistillationLoss, _native, linear_distillation, sample_logits, top_logits
+from linear_cross_entropy_loss_b200 import (LinearDistillationLoss, _native, linear_distillation, linear_logits,
+                                            linear_sample, linear_top_logits, sample_logits, top_logits)
 
 
 @pytest.fixture(scope="module")
@@ -241,3 +242,26 @@ def test_grad_scale_pair_abi_refuses(lib, kw, code):
     a = dict(a=32, b=64, f=16, rows=4, cols=16, ld=16, dtype=1)
     a.update(kw)
     assert lib.lce_grad_scale_pair(a["a"], a["ld"], a["rows"], a["cols"], a["b"], 16, 4, 16, a["dtype"], a["f"], None) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=7), -1), (dict(x=None), -1), (dict(w=None), -1), (dict(out=None), -1), (dict(status=None), -1), (dict(rows=0), -1),
+    (dict(hidden=0), -1), (dict(vocab=0), -1), (dict(x_ld=56), -1), (dict(w_ld=96), -1), (dict(out_ld=96), -1), (dict(scale=0.0), -1),
+    (dict(hidden=60, x_ld=64), -2), (dict(vocab=1 << 31, w_ld=1 << 31, out_ld=1 << 31), -8), (dict(x=24), -3), (dict(out=24), -3), (dict(w_ld=101), -3), (dict(out_ld=101), -3),
+])
+def test_linear_logits_abi_refuses(lib, kw, code):
+    a = dict(dtype=1, x=16, x_ld=64, w=16, w_ld=104, rows=4, hidden=64, vocab=100, scale=1.0, out=16, out_ld=100, status=16)
+    a.update(kw)
+    assert lib.lce_linear_logits(a["dtype"], a["x"], a["x_ld"], a["w"], a["w_ld"], a["rows"], a["hidden"], a["vocab"], a["scale"],
+                                 a["out"], a["out_ld"], a["status"], None) == code
+
+
+def test_head_operators_refuse():
+    x, At = torch.zeros(4, 16), torch.zeros(16, 32)
+    for call in (lambda: linear_logits(x, torch.zeros(15, 32)), lambda: linear_logits(x, At, 0.0), lambda: linear_logits(x, At.half()),
+                 lambda: linear_top_logits(x, At, 3, N_chunk_size=0), lambda: linear_logits(x.double(), At.double())):
+        with pytest.raises(AssertionError):
+            call()
+    for call in (lambda: linear_logits(x, At), lambda: linear_top_logits(x, At, 3), lambda: linear_sample(x, At, torch.zeros(4))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
