@@ -64,7 +64,7 @@ __device__ __forceinline__ RowWeights row_weights(const SampleParams& p, const R
   w.only_largest = largest == INFINITY;
   w.steps = fmin(1.0 / (kStepLn2 * s.temperature), 1e300);
   w.to_int = __hiloint2double((1023 + 52 - p.weight_bits) << 20, 0);  // 2^(52 - bits)
-  w.table = table;
+  w.table = smem_u32(table);
   return w;
 }
 // Smallest prefix whose mass reaches top_p of the whole.
@@ -80,7 +80,7 @@ __device__ __forceinline__ unsigned long long draw_target(double u, unsigned lon
 __device__ __forceinline__ float log_share(const SampleParams& p, const RowSettings& s, const RowWeights& w, float logit,
                                            unsigned long long weight, unsigned long long total) {
   if (s.greedy) return 0.f;
-  if (w.only_largest) return float(log(double(weight) / double(total)));
+  if (w.only_largest) return float(log(double(weight) / double(total)));  // all shares alike
   return float(weight_steps(w, logit) * kStepLn2 - log(ldexp(double(total), -p.weight_bits)));
 }
 __device__ __forceinline__ void draw_nothing(long long r, long long* tokens, float* logprobs) {
@@ -400,6 +400,7 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
   __syncthreads();
   for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) s.bins.low[i] = s.bins.high[i] = 0;
   __syncthreads();
+  const uint32_t spare = uint32_t(kRowBins) + (threadIdx.x & 31);
   for (int step = 0; step < x.steps; ++step)
     x.at_step(step, [&](uint32_t index, float(&l)[RowStretch<T>::kPer]) {
       // Four elements side by side, without branches: what is not active goes, whatever its amount comes out as, to a
@@ -411,7 +412,7 @@ __device__ __forceinline__ Crossing find_bin(const RowCluster& c, const RowStret
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const unsigned long long a = amount(l[i0 + i]);
-          at[i] = active(index + i0 + i, l[i0 + i]) ? bin(l[i0 + i]) : uint32_t(kRowBins) + (threadIdx.x & 31);
+          at[i] = active(index + i0 + i, l[i0 + i]) ? bin(l[i0 + i]) : spare;
           low[i] = uint32_t(a);
           high[i] = uint32_t(a >> 32);
         }
@@ -713,8 +714,12 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     if (c.rank == 0 && threadIdx.x == 0) draw_nothing(r, tokens, logprobs);
     return;  // the whole cluster; nothing of it is read any more
   }
-  const RowWeights w = row_weights(p, set, top, s.table);
-  auto weight = [&](float l) { return w.only_largest ? 1ull << 32 : weight_of_steps(w, weight_steps(w, l)); };
+  RowWeights w = row_weights(p, set, top, s.table);
+  // Of a row with +inf only those are kept: for their weights they are the largest finite number, as is the row's largest
+  // logit then, and all weights come out alike.
+  constexpr float kLargestFinite = 3.4028234663852886e38f;
+  if (w.only_largest) w.largest = kLargestFinite;
+  auto weight = [&](float l) { return weight_of_steps(w, (double(fminf(l, kLargestFinite)) - w.largest) * w.steps); };
 
   // ---- the cuts, among the logits that have any weight. First bins: equal steps of the logit below the largest.
   const double inv_steps = set.temperature * kStepLn2;
@@ -760,7 +765,8 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     x.at_step(step, [&](uint32_t index, float(&l)[kPer]) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const bool is = kept(index + i, l[i]);
+        bool is = l[i] >= cut.value;
+        if (cut.end != kNoEnd) is = kept(index + i, l[i]);
         const unsigned long long a = weight(is ? l[i] : top);
         sum += is ? a : 0ull;
       }

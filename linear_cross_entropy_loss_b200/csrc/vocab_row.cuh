@@ -178,7 +178,7 @@ struct RowWeights {
   double largest;        // the row's largest logit
   double steps;          // kSteps log2(e) / T: logit difference -> n
   double to_int;         // 2^(52 - bits): adding it leaves w * 2^bits in the low bits of the sum
-  const double* table;   // shared memory: 2^(j / kSteps), j = 0 .. kSteps - 1
+  uint32_t table;        // shared-memory address of 2^(j / kSteps), j = 0 .. kSteps - 1
   bool only_largest;     // the largest logit is +inf: it alone has weight
 };
 constexpr int kWeightBits = 44;
@@ -199,7 +199,9 @@ __device__ __forceinline__ unsigned long long weight_of_steps(const RowWeights& 
   double p = fma(y, c * c * c / 6.0, c * c / 2.0);
   p = fma(y, p, c);
   p = fma(y, p, 1.0);
-  p *= w.table[n & (kSteps - 1)];
+  double step;
+  asm("ld.shared.f64 %0, [%1];" : "=d"(step) : "r"(w.table + (uint32_t(n) & (kSteps - 1)) * 8u));
+  p *= step;
   constexpr int kShift = 20 - 7;  // n / kSteps into the exponent
   static_assert(kSteps == 1 << 7, "kShift goes with it");
   p = __hiloint2double(__double2hiint(p) + ((n & ~(kSteps - 1)) << kShift), __double2loint(p));
