@@ -32,7 +32,9 @@
 namespace lce {
 
 enum : int { KIND_F16 = 0, KIND_BF16 = 1, KIND_TF32 = 2 };
-enum : int { EPI_F32 = 0, EPI_FWD = 1 };
+// EPI_FWD_LIST: EPI_FWD that also copies the logits at listed columns; a kernel of its own, so that the cross-entropy's
+// stays as it is
+enum : int { EPI_F32 = 0, EPI_FWD = 1, EPI_FWD_LIST = 2 };
 
 constexpr int BLOCK_M = 128;
 constexpr int BLOCK_N = 256;
@@ -115,7 +117,7 @@ struct GemmParams {
   long long vocab_offset;      // global class id of local column 0
   float scale;                 // logit scale (> 0)
   const float* row_ref;        // [rows] row-reference mode: slab = exp(z - row_ref[i]); null = reference 0
-  // lists of columns whose logits are wanted (distillation; list_idx null = none): row i has the ascending columns
+  // EPI_FWD_LIST: lists of columns whose logits are wanted. Row i has the ascending columns
   // list_idx[i * list_k + e]; those of tile t are e = list_start[t * list_start_ld + i] up to the same of tile t + 1
   const int* list_idx;
   const unsigned short* list_start;
@@ -394,7 +396,7 @@ __device__ __forceinline__ void gather_listed(const GemmParams& p, uint32_t tadd
 //   monitoring: tile_ez = sum_j exp(z - tile_max) * z,  tile_sq = sum_j z^2
 // Two passes over the accumulator (max first). Used for fp16, whose narrow exponent range needs the
 // exponentials normalised per tile; the slab is rescaled to the row's log-sum-exp afterwards.
-template <int kKind, bool kMonitor>
+template <int kKind, bool kMonitor, bool kList>
 __device__ __forceinline__ void epilogue_forward_tilemax(const GemmParams& p, const CUtensorMap* tmC, WarpStage& stage,
                                                          uint32_t taddr, int m_blk, int n_blk, int row_in_tile) {
   using Elem = typename SlabElem<kKind>::type;
@@ -466,7 +468,7 @@ __device__ __forceinline__ void epilogue_forward_tilemax(const GemmParams& p, co
     }
     if (ycol >= 0) p.target_logit[r] = tv * p.scale;
   }
-  if (p.list_idx != nullptr) gather_listed(p, taddr, n_blk, r, row_ok);
+  if (kList) gather_listed(p, taddr, n_blk, r, row_ok);
 }
 
 // Forward epilogue, row-reference mode (bf16 and fp32 slabs, whose exponent range is that of fp32): one pass.
@@ -476,7 +478,7 @@ __device__ __forceinline__ void epilogue_forward_tilemax(const GemmParams& p, co
 // sums of a row simply add up and dZ = exp(ref_i - lse_i) (1 + 2 z_reg lse_i) * slab - onehot needs only a
 // PER-ROW factor: the slab feeds the gradient GEMMs as it is. If |row max - ref_i| turns out to exceed 60 the
 // host-side sequence re-runs the chunk with ref_i = row max (see row_stats_rowref_kernel).
-template <int kKind, bool kMonitor>
+template <int kKind, bool kMonitor, bool kList>
 __device__ __forceinline__ void epilogue_forward_rowref(const GemmParams& p, const CUtensorMap* tmC, WarpStage& stage,
                                                         uint32_t taddr, int m_blk, int n_blk, int row_in_tile) {
   using Elem = typename SlabElem<kKind>::type;
@@ -553,7 +555,7 @@ __device__ __forceinline__ void epilogue_forward_rowref(const GemmParams& p, con
     }
     if (ycol >= 0) p.target_logit[r] = tv * p.scale;
   }
-  if (p.list_idx != nullptr) gather_listed(p, taddr, n_blk, r, row_ok);
+  if (kList) gather_listed(p, taddr, n_blk, r, row_ok);
 }
 
 // fp16 slabs are always normalised per tile; bf16 / fp32 slabs per row unless the launch asks for tiles.
@@ -562,13 +564,13 @@ struct ForwardMode {
   static constexpr bool kRowRef = (kKind != KIND_F16);
 };
 
-template <int kKind, bool kMonitor>
+template <int kKind, bool kMonitor, bool kList>
 __device__ __forceinline__ void epilogue_forward(const GemmParams& p, const CUtensorMap* tmC, WarpStage& stage,
                                                  uint32_t taddr, int m_blk, int n_blk, int row_in_tile) {
   if (ForwardMode<kKind>::kRowRef && !p.tile_mode)
-    epilogue_forward_rowref<kKind, kMonitor>(p, tmC, stage, taddr, m_blk, n_blk, row_in_tile);
+    epilogue_forward_rowref<kKind, kMonitor, kList>(p, tmC, stage, taddr, m_blk, n_blk, row_in_tile);
   else
-    epilogue_forward_tilemax<kKind, kMonitor>(p, tmC, stage, taddr, m_blk, n_blk, row_in_tile);
+    epilogue_forward_tilemax<kKind, kMonitor, kList>(p, tmC, stage, taddr, m_blk, n_blk, row_in_tile);
 }
 
 // Plain fp32 epilogue: result = coef * acc (+ what earlier launches accumulated). It goes to the fp32 array `out`
@@ -927,8 +929,8 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (uint32_t(lane_group * 32) << 16) + uint32_t(acc * BLOCK_N);
-      if (kEpi == EPI_FWD)
-        epilogue_forward<kKind, kMonitor>(p, &tmC, stage, taddr, m_blk, n_blk, row_in_tile);
+      if (kEpi == EPI_FWD || kEpi == EPI_FWD_LIST)
+        epilogue_forward<kKind, kMonitor, kEpi == EPI_FWD_LIST>(p, &tmC, stage, taddr, m_blk, n_blk, row_in_tile);
       else
         epilogue_f32<kKind>(p, &tmC, stage, taddr, m_blk, n_blk, split, row_in_tile);
       tc_fence_before_sync();
@@ -1184,8 +1186,8 @@ lce_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (uint32_t(lane_group * 32) << 16) + uint32_t(acc * BLOCK_N);
-      if (kEpi == EPI_FWD)
-        epilogue_forward<kKind, kMonitor>(p, &tmC, stage, taddr, m_blk128, n_blk, row_in_tile);
+      if (kEpi == EPI_FWD || kEpi == EPI_FWD_LIST)
+        epilogue_forward<kKind, kMonitor, kEpi == EPI_FWD_LIST>(p, &tmC, stage, taddr, m_blk128, n_blk, row_in_tile);
       else
         epilogue_f32<kKind>(p, &tmC, stage, taddr, m_blk128, n_blk, split, row_in_tile);
       tc_fence_before_sync();

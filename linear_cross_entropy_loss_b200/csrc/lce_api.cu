@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstddef>
 #include <cstdio>
 #include <cstdlib>
@@ -52,6 +53,7 @@ cudaError_t set_smem_attr_kind() {
   cudaError_t e;
   if ((e = set_smem_attr<kKind, false, true, EPI_FWD, false>()) != cudaSuccess) return e;
   if ((e = set_smem_attr<kKind, false, true, EPI_FWD, true>()) != cudaSuccess) return e;
+  if ((e = set_smem_attr<kKind, false, true, EPI_FWD_LIST, false>()) != cudaSuccess) return e;
   if ((e = set_smem_attr<kKind, false, false, EPI_F32, false>()) != cudaSuccess) return e;
   if ((e = set_smem_attr<kKind, true, true, EPI_F32, false>()) != cudaSuccess) return e;
   if ((e = set_smem_attr<kKind, false, true, EPI_F32, false>()) != cudaSuccess) return e;
@@ -552,6 +554,8 @@ int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void*
   const long long* lab = reinterpret_cast<const long long*>(labels) + row0;
   float* parts = row_parts_local != nullptr ? row_parts_local + local0 : nullptr;
   auto launch_forward = [&]() {
+    if (distill != nullptr)
+      return launch_gemm_dtype<false, true, EPI_FWD_LIST, false>(p->dtype, ta, tb, tc, gp, sms, st, pair);
     return p->monitoring ? launch_gemm_dtype<false, true, EPI_FWD, true>(p->dtype, ta, tb, tc, gp, sms, st, pair)
                          : launch_gemm_dtype<false, true, EPI_FWD, false>(p->dtype, ta, tb, tc, gp, sms, st, pair);
   };
@@ -586,7 +590,6 @@ int forward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void*
     GemmParams pp = gp;
     pp.n_tiles = kProbeTiles;
     pp.store_slab = 0;
-    pp.list_idx = nullptr;
     if ((v = launch_gemm_dtype<false, true, EPI_FWD, false>(p->dtype, ta, tb, tc, pp, sms, st, pair)) != LCE_OK) return v;
     probe_ref_kernel<<<(int)((rows + 255) / 256), 256, 0, st>>>(gp.tile_max, p->chunk_rows, kProbeTiles, (int)rows,
                                                                w.row_ref + local0);
@@ -1473,7 +1476,8 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
   int v = validate_distill(p_in, teacher->k);
   if (v != LCE_OK) return v;
   const float temperature = teacher->temperature;
-  if (!(temperature > 0.f) || !(temperature < INFINITY)) return LCE_ERR_INVALID_ARGUMENT;
+  if (!(temperature > 0.f) || !(temperature < INFINITY) || !(1.f / temperature < INFINITY))
+    return LCE_ERR_INVALID_ARGUMENT;
   if (teacher->logits_dtype != LCE_DTYPE_F16 && teacher->logits_dtype != LCE_DTYPE_BF16 &&
       teacher->logits_dtype != LCE_DTYPE_F32)
     return LCE_ERR_INVALID_ARGUMENT;
