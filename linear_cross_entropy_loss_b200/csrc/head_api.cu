@@ -4,6 +4,7 @@
 #include "top_logits.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -71,13 +72,14 @@ int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size
   return check_launch();
 }
 
-// Blocks that share a row: doubled while the blocks of all rows fit the GPU at once (three of kTopThreads on an SM), a part
-// keeps a whole batch, and the lists of all parts fit one.
+// Blocks that share a row: doubled while the blocks of all rows fit the GPU at once (three of kTopThreads on an SM),
+// a part keeps a whole batch, and the lists of all parts fit one.
 template <typename T>
 int top_parts(int64_t rows, int64_t vocab, int k) {
   const int64_t batch = (int64_t)kTopBatch * (32 / (int)sizeof(T));
   int parts = 1;
-  while (parts < kTopParts && rows * parts * 2 <= 3ll * sm_count() && vocab >= batch * parts && k * parts * 2 <= kTopList) parts *= 2;
+  while (parts < kTopParts && rows * parts * 2 <= 3ll * sm_count() && vocab >= batch * parts && k * parts * 2 <= kTopList)
+    parts *= 2;
   return parts;
 }
 
@@ -92,9 +94,9 @@ int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
                          reinterpret_cast<T*>(values), reinterpret_cast<long long*>(indices), lse);
 }
 
-// Blocks that share a row of sample_row_kernel, and the vectors of 16 bytes that each keeps in shared memory (0: too long a
-// row, it is read again for each sweep). A block keeps up to 65 KiB, so that two are on an SM; few rows are split further, down to 8 KiB; up
-// to 176 KiB where eight blocks are not enough.
+// Blocks that share a row of sample_row_kernel, and the vectors of 16 bytes that each keeps in shared memory (0: too
+// long a row, it is read again for each sweep). A block keeps up to 65 KiB, so that two are on an SM; few rows are
+// split further, down to 8 KiB; up to 176 KiB where eight blocks are not enough.
 constexpr int64_t kRowCacheMax = 176 << 10;
 static_assert((sizeof(RowShared) + 15) / 16 * 16 + kRowCacheMax <= 232448, "dynamic shared memory limit of sm_100");
 void row_layout(int64_t rows, int64_t vocab, int es, int* parts, int* cache_vectors) {
@@ -114,9 +116,9 @@ int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, 
   const T* logits = reinterpret_cast<const T*>(logits_);
   long long* tokens = reinterpret_cast<long long*>(tokens_);
   p.weight_bits = kWeightBits;  // the sum over the row stays below 2^62
-  while (p.weight_bits > 0 && (vocab << p.weight_bits) > (1ll << 62)) --p.weight_bits;
-  // top_k for all rows: one of the two kernels has them all, but for greedy rows, which the list has. A top_k for each row: both run,
-  // and a cluster whose row is the other's ends at once.
+  while (vocab > (1ll << (62 - p.weight_bits))) --p.weight_bits;
+  // top_k for all rows: one of the two kernels has them all, but for greedy rows, which the list has. A top_k for
+  // each row: both run, and a cluster whose row is the other's ends at once.
   const bool each = p.top_k != nullptr;
   const int want = each ? 256 : (int)std::min<long long>(std::max<long long>(p.top_k_all, 1), kTopMax);
   const int list_parts = top_parts<T>(rows, vocab, want);
@@ -149,7 +151,9 @@ int lce_top_logits(int32_t dtype, const void* logits, int64_t ld, int64_t rows, 
                    float temperature, void* values, int64_t* indices, float* lse, void* stream) {
   const int v = check_rows(dtype, logits, ld, rows, vocab);
   if (v != LCE_OK) return v;
-  if (k < 1 || !(temperature > 0.f)) return LCE_ERR_INVALID_ARGUMENT;
+  // (a temperature whose reciprocal is a number too)
+  if (k < 1 || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.f / temperature < INFINITY))
+    return LCE_ERR_INVALID_ARGUMENT;
   if (k > vocab || k > LCE_TOP_MAX) return LCE_ERR_TOO_LARGE;
   if (rows == 0) return LCE_OK;
   if (!values || !indices || !lse) return LCE_ERR_INVALID_ARGUMENT;

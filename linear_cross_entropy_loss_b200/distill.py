@@ -58,8 +58,8 @@ def _run_pass(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size, want_d
     dx = torch.empty((N, H), dtype=x.dtype, device=dev) if want_dx else None
     dW = dW_res = None
     if want_dW:
-        # rows on 32-byte boundaries (16 elements of the 16-bit types): the contraction then writes whole sectors. On 16-byte
-        # ones it goes element by element: 556 against 80 us for 1000 x 50257 in fp16.
+        # rows on 32-byte boundaries (16 elements of the 16-bit types): the contraction then writes whole sectors. On
+        # 16-byte ones it goes element by element: 556 against 86 us for 1000 x 1000 x 50257 in fp16.
         dW = _aligned_rows_like((H, V), At.dtype, dev, 16)
         if N > N_group and At.dtype != torch.float32:
             dW_res = _aligned_rows_like((H, V), At.dtype, dev, 16)  # the rounding residual of the sum over the chunks
@@ -151,20 +151,21 @@ def linear_distillation(
     """The distillation loss of the head ``x @ At`` against a teacher's top logits (a scalar, float32).
 
     x: (..., H); At: (H, V), the transposed weight of :class:`LinearCrossEntropyLoss`; float16, bfloat16 or float32
-    (multiplied as TF32), any sizes. teacher_logits: (..., K) in any of these types; teacher_indices: (..., K) int64 or int32;
-    1 <= K <= 1024. Both as :func:`top_logits` returns them; any order will do.
+    (multiplied as TF32), any sizes. teacher_logits: (..., K) in any of these types; teacher_indices: (..., K) int64 or
+    int32; 1 <= K <= 1024. Both as :func:`top_logits` returns them; any order will do.
 
     The teacher's distribution is softmax(teacher_logits / temperature) over the K listed tokens, or, with
-    teacher_lse: (...) = logsumexp(all teacher logits / temperature), exp(teacher_logits / temperature - teacher_lse): then the
-    mass that the list leaves out has no target, and the student's mass on the listed tokens is drawn to Q = sum(q) times
-    its softmax. teacher_lse has to be at least the log-sum-exp of the listed logits.
+    teacher_lse: (...) = logsumexp(all teacher logits / temperature), exp(teacher_logits / temperature - teacher_lse):
+    then the mass that the list leaves out has no target, and with Q = sum(q) < 1 the gradient of a row's logits is
+    Q softmax - q. teacher_lse has to be at least the log-sum-exp of the listed logits.
 
-    An entry with an index outside [0, V) is not there, whatever its logit (lists of different lengths are padded with -1); one
-    with logit -inf has no weight; rows without any weight do not count (if none counts, the loss is NaN, like that of the
-    cross-entropy). NaN or +inf in an entry that is there make the loss NaN. An index that is listed twice counts twice.
+    An entry with an index outside [0, V) is not there, whatever its logit (lists of different lengths are padded with
+    -1); one with logit -inf has no weight; rows without any weight do not count (if none counts, the loss is NaN, like
+    that of the cross-entropy). NaN or +inf in an entry that is there make the loss NaN. An index that is listed twice
+    counts twice.
 
-    Gradients for x and At only (those that are wanted are computed during the forward pass); under CUDA autocast x and At
-    are cast as :func:`set_autocast_policy` says.
+    Gradients for x and At only (those that are wanted are computed during the forward pass; no second derivatives);
+    under CUDA autocast x and At are cast as :func:`set_autocast_policy` says.
     """
     assert x.dim() >= 1 and At.dim() == 2 and At.shape[0] == x.shape[-1], "x and the weight disagree on the hidden size"
     rows = x.shape[:-1]
@@ -174,7 +175,7 @@ def linear_distillation(
     assert 1 <= k <= _native.TEACHER_MAX, f"between 1 and {_native.TEACHER_MAX} entries per row"
     assert teacher_logits.dtype in _DTYPE_CODE, f"unsupported dtype {teacher_logits.dtype} of teacher_logits"
     assert teacher_indices.dtype in (torch.int64, torch.int32), "teacher_indices must be int64 or int32"
-    assert temperature > 0 and temperature < float("inf"), "temperature must be positive"
+    assert 2**-126 <= temperature < float("inf"), "temperature must be positive"
     assert logit_scale > 0
     assert int(N_chunk_size) >= 1
     assert x.numel() > 0 and At.shape[1] >= 1, "x must have at least one row"
@@ -202,16 +203,59 @@ def linear_distillation(
 
     if not torch.is_grad_enabled():
         x, At = x.detach(), At.detach()
+    if torch.compiler.is_compiling():
+        want_grad = torch.is_grad_enabled() and (x.requires_grad or At.requires_grad)
+        return distillation_op(x, At, teacher_logits.detach(), teacher_indices, teacher_lse, float(temperature),
+                               float(logit_scale), int(N_chunk_size), want_grad)[0]
     return LinearDistillationImplementation.apply(
         x, At, lists(teacher_logits), lists(teacher_indices), teacher_lse, temperature, logit_scale, N_chunk_size)
+
+
+# While a compiler traces, the pass is one opaque operator with its gradients among the outputs, as for the loss.
+@torch.library.custom_op("lce_b200::distillation", mutates_args=())
+def distillation_op(x: torch.Tensor, At: torch.Tensor, t: torch.Tensor, idx: torch.Tensor, lse: Optional[torch.Tensor],
+                    temperature: float, logit_scale: float, N_chunk_size: int,
+                    want_grad: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss, dx, dAt); the gradients are empty without want_grad."""
+    xd, Ad = x.detach(), At.detach()
+    if not want_grad:
+        return linear_distillation(xd, t, idx, Ad, lse, temperature, logit_scale, N_chunk_size), x.new_empty(0), x.new_empty(0)
+    with torch.enable_grad():
+        xd, Ad = xd.requires_grad_(), Ad.requires_grad_()
+        loss = linear_distillation(xd, t, idx, Ad, lse, temperature, logit_scale, N_chunk_size)
+    dx, dA = loss.grad_fn.lce_grads
+    return loss.detach(), dx.reshape(x.shape), dA
+
+
+@distillation_op.register_fake
+def _distillation_fake(x, At, t, idx, lse, temperature, logit_scale, N_chunk_size, want_grad):
+    loss = x.new_empty((), dtype=torch.float32)
+    if not want_grad:
+        return loss, x.new_empty(0), x.new_empty(0)
+    return loss, x.new_empty(x.shape), At.new_empty(At.shape)
+
+
+def _distillation_setup(ctx, inputs, output):
+    ctx.lce_want_grad = inputs[-1]
+    ctx.save_for_backward(output[1], output[2])
+
+
+def _distillation_backward(ctx, grad_loss, grad_dx, grad_dA):
+    if not ctx.lce_want_grad:
+        raise RuntimeError("the distillation loss was traced without gradients")
+    dx, dA = ctx.saved_tensors
+    return (dx * grad_loss).to(dx.dtype), (dA * grad_loss).to(dA.dtype), None, None, None, None, None, None, None
+
+
+distillation_op.register_autograd(_distillation_backward, setup_context=_distillation_setup)
 
 
 class LinearDistillationLoss(LinearCrossEntropyLoss):
     """The head of :class:`LinearCrossEntropyLoss` (same constructor, weight and ``state_dict``) with
     ``forward(x, teacher_logits, teacher_indices, teacher_lse=None)`` = :func:`linear_distillation`.
 
-    Assign ``distill.weight = head.weight`` to train one weight with both losses. ``ignore_index``, ``z_regularization`` and
-    ``monitoring`` have no meaning here.
+    Assign ``distill.weight = head.weight`` to train one weight with both losses. ``ignore_index``, ``z_regularization``
+    and ``monitoring`` have no meaning here.
     """
 
     def __init__(self, in_features: int, out_features: int, device=None, dtype=None, temperature: float = 1.0,

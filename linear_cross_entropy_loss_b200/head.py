@@ -2,14 +2,14 @@
 
 ``top_logits`` lists the k largest logits of each row with the row's log-sum-exp -- the form in which a teacher's
 distribution is kept for :func:`linear_distillation`. ``sample_logits`` draws one token per row from given random
-numbers. Both read the logits once, in ``liblce_b200.so``, on the current stream of the logits' device; like the loss they
-have no CPU fallback. ``linear_logits``, ``linear_top_logits`` and ``linear_sample`` start from the head's input and
+numbers. Both read the logits once, in ``liblce_b200.so``, on the current stream of the logits' device; like the loss
+they have no CPU fallback. ``linear_logits``, ``linear_top_logits`` and ``linear_sample`` start from the head's input and
 weight instead and take their logits from the contraction of the loss. The reference project has no counterpart of any of
 them.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Union
+from typing import NamedTuple, Optional, Union
 
 import torch
 
@@ -54,7 +54,9 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     rows = _rows_of(logits)
     assert 1 <= k <= rows.shape[1], "k must lie between 1 and the number of columns"
     assert k <= _native.TOP_MAX, f"k must be at most {_native.TOP_MAX}"
-    assert temperature > 0, "temperature must be positive"
+    assert 2**-126 <= temperature < float("inf"), "temperature must be positive"
+    if torch.compiler.is_compiling():
+        return TopLogits(*top_logits_op(logits, k, float(temperature)))
     backend = get_backend()
     _require_cuda(backend, rows)
     lead = logits.shape[:-1]
@@ -103,8 +105,8 @@ def _logit_rows(x, At, scale: float) -> torch.Tensor:
 
 
 def linear_logits(x: torch.Tensor, At: torch.Tensor, logit_scale: float = 1.0) -> torch.Tensor:
-    """``logit_scale * (x @ At)`` in float32, (..., V), from the tensor-core contraction of the loss (products accumulated in
-    fp32; float32 inputs are multiplied as TF32). Not differentiable: the losses never need the logits themselves."""
+    """``logit_scale * (x @ At)`` in float32, (..., V), from the tensor-core contraction of the loss (products accumulated
+    in fp32; float32 inputs are multiplied as TF32). Not differentiable: the losses never need the logits themselves."""
     assert logit_scale > 0
     rows, A = _head_operands(x, At)
     return _logit_rows(rows, A, logit_scale).reshape(*x.shape[:-1], At.shape[1])
@@ -177,12 +179,18 @@ def sample_logits(
     w_j >= ``min_p``. The token is the first one in INDEX order at which the kept weights, added up, exceed u times their
     sum; ``logprobs`` is log(w / sum). temperature 0 gives the largest logit (the lowest index among equals).
 
-    Each setting is a number, which is checked, or a tensor with one entry per row (float32; ``top_k`` int32), which is not: out-of-range
-    entries are taken as the nearest value that means something. -inf and NaN logits are never drawn; +inf logits share
-    all the mass. A row without any logit to draw gives token -1 and logprob -inf.
+    Each setting is a number, which is checked, or a tensor with one entry per row (taken as float32; ``top_k`` as int32),
+    which is not: out-of-range entries are taken as the nearest value that means something. -inf and NaN logits are never
+    drawn; +inf logits share all the mass. A row without any logit to draw gives token -1 and logprob -inf.
 
     Weights and sums are kept in 64-bit integers, so the answer for a row depends on its inputs alone.
     """
+    if torch.compiler.is_compiling():
+        given = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
+        numbers = [default if isinstance(v, torch.Tensor) else v
+                   for v, default in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0))]
+        return Sampled(*sample_logits_op(logits, u, *given, float(numbers[0]), int(numbers[1]), float(numbers[2]),
+                                         float(numbers[3])))
     rows = _rows_of(logits)
     n, dev = rows.shape[0], rows.device
     assert u.numel() == n, "u must have one entry per row of the logits"
@@ -197,7 +205,7 @@ def sample_logits(
                                ("top_p", torch.float32, top_p), ("min_p", torch.float32, min_p)):
         number, tensor = _setting(value, name, dtype, n, dev)
         if tensor is None:
-            setattr(s, f"{name}_all", int(number) if name == "top_k" else float(number))
+            setattr(s, f"{name}_all", min(int(number), 2**62) if name == "top_k" else float(number))
         else:
             alive.append(tensor)
             setattr(s, name, tensor.data_ptr())
@@ -213,3 +221,34 @@ def sample_logits(
         backend.sample_logits(rows, s, tokens, logprobs)
     lead = logits.shape[:-1]
     return Sampled(tokens, logprobs) if len(lead) == 1 else Sampled(tokens.view(lead), logprobs.view(lead))
+
+
+# ------------------------------------------------------------------------------------------------
+# torch.library registration, as for the loss: while a compiler traces, each call is one opaque operator.
+# ------------------------------------------------------------------------------------------------
+@torch.library.custom_op("lce_b200::top_logits", mutates_args=())
+def top_logits_op(logits: torch.Tensor, k: int, temperature: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(top_logits(logits, k, temperature))
+
+
+@top_logits_op.register_fake
+def _top_logits_fake(logits, k, temperature):
+    lead = logits.shape[:-1]
+    return (logits.new_empty((*lead, k)), logits.new_empty((*lead, k), dtype=torch.int64),
+            logits.new_empty(lead, dtype=torch.float32))
+
+
+@torch.library.custom_op("lce_b200::sample_logits", mutates_args=())
+def sample_logits_op(logits: torch.Tensor, u: torch.Tensor, temperatures: Optional[torch.Tensor],
+                     top_ks: Optional[torch.Tensor], top_ps: Optional[torch.Tensor], min_ps: Optional[torch.Tensor],
+                     temperature: float, top_k: int, top_p: float, min_p: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """Each setting as a tensor, or, where that is None, as a number."""
+    return tuple(sample_logits(logits, u, temperature if temperatures is None else temperatures,
+                               top_k if top_ks is None else top_ks, top_p if top_ps is None else top_ps,
+                               min_p if min_ps is None else min_ps))
+
+
+@sample_logits_op.register_fake
+def _sample_logits_fake(logits, u, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p):
+    lead = logits.shape[:-1]
+    return logits.new_empty(lead, dtype=torch.int64), logits.new_empty(lead, dtype=torch.float32)

@@ -344,6 +344,26 @@ def test_rows_are_moved_to_boundaries(dtype, rows, cols, ld, offset):
     assert rows == 1 or got.stride(0) * got.element_size() % 16 == 0
 
 
+def test_traced_by_torch_compile_without_a_graph_break():
+    x, At, t, idx = problem(100, 64, 700, 6, torch.bfloat16, seed=25)
+    want = run(x, At, t, idx, temperature=1.5)
+    xd, Ad, td, id_ = x.cuda().requires_grad_(), At.cuda().requires_grad_(), t.cuda(), idx.cuda()
+    step = torch.compile(lambda a, b: 2.0 * linear_distillation(a, td, id_, b, temperature=1.5), fullgraph=True, backend="aot_eager")
+    loss = step(xd, Ad)
+    loss.backward()
+    assert loss.item() == 2 * want[0]
+    assert torch.equal(xd.grad, 2 * want[1]) and torch.equal(Ad.grad, 2 * want[2])
+
+
+def test_second_derivatives_are_refused():
+    x, At, t, idx = problem(16, 64, 300, 4, torch.bfloat16)
+    xd = x.cuda().requires_grad_()
+    loss = linear_distillation(xd, t.cuda(), idx.cuda(), At.cuda())
+    (g,) = torch.autograd.grad(loss, xd, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
 # ---------------------------------------------------------------------------------------------------- the head itself
 def grid_head(N, H, V, dtype, seed):
     """x and At on grids on which every sum of products is exact in fp32 in any order: multiples of 2^-3 below 4 and of

@@ -297,3 +297,56 @@ def test_calls_side_by_side_on_two_streams():
     for runs in got:
         for run in runs[1:]:
             assert all(torch.equal(p, q) for p, q in zip(run, runs[0]))
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 500003), (torch.bfloat16, 1000003), (torch.float16, 3000001)])
+def test_rows_longer_than_shared_memory(dtype, V):
+    logits = normal(2, V, dtype, seed=V).cuda()
+    logits[1, ::2] = -INF
+    check_top(logits, 50)
+    check_top(logits, 1024, T=3.0)
+    for settings in (dict(), dict(top_p=0.9), dict(min_p=0.01), dict(top_k=5000, top_p=0.9), dict(top_k=40)):
+        check_sample(logits, uniform(2, V), **settings)
+    equal = torch.full((1, V), 0.5, dtype=dtype).cuda()
+    check_sample(equal, uniform(1, V), top_p=0.3)
+    check_sample(equal, uniform(1, V), top_k=1500)
+    check_top(equal, 300)
+
+
+@pytest.mark.parametrize("T", [1e38, 3e37, 1e30, float("inf")])
+def test_sample_logits_spans_that_a_float_does_not_hold(T):
+    rows = normal(4, 2000, torch.float32, seed=6)
+    rows[:, ::3] = torch.finfo(torch.float32).max
+    rows[:, 1::3] = torch.finfo(torch.float32).min
+    for settings in (dict(), dict(top_p=0.5), dict(top_p=0.95), dict(top_k=1500), dict(min_p=0.2)):
+        check_sample(rows.cuda(), uniform(4), T=T, **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_logits_many_values_in_one_bin(dtype):
+    """A temperature so high that a whole row of different logits falls into the first bins."""
+    logits = normal(3, 40000, dtype, seed=2).cuda()
+    for settings in (dict(top_p=0.5), dict(top_k=20000), dict(top_k=30000, top_p=0.7)):
+        check_sample(logits, uniform(3), T=300.0, **settings)
+
+
+def test_rows_in_rising_order_split_over_blocks():
+    """All of the largest logits lie in the last part of a row: its list runs full."""
+    up = torch.linspace(-20, 20, 131072).repeat(2, 1)
+    up[1] = up[1].flip(0)
+    for k in (1, 64, 512, 1024):
+        check_top(up.cuda(), k)
+        check_top(up.to(torch.bfloat16).cuda(), k)
+    check_sample(up.cuda(), uniform(2), top_k=100, top_p=0.9)
+
+
+@pytest.mark.parametrize("what", ["top", "sample"])
+def test_traced_by_torch_compile_without_a_graph_break(what):
+    logits, u = normal(6, 500, torch.bfloat16).cuda(), uniform(6)
+    T = torch.full((6,), 0.8).cuda()
+    if what == "top":
+        call = lambda x, v: tuple(top_logits(x + 0, 9, temperature=1.5))  # noqa: E731
+    else:
+        call = lambda x, v: tuple(sample_logits(x + 0, v, temperature=T, top_k=20, top_p=0.9))  # noqa: E731
+    got = torch.compile(call, fullgraph=True, backend="aot_eager")(logits, u)
+    assert all(torch.equal(a, b) for a, b in zip(got, call(logits, u)))

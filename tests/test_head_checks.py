@@ -14,7 +14,7 @@ def lib():
 
 
 @pytest.mark.parametrize("kw", [dict(k=0), dict(k=-1), dict(k=9), dict(k=3, temperature=0.0), dict(k=3, temperature=-1.0),
-                                dict(k=3, temperature=float("nan"))])
+                                dict(k=3, temperature=float("nan")), dict(k=3, temperature=float("inf")), dict(k=3, temperature=1e-39)])
 def test_top_logits_refuses(kw):
     with pytest.raises(AssertionError):
         top_logits(torch.zeros(2, 8), **kw)
@@ -55,7 +55,7 @@ def test_there_is_no_cpu_fallback():
 
 @pytest.mark.parametrize("change,code", [
     (dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(logits=None), -1), (dict(ld=-1), -1), (dict(rows=-1), -1),
-    (dict(vocab=0), -1), (dict(k=0), -1), (dict(t=0.0), -1), (dict(t=float("nan")), -1), (dict(values=None), -1),
+    (dict(vocab=0), -1), (dict(k=0), -1), (dict(t=0.0), -1), (dict(t=float("nan")), -1), (dict(values=None), -1), (dict(t=float("inf")), -1), (dict(t=1e-40), -1),
     (dict(indices=None), -1), (dict(lse=None), -1), (dict(k=101), -8), (dict(vocab=4000, k=1025), -8),
     (dict(vocab=1 << 31), -8), (dict(rows=1 << 31), -8), (dict(logits=17), -3), (dict(dtype=2, logits=18), -3),
 ])
