@@ -292,6 +292,7 @@ int lce_eval_loss_static(const lce_problem* p, const void* x, int64_t x_ld, cons
  * without weight do not count (n = rows that do; none: the loss is NaN). NaN or +inf in an entry that is there makes
  * the loss NaN. The same index twice in a row: both count.
  * p: as for lce_fused_pass; ignore_index is not used; z_regularization and monitoring must be 0, chunk_buffers 0 or 1.
+ * lse, where given, has to be at least the log-sum-exp of the row's entries. Nothing of it is checked on the device.
  * workspace: lce_distill_workspace_bytes() bytes. dx (element type of x), dweight, dweight_residual: as for lce_fused_pass.
  * loss: one float. Nothing synchronises, nothing is allocated. */
 #define LCE_TEACHER_MAX 1024
@@ -311,8 +312,8 @@ int lce_distill_pass(const lce_problem* p, const lce_teacher* teacher, const voi
                      const void* weight, int64_t w_ld, void* workspace, void* dx, int64_t dx_ld, void* dweight,
                      int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, float* loss, void* stream);
 
-/* dst[r, c] = src[r, c] for src rows that start anywhere (src_ld elements apart) and dst rows on 16-byte boundaries: what x and W
- * need before a pass when their sizes are not multiples of 16 bytes. Whole vectors of 16 bytes are written, so dst_ld must
+/* dst[r, c] = src[r, c] for src rows that start anywhere (src_ld elements apart) and dst rows on 16-byte boundaries:
+ * what x and W need before a pass when their sizes are not multiples of 16 bytes. Whole vectors of 16 bytes are written, so dst_ld must
  * be at least cols rounded up to them; what lies behind column cols is unspecified. No counterpart in the reference. */
 int lce_align_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype, int64_t rows,
                    int64_t cols, void* stream);
@@ -331,8 +332,8 @@ int lce_linear_logits(int32_t dtype, const void* x, int64_t x_ld, const void* we
                       void* stream);
 
 /* ---- operators on given logits ------------------------------------------------------------------
- * No counterpart in the reference. They need no workspace; logits: [rows, vocab] device memory of element type dtype, rows
- * ld elements apart (ld >= 0, any alignment of the element type).
+ * No counterpart in the reference. They need no workspace; logits: [rows, vocab] device memory of element type dtype,
+ * rows ld elements apart (ld >= 0, any alignment of the element type).
  *
  * lce_top_logits: the k largest logits of each row, descending, equal ones by ascending index (-0 equals +0, a NaN
  * is larger than everything), and lse = log(sum_j exp(logit_j / temperature)).
@@ -342,18 +343,18 @@ int lce_linear_logits(int32_t dtype, const void* x, int64_t x_ld, const void* we
  * the order (logit descending, index ascending): the first top_k of the order stay (0: all); of those the shortest
  * prefix whose mass reaches top_p of their mass (1: all); of those w_j >= min_p (0: all). The token is the first
  * one in index order at which the kept weights, added up, exceed u * (their sum); logprobs = log(w / their sum).
- * temperature 0: the largest logit with the lowest index. -inf and NaN logits are never drawn; +inf logits share all the
- * mass. A row without any logit that may be drawn gives token -1 and logprob -inf.
+ * temperature 0: the largest logit with the lowest index. -inf and NaN logits are never drawn; +inf logits share all
+ * the mass. A row without any logit that may be drawn gives token -1 and logprob -inf.
  * Weights and their sums are held in 64-bit integers: the answer does not depend on the order of summation. */
 #define LCE_TOP_MAX 1024
 int lce_top_logits(int32_t dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, int32_t k,
                    float temperature, void* values, int64_t* indices, float* lse, void* stream);
 
 #define LCE_SAMPLING_U_F64 3 /* u_dtype: double (LCE_DTYPE_F32: float) */
-/* Each setting is one value for all rows, or -- where the pointer is not null -- one device value per row. Values
- * out of range in device memory are taken as the nearest that means something: temperature <= 0 or NaN as 0, top_k <= 0 as all,
- * top_p <= 0 as the first token alone, >= 1 or NaN as all, min_p <= 0 or NaN as none, > 1 as 1; u outside [0, 1) as
- * the nearest inside. The values for all rows are checked (LCE_ERR_INVALID_ARGUMENT). */
+/* Each setting is one value for all rows, or -- where the pointer is not null -- one device value per row. Values out of
+ * range in device memory are taken as the nearest that means something: temperature <= 0 or NaN as 0, top_k <= 0 as all,
+ * top_p <= 0 as the first token alone, >= 1 or NaN as all, min_p <= 0 or NaN as none, > 1 as 1; u outside [0, 1) as the
+ * nearest inside, NaN as 0. The values for all rows are checked (LCE_ERR_INVALID_ARGUMENT). */
 typedef struct lce_sampling {
   const void* u;            /* [rows] random numbers in [0, 1) */
   const float* temperature; /* [rows] or null */

@@ -1,17 +1,23 @@
 // The k largest logits of a row, found while the row streams past once.
 //
-// The row is looked at in groups of 32 bytes (8 or 16 logits). The k groups that come first by (largest logit descending,
-// place ascending) hold the k first logits, since a group ahead of another has a logit ahead of all of its. So only the groups'
-// maxima are kept, and the search works on them:
+// The row is looked at in groups of 32 bytes (8 or 16 logits). The k groups that come first by (largest logit
+// descending, place ascending) hold the k first logits, since a group ahead of another has a logit ahead of all of
+// its. So only the groups' maxima are kept, and the search works on them:
 //
 // 1. Stream: each thread loads two groups at a time, the next two on their way; a group's maximum goes to shared memory,
 //    and four running maxima of the thread's groups stay in registers. No barrier, nothing that depends on the data.
-// 2. Bound: the k-th largest of the block's 1024 running maxima. At least k groups reach it, and of a row of random order
-//    about k (1 + k / 2048) do.
+// 2. Bound: the k-th largest of the block's 1024 running maxima. At least k groups reach it, and of a row of random
+//    order about k (1 + k / 2048) do.
 // 3. Collect: the groups that reach the bound go to a list. If it runs full (rows in an unlucky order, many equal
-//    logits, several segments) it is cut back to its first k and the bound raised behind the last of them: an equal maximum that
-//    comes later is behind.
+//    logits, several segments) it is cut back to its first k and the bound raised behind the last of them: an equal
+//    maximum that comes later is behind.
 // 4. Rank: the logits of the listed groups are read again and those that reach the bound sorted.
+//
+// What bounds it: for many long rows the stream (4096 x 131072 bf16, k = 64: 229 us, 4.7 TB/s; with the search left
+// out 167 us would be the rate of a copy). The log-sum-exp costs an exponential per logit and about a tenth of that
+// time; steps 2 to 4 are 17,000 of a block's 44,000 cycles, which the other two blocks of an SM hide in part. Four
+// blocks of 64 registers were slower (261 us: they spill). Few or short rows are bound by the chain of barriers: 15
+// us for one row.
 //
 // A row with more groups than the shared array takes goes through 1 to 3 in segments. A row may also be split over
 // the blocks of a cluster, which share their first bounds and hand their lists to the first block.
@@ -40,7 +46,7 @@ static_assert(kTopFull >= kTopMax, "the list keeps k groups and takes a chunk");
 
 struct TopShared {
   unsigned long long list[kTopList];    // order_pair(largest logit, group); later, of a row in parts, the elements
-  unsigned long long other[kTopList];   // the elements, order_pair(logit, index); of a row in parts first all parts' lists
+  unsigned long long other[kTopList];   // the elements, order_pair(logit, index); of a row in parts first all lists
   uint4 maxima[kTopSegmentBytes / 16];  // the segment's groups: their maxima in the type of the logits
   unsigned int bins[kSearchBins];
   unsigned int range[2];
@@ -205,9 +211,10 @@ __device__ __forceinline__ unsigned long long add_exponentials(unsigned long lon
   return sum2;
 }
 
-// A key that at least k of the block's keys reach, and (unless many are equal) at most k + slack. least / most: over this
-// thread's keys; each(f): f(key) for this thread's keys, 0 for one that does not exist. 0 when there are fewer than k.
-// A histogram of 256 bins over the range of the keys; where the bin in question holds too many, one over that bin.
+// A key that at least k of the block's keys reach, and (unless many are equal) at most k + slack. least / most: over
+// this thread's keys; each(f): f(key) for this thread's keys, 0 for one that does not exist. 0 when there are fewer
+// than k. A histogram of 256 bins over the range of the keys; where the bin in question holds too many, one over that
+// bin.
 template <typename Each>
 __device__ __forceinline__ uint32_t bound_for(TopShared& s, int k, int slack, uint32_t least, uint32_t most, Each each) {
   const int lane = int(threadIdx.x & 31);
@@ -290,7 +297,8 @@ __device__ __forceinline__ void filter_list(unsigned long long* list, unsigned i
 
 // Leaves at least the k first entries of a list, and at most `most_left` (k <= most_left) of them. Returns a key that
 // all of them reach; what comes behind them in the order has a smaller one, or the same.
-__device__ __noinline__ uint32_t cut_list(TopShared& s, unsigned long long* list, unsigned int& count, int k, int most_left) {
+__device__ __noinline__ uint32_t cut_list(TopShared& s, unsigned long long* list, unsigned int& count, int k,
+                                          int most_left) {
   __syncthreads();
   const int n = int(count);
   uint32_t least = 0xffffffffu, most = 0;
@@ -478,8 +486,8 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
     }
     __syncthreads();
     // The first bound. A row in parts needs k groups from all of them: each part finds a share of k among its first
-    // segment, and the lowest of the parts' bounds is one that k groups reach. Where one part lies far above the others its
-    // list runs full and is cut.
+    // segment, and the lowest of the parts' bounds is one that k groups reach. Where one part lies far above the
+    // others its list runs full and is cut.
     if (parts == 1 || seg == v0) {
       const int want = (k + parts - 1) / parts;
       uint32_t from;
@@ -507,8 +515,8 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
   __syncthreads();
 }
 
-// The list that has the row's k first groups among its entries, and their number; of a row in parts in the first block, the others
-// return with 0. `free_list`: room for the elements.
+// The list that has the row's k first groups among its entries, and their number; of a row in parts in the first
+// block, the others return with 0. `free_list`: room for the elements.
 struct TopGroups {
   unsigned long long* list;
   unsigned long long* free_list;
@@ -547,8 +555,8 @@ __device__ __noinline__ void rank_list(TopShared& s, unsigned long long* list, u
     __syncthreads();
     return;
   }
-  // Entries go to 256 bins over the range of the keys; an entry's place is the number of those in bins ahead and of those of its own bin
-  // ahead of it, of which there are few.
+  // Entries go to 256 bins over the range of the keys; an entry's place is the number of those in bins ahead and of
+  // those of its own bin ahead of it, of which there are few.
   if (threadIdx.x == 0) {
     s.range[0] = 0xffffffffu;
     s.range[1] = 0;
@@ -602,8 +610,8 @@ __device__ __noinline__ void rank_list(TopShared& s, unsigned long long* list, u
   __syncthreads();
 }
 
-// The listed groups' logits again: the k first logits of the row (all of them if there are fewer), sorted, in g.free_list;
-// returns how many.
+// The listed groups' logits again: the k first logits of the row (all of them if there are fewer), sorted, in
+// g.free_list; returns how many.
 template <Nan kNan, typename T>
 __device__ __forceinline__ int rank_elements(TopShared& s, const RowGroups<T>& row, const TopGroups& g, int k) {
   constexpr int kPer = RowGroups<T>::kPer, kPart = kPer / 4;  // logits of a thread: a quarter of a group

@@ -96,9 +96,9 @@ __device__ __forceinline__ T block_prefix(T v, T* scratch /*[32]*/, T* total) {
   return before + inc - v;
 }
 
-// Sorts kThreads * kEach numbers in shared memory, largest first (a bitonic network). Thread t holds the places t * kEach ..:
-// strides below kEach stay in its registers, strides below 32 * kEach go through shuffles, and only the few longer ones
-// through shared memory. (All 55 steps of 1024 numbers through shared memory took 21,000 cycles.)
+// Sorts kThreads * kEach numbers in shared memory, largest first (a bitonic network). Thread t holds the places t *
+// kEach ..: strides below kEach stay in its registers, strides below 32 * kEach go through shuffles, and only the few
+// longer ones through shared memory. (All 55 steps of 1024 numbers through shared memory took 21,000 cycles.)
 template <int kThreads, int kEach>
 __device__ __forceinline__ void block_sort_each(unsigned long long* a) {
   unsigned long long v[kEach];
