@@ -160,6 +160,7 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
         if (head)
           for (int m = k; m < padded && uint32_t(mine[m] >> 32) == col; ++m) q += __uint_as_float(uint32_t(mine[m]));
         const uint32_t heads = __ballot_sync(0xffffffffu, head);
+        __syncwarp();  // all have read what the places below are about to hold
         const int at = length + __popc(heads & ((1u << lane) - 1u));
         if (head) {
           mine[at] = ((unsigned long long)col << 32) | __float_as_uint(q);

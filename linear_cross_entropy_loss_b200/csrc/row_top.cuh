@@ -61,6 +61,12 @@ struct TopShared {
   float part_ref[kTopParts], part_sum[kTopParts];  // log-sum-exp of a part
 };
 
+// A block may write into another's shared memory only once that one runs: each block of a cluster says so as it starts
+// (cluster_started) and waits for the others where it first writes (cluster_wait_started), by when they long have.
+// Whole warps, every thread of the block.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;"); }
+__device__ __forceinline__ void cluster_wait_started() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 struct Group {
   uint32_t w[8];
 };
@@ -422,6 +428,7 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
   constexpr int kSegment = kTopSegmentBytes / int(sizeof(T));  // groups
   static_assert(kSegment % kTopChunk == 0 && kSegment % (2 * kTopBatch) == 0, "segments are whole chunks");
   const T* tag = nullptr;
+  if (parts > 1) cluster_started();
   const int limit = min(2 * k + 64, kTopFull);
   T* const maxima = reinterpret_cast<T*>(s.maxima);
   __syncthreads();
@@ -503,6 +510,7 @@ __device__ __forceinline__ void stream_top(TopShared& s, const RowGroups<T>& row
       }
       if (parts > 1) {  // every part comes here once: it has groups
         cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        cluster_wait_started();
         if (int(threadIdx.x) < parts) cluster.map_shared_rank(&s, threadIdx.x)->part_bound[cluster.block_rank()] = from;
         cluster.sync();
         for (int part = 0; part < parts; ++part) from = min(from, s.part_bound[part]);

@@ -680,6 +680,7 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const long long r = blockIdx.x / parts;
   const RowSettings set = row_settings(p, r);
   if (by_list(p, set)) return;  // the whole cluster
+  cluster_started();
   RowCluster c{cooperative_groups::this_cluster(), int(blockIdx.x % parts), parts, s};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPer = RowStretch<T>::kPer;
@@ -717,6 +718,7 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   // ---- the largest logit
   float top = x.largest();  // passes NaN over
   top = block_max(top, s.reduce_f);
+  cluster_wait_started();
   if (int(threadIdx.x) < parts) c.of(threadIdx.x).part_max[c.rank] = top;
   c.group.sync();
   for (int part = 0; part < parts; ++part) top = fmaxf(top, s.part_max[part]);
@@ -754,6 +756,7 @@ sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     auto all = [&](uint32_t, float l) { return l >= weighty; };
     const Crossing at = find_bin(c, x, one, bin, all, [&](unsigned long long total) { return total < k ? total : k; });
     if (at.total > k) cut = find_place(c, x, at.before, k, one, logits_of(at.bin), cut);
+    else c.group.sync();  // the others may still read the bins, which the next cut overwrites
   }
   if (set.top_p < 1.0) {
     const RowCut outer = cut;

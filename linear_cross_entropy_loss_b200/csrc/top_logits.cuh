@@ -46,6 +46,9 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
     const double put_back = largest * (double(inv_temperature) - double(log2_scale) * kLn2);
     float v = float((double(top) + double(log2f(total))) * kLn2 + put_back);
     if (first >= kKeyPosInf || first == kKeyNegInf) v = key_to_float(first);  // +inf, NaN; nothing but -inf
+    // From 2^30 on a float's steps are 64 and more, and the others (at most 2^30, log 21) do not move it. The sum is of no
+    // use there: its terms are off by the rounding of the reference, which is an exponent of 2^6 and more.
+    else if (fabs(largest * double(inv_temperature)) >= 1073741824.0) v = float(largest * double(inv_temperature));
     lse[r] = v;
   }
 }

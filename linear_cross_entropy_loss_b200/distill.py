@@ -91,7 +91,7 @@ def _operands(x, At):
 
 def _aligned(m):
     """m, or a copy of it whose rows start on 16-byte boundaries."""
-    if _tma_ready(m):
+    if _tma_ready(m) and m.stride(0) >= m.shape[1]:  # (an expanded row has stride 0)
         return m
     copy = _aligned_rows_like(m.shape, m.dtype, m.device)
     if m.stride(1) == 1:
@@ -164,7 +164,8 @@ def linear_distillation(
     that of the cross-entropy). NaN or +inf in an entry that is there make the loss NaN. An index that is listed twice
     counts twice.
 
-    Gradients for x and At only (those that are wanted are computed during the forward pass; no second derivatives);
+    Gradients for x and At only (those that are wanted are computed during the forward pass; no second derivatives; a step
+    may be captured into a graph under torch's own rule, that no autograd graph of the same leaves from outside is alive);
     under CUDA autocast x and At are cast as :func:`set_autocast_policy` says.
     """
     assert x.dim() >= 1 and At.dim() == 2 and At.shape[0] == x.shape[-1], "x and the weight disagree on the hidden size"
@@ -224,7 +225,7 @@ def distillation_op(x: torch.Tensor, At: torch.Tensor, t: torch.Tensor, idx: tor
         xd, Ad = xd.requires_grad_(), Ad.requires_grad_()
         loss = linear_distillation(xd, t, idx, Ad, lse, temperature, logit_scale, N_chunk_size)
     dx, dA = loss.grad_fn.lce_grads
-    return loss.detach(), dx.reshape(x.shape), dA
+    return loss.detach(), dx.reshape(x.shape).contiguous(), dA.contiguous()
 
 
 @distillation_op.register_fake

@@ -72,7 +72,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
 
 
 def _head_operands(x: torch.Tensor, At: torch.Tensor):
-    """x as (rows, H) and At, as the kernels read them."""
+    """x as (rows, H) and At, as the kernels read them (while a compiler traces: as linear_logits_op takes them)."""
     from .distill import _operands
     from .ops import _autocast_target
 
@@ -85,8 +85,10 @@ def _head_operands(x: torch.Tensor, At: torch.Tensor):
         x, At = x.to(target), At.to(target)
     assert x.dtype == At.dtype, "x and the weight must have the same dtype"
     assert x.dtype in _DTYPE_CODE, f"unsupported dtype {x.dtype}"
-    _require_cuda(get_backend(), x)
     x = x.reshape(-1, x.shape[-1])
+    if torch.compiler.is_compiling():
+        return x, At
+    _require_cuda(get_backend(), x)
     if x.shape[0] == 0:
         return x, At
     with _device_guard(x):
@@ -95,6 +97,8 @@ def _head_operands(x: torch.Tensor, At: torch.Tensor):
 
 def _logit_rows(x, At, scale: float) -> torch.Tensor:
     """(rows, V) float32 logits, rows on 16-byte boundaries."""
+    if torch.compiler.is_compiling():
+        return linear_logits_op(x, At, float(scale))
     V = At.shape[1]
     out = torch.empty((x.shape[0], -(-V // 4) * 4), dtype=torch.float32, device=x.device)
     if x.shape[0] > 0:
@@ -156,8 +160,8 @@ def _setting(value, name: str, dtype, n: int, device):
     assert value.numel() in (1, n), f"{name} must be a number or have one entry per row"
     assert value.device == device, f"{name} must be on the device of the logits"
     if dtype == torch.int32 and value.dtype != torch.int32:
-        assert not value.is_floating_point(), f"{name} must hold whole numbers"
-        value = value.clamp(0, 2**31 - 1)
+        assert not value.is_floating_point() and not value.is_complex(), f"{name} must hold whole numbers"
+        value = value.to(torch.int64).clamp(0, 2**31 - 1)
     if value.dtype == dtype and value.dim() == 1 and value.shape[0] == n and value.is_contiguous():
         return None, value
     return None, value.detach().reshape(-1).to(dtype).expand(n).contiguous()
@@ -236,6 +240,17 @@ def _top_logits_fake(logits, k, temperature):
     lead = logits.shape[:-1]
     return (logits.new_empty((*lead, k)), logits.new_empty((*lead, k), dtype=torch.int64),
             logits.new_empty(lead, dtype=torch.float32))
+
+
+@torch.library.custom_op("lce_b200::linear_logits", mutates_args=())
+def linear_logits_op(x: torch.Tensor, At: torch.Tensor, logit_scale: float) -> torch.Tensor:
+    """x: (rows, H)."""
+    return linear_logits(x, At, logit_scale).contiguous()
+
+
+@linear_logits_op.register_fake
+def _linear_logits_fake(x, At, logit_scale):
+    return x.new_empty((x.shape[0], At.shape[1]), dtype=torch.float32)
 
 
 @torch.library.custom_op("lce_b200::sample_logits", mutates_args=())

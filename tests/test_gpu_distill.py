@@ -355,6 +355,70 @@ def test_traced_by_torch_compile_without_a_graph_break():
     assert torch.equal(xd.grad, 2 * want[1]) and torch.equal(Ad.grad, 2 * want[2])
 
 
+def test_a_head_traced_by_torch_compile_without_a_graph_break():
+    head = LinearCrossEntropyLoss(64, 1001, device="cuda", dtype=torch.bfloat16, N_chunk_size=50)
+    h, u = torch.randn(4, 30, 64, device="cuda", dtype=torch.bfloat16), torch.rand(4, 30, device="cuda")
+    call = lambda h, u: (head.logits(h), *head.top_logits(h, 5), *head.sample(h, u, top_p=0.9))  # noqa: E731
+    got = torch.compile(call, fullgraph=True, backend="aot_eager")(h, u)
+    want = call(h, u)
+    assert all(a.shape == b.shape and a.dtype == b.dtype for a, b in zip(got, want))
+    # rows of the traced logits lie 1001 elements apart, not 1004, so their exponentials are added up in another order: at
+    # most 64 one after the other, in both
+    lse = got[3], want[3]
+    assert ((lse[0] - lse[1]).abs() <= 2 * (64 + lse[0].abs()) * 2.0**-24).all()
+    assert all(torch.equal(a, b) for i, (a, b) in enumerate(zip(got, want)) if i != 3)
+
+
+def test_traced_operators_are_what_their_shapes_promise():
+    """Sizes and strides of the outputs, at a vocabulary whose rows are padded inside."""
+    x, At, t, idx = (v.cuda() for v in problem(40, 60, 701, 6, torch.bfloat16, seed=26))
+    ops, utils = torch.ops.lce_b200, ("test_schema", "test_faketensor")
+    lse, u = torch.logsumexp(t.float(), 1), torch.rand(40, device="cuda")
+    ks = torch.full((40,), 9, device="cuda")
+    torch.library.opcheck(ops.distillation.default, (x, At, t, idx, lse, 2.0, 1.0, 128, True), test_utils=utils)
+    torch.library.opcheck(ops.distillation.default, (x, At, t, idx, None, 2.0, 1.0, 4096, False), test_utils=utils)
+    torch.library.opcheck(ops.linear_logits.default, (x, At, 1.0), test_utils=utils)
+    logits = linear_logits(x, At).view(4, 10, 701)
+    torch.library.opcheck(ops.top_logits.default, (logits, 5, 1.0), test_utils=utils)
+    torch.library.opcheck(ops.sample_logits.default, (logits, u.view(4, 10), None, ks, None, None, 1.0, 0, 0.9, 0.0),
+                          test_utils=utils)
+
+
+def test_broadcast_inputs_and_lists():
+    """One row of x and one list for all rows: the gradient is the sum, the loss that of one row."""
+    x, At, t, idx = problem(1, 64, 700, 6, torch.float32, seed=27)
+    one = run(x, At, t, idx)
+    xd, Ad = x.cuda().requires_grad_(), At.cuda().requires_grad_()
+    loss = linear_distillation(xd.expand(40, 64), t.cuda().expand(40, 6), idx.cuda().expand(40, 6), Ad)
+    loss.backward()
+    assert abs(loss.item() - one[0]) <= 1e-6 * abs(one[0])
+    for got, want in ((xd.grad, one[1]), (Ad.grad, one[2])):  # each within the 6e-3 of check() from the formula
+        assert (got - want).norm() <= 1.2e-2 * want.norm()
+
+
+def test_given_log_sum_exp_of_rows_without_a_list():
+    """What a teacher's log-sum-exp is where its list is empty does not matter, and -inf lists with -inf neither."""
+    x, At, t, idx = problem(50, 64, 700, 6, torch.bfloat16, seed=28)
+    lse = torch.logsumexp(t.double(), 1).float() + 0.3
+    idx[3], idx[4] = -1, 700
+    t[5] = -math.inf
+    want = run(x, At, t, idx, lse=lse)
+    lse[3], lse[4], lse[5] = math.nan, math.inf, -math.inf
+    got = run(x, At, t, idx, lse=lse)
+    assert math.isfinite(got[0]) and got[0] == want[0] and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+def test_lists_further_apart_than_31_bits():
+    x, At, t, idx = problem(2, 64, 700, 6, torch.bfloat16, seed=29)
+    far = torch.zeros(2**31 + 100, dtype=torch.bfloat16, device="cuda").as_strided((2, 6), (2**31 + 5, 1), 3)
+    far.copy_(t)
+    want, got = run(x, At, far.cpu(), idx), None
+    xd, Ad = x.cuda().requires_grad_(), At.cuda().requires_grad_()
+    got = linear_distillation(xd, far, idx.cuda(), Ad)
+    got.backward()
+    assert got.item() == want[0] and torch.equal(xd.grad, want[1]) and torch.equal(Ad.grad, want[2])
+
+
 def test_second_derivatives_are_refused():
     x, At, t, idx = problem(16, 64, 300, 4, torch.bfloat16)
     xd = x.cuda().requires_grad_()

@@ -350,3 +350,70 @@ def test_traced_by_torch_compile_without_a_graph_break(what):
         call = lambda x, v: tuple(sample_logits(x + 0, v, temperature=T, top_k=20, top_p=0.9))  # noqa: E731
     got = torch.compile(call, fullgraph=True, backend="aot_eager")(logits, u)
     assert all(torch.equal(a, b) for a, b in zip(got, call(logits, u)))
+
+
+def test_rows_further_apart_than_31_bits():
+    flat = torch.full((2**31 + 9000,), -INF, dtype=torch.float16, device="cuda")
+    rows = flat.as_strided((2, 5003), (2**31 + 5, 1), 3)
+    rows.copy_(normal(2, 5003, torch.float16, seed=8))
+    check_top(rows, 33)
+    for settings in (dict(), dict(top_k=30), dict(top_p=0.8)):
+        check_sample(rows, uniform(2), **settings)
+
+
+@pytest.mark.parametrize("T", [2.0**-126, 2.0**-123, 1e-30, 1e-12, 1e-9, 3e-8, 1e-6, 1e-3, 1e30])
+def test_log_sum_exp_at_any_temperature(T):
+    """Up to quotients that a float does not hold."""
+    rows = normal(3, 3000, torch.float32, seed=3).abs() + 1
+    rows[1] = -rows[1]
+    rows[2, 5] = 0.0
+    got = top_logits(rows.cuda(), 4, temperature=T).lse.cpu()
+    T = float(torch.tensor(T, dtype=torch.float32))
+    want = torch.logsumexp(rows.double() / T, 1)
+    # the rounding of 1 / T and of the result, of the sum's 3000 terms (at most 64 of them one after the other)
+    bound = want.abs() * 2.0**-23 + 68 * 2.0**-24
+    big = want.abs() > torch.finfo(torch.float32).max
+    assert torch.equal(got[big], want[big].float())
+    assert ((got.double() - want).abs()[~big] <= bound[~big]).all(), (got, want)
+
+
+def test_few_with_weight_before_a_second_cut_in_a_cluster():
+    """top_k keeps all that have weight, and top_p follows at once: the blocks of a row share the same arrays for both."""
+    logits = torch.full((40, 131072), -1e4)
+    logits[:, ::1000] = normal(40, 132, torch.float32, seed=4)
+    for _ in range(20):
+        check_sample(logits.cuda(), uniform(40), top_k=2000, top_p=0.6)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int64, torch.bool])
+def test_top_k_per_row_in_any_whole_type(dtype):
+    logits, u = normal(5, 700, torch.float32, seed=5).cuda(), uniform(5)
+    ks = torch.tensor([0, 1, 1, 0, 1]).to(dtype).cuda()
+    want = sample_logits(logits, u, top_k=ks.to(torch.int32))
+    got = sample_logits(logits, u, top_k=ks)
+    assert torch.equal(got.tokens, want.tokens) and torch.equal(got.logprobs, want.logprobs)
+
+
+def test_two_threads():
+    import threading
+
+    jobs = [(normal(64, 20000 + 64 * i, torch.bfloat16, seed=i).cuda(), uniform(64, i)) for i in range(4)]
+    want = [(top_logits(x, 20), sample_logits(x, u, top_p=0.9)) for x, u in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                x, u = jobs[i]
+                got = (top_logits(x, 20), sample_logits(x, u, top_p=0.9))
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for g, w in zip(got, want[i]) for a, b in zip(g, w)):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
