@@ -256,42 +256,55 @@ distill_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ x
 // Per-tile mode (see dz_transform_kernel): slab = boost * (Q softmax - q), in place. boost: a power of two that the
 // contractions divide by again. |dZ| <= 1 before it is scaled, so fp16 has room for 2^14, without which a softmax entry
 // of 1 / V is a subnormal number.
+// grid: x over groups of kDzTiles tiles, y over groups of 8 rows. A warp takes the tiles of a row, all their loads on the way before the first is used.
+constexpr int kDzTiles = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
 distill_dz_kernel(T* __restrict__ slab, long long slab_ld, const float* __restrict__ tile_max,
                   const float* __restrict__ lse, const float* __restrict__ mass, const TeacherRows t, int rows,
                   int rows_valid, int n_tiles, long long stat_ld, float boost) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long items = (long long)(rows / 8) * n_tiles;
-  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const int tile = (int)(item % n_tiles);
-    const int r = (int)(item / n_tiles) * 8 + warp;
+  const int tile0 = blockIdx.x * kDzTiles;
+  for (int r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
     const bool exists = r < rows_valid;
+    T* const ptr = slab + (long long)r * slab_ld + (long long)tile0 * 256 + lane * 8;
+    Vec8<T> v[kDzTiles];
+    float most[kDzTiles];
+    int start[kDzTiles + 1];
+#pragma unroll
+    for (int i = 0; i < kDzTiles; ++i)
+      if (tile0 + i < n_tiles) v[i].load(ptr + i * 256);
     const float Q = exists ? mass[r] : 0.f;
     const float l = exists ? lse[r] : 0.f;
-    const float coef = Q != 0.f ? Q * __expf(tile_max[(long long)tile * stat_ld + r] - l) * boost : 0.f;
-    T* ptr = slab + (long long)r * slab_ld + (long long)tile * 256 + lane * 8;
-    Vec8<T> v;
-    v.load(ptr);
-    float f[8];
-    v.to_float(f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= coef;
-    if (Q != 0.f) {
-      const int end = t.start[(long long)(tile + 1) * t.start_ld + r];
-      for (int k = t.start[(long long)tile * t.start_ld + r]; k < end; ++k) {
-        const long long at = (long long)r * t.k + k;
-        const int c = t.idx[at] - tile * 256;
-        if ((c >> 3) == lane) {
-          const float dz = listed_dz(t.z[at], l, Q, t.q[at]) * boost;
+    for (int i = 0; i < kDzTiles; ++i)
+      most[i] = exists && tile0 + i < n_tiles ? tile_max[(long long)(tile0 + i) * stat_ld + r] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i == (c & 7)) f[i] = dz;
+    for (int i = 0; i <= kDzTiles; ++i)
+      start[i] = exists ? t.start[(long long)min(tile0 + i, n_tiles) * t.start_ld + r] : 0;
+#pragma unroll
+    for (int i = 0; i < kDzTiles; ++i) {
+      if (tile0 + i >= n_tiles) break;
+      const float coef = Q != 0.f ? Q * __expf(most[i] - l) * boost : 0.f;
+      float f[8];
+      v[i].to_float(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= coef;
+      if (Q != 0.f) {
+        for (int k = start[i]; k < start[i + 1]; ++k) {
+          const long long at = (long long)r * t.k + k;
+          const int c = t.idx[at] - (tile0 + i) * 256;
+          if ((c >> 3) == lane) {
+            const float dz = listed_dz(t.z[at], l, Q, t.q[at]) * boost;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j == (c & 7)) f[j] = dz;
+          }
         }
       }
+      v[i].from_float(f);
+      v[i].store(ptr + i * 256);
     }
-    v.from_float(f);
-    v.store(ptr);
   }
 }
 

@@ -1452,7 +1452,8 @@ void launch_distill_dz(const lce_problem* p, const DistillWorkspace& w, const Di
       return;
     }
   }
-  distill_dz_kernel<T><<<grid_for((rows_pad / 8) * n_vtiles, 1, sms, 16), 256, 0, st>>>(
+  const dim3 grid((n_vtiles + kDzTiles - 1) / kDzTiles, (unsigned)std::min<long long>(rows_pad / 8, 65535));
+  distill_dz_kernel<T><<<grid, 256, 0, st>>>(
       slab, v_pad, w.pass.tile_max, w.pass.lse, d.lists.mass, d.lists, (int)rows_pad, (int)rows, n_vtiles,
       p->chunk_rows, d.boost);
 }
