@@ -133,14 +133,29 @@ struct TeacherRows {
 // each; dots is complete after the caller's next __syncthreads).
 __device__ __forceinline__ void listed_dots(const TeacherRows& t, int r0, int rows, float* dots /*[32]*/) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = 4 * warp; i < 4 * warp + 4; ++i) {
-    const int r = r0 + i;
-    if (r >= rows) break;
-    const int n = t.start[(long long)t.n_tiles * t.start_ld + r];
-    float d = 0.f;
-    for (int e = lane; e < n; e += 32) d = fmaf(t.q[(long long)r * t.k + e], t.z[(long long)r * t.k + e], d);
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) dots[i] = d - t.plogp[r];
+  // the four rows side by side: their loads wait for one another only along a row
+  int n[4], longest = 0;
+  float plogp[4], d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + 4 * warp + i;
+    n[i] = r < rows ? t.start[(long long)t.n_tiles * t.start_ld + r] : 0;
+    plogp[i] = r < rows ? t.plogp[r] : 0.f;
+    d[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) longest = max(longest, n[i]);
+  for (int e = lane; e < longest; e += 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long at = (long long)(r0 + 4 * warp + i) * t.k + e;
+      if (e < n[i]) d[i] = fmaf(t.q[at], t.z[at], d[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    for (int o = 16; o > 0; o >>= 1) d[i] += __shfl_xor_sync(0xffffffffu, d[i], o);
+    if (lane == 0) dots[4 * warp + i] = d[i] - plogp[i];
   }
 }
 
@@ -167,12 +182,25 @@ row_stats_kernel(const float* __restrict__ tile_max, const float* __restrict__ t
   const int r = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f, u = 0.f, q = 0.f;
   if (r < rows) {
-    for (int t = warp; t < n_tiles; t += 8) {
-      const long long i = (long long)t * stat_ld + r;
-      const float mt = tile_max[i], st = tile_sum[i];
-      const float ut = kMonitor ? tile_ez[i] : 0.f;
-      if (kMonitor) q += tile_sq[i];
-      lse_merge(m, s, u, mt, st, ut);
+    constexpr int kAhead = 4;  // tiles loaded before they are merged, in the same order
+    for (int t0 = warp; t0 < n_tiles; t0 += 8 * kAhead) {
+      float mt[kAhead], st[kAhead], ut[kAhead], qt[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int t = t0 + 8 * j;
+        const long long i = (long long)t * stat_ld + r;
+        const bool is = t < n_tiles;
+        mt[j] = is ? tile_max[i] : 0.f;
+        st[j] = is ? tile_sum[i] : 0.f;
+        ut[j] = kMonitor && is ? tile_ez[i] : 0.f;
+        qt[j] = kMonitor && is ? tile_sq[i] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (t0 + 8 * j >= n_tiles) break;
+        if (kMonitor) q += qt[j];
+        lse_merge(m, s, u, mt[j], st[j], ut[j]);
+      }
     }
   }
   sm[warp][0][lane] = m;
