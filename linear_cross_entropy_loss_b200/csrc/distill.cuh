@@ -255,8 +255,9 @@ distill_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ x
 
 // Per-tile mode (see dz_transform_kernel): slab = boost * (Q softmax - q), in place. boost: a power of two that the
 // contractions divide by again. |dZ| <= 1 before it is scaled, so fp16 has room for 2^14, without which a softmax entry
-// of 1 / V is a subnormal number.
-// grid: x over groups of kDzTiles tiles, y over groups of 8 rows. A warp takes the tiles of a row, all their loads on the way before the first is used.
+// of 1 / V is a subnormal number. It reads and writes the slab once: 1000 x 50257 in fp16 31 us, 6.6 TB/s.
+// grid: x over groups of kDzTiles tiles, y over groups of 8 rows. A warp takes the tiles of a row, all their loads on the
+// way before the first is used. (One tile at a time, its place from 64-bit divisions: 58 us.)
 constexpr int kDzTiles = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)

@@ -49,22 +49,30 @@ int allow_smem(size_t bytes) {
   return LCE_OK;
 }
 
-// One launch of `blocks` blocks in clusters of `parts`.
+// One launch of `blocks` blocks in clusters of `parts`. `beside`: it may start once all blocks of the launch before it
+// have started.
 template <typename... Args, typename... Given>
-int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size_t smem, int parts, cudaStream_t st,
-                    Given... given) {
+int launch_clusters(void (*kernel)(Args...), long long blocks, int threads, size_t smem, int parts, bool beside,
+                    cudaStream_t st, Given... given) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)blocks);
   config.blockDim = dim3((unsigned)threads);
   config.dynamicSmemBytes = smem;
   config.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)parts;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  config.attrs = &attr;
-  config.numAttrs = parts > 1 ? 1 : 0;
+  cudaLaunchAttribute attrs[2];
+  config.attrs = attrs;
+  if (parts > 1) {
+    cudaLaunchAttribute& attr = attrs[config.numAttrs++];
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)parts;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+  }
+  if (beside) {
+    cudaLaunchAttribute& attr = attrs[config.numAttrs++];
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+  }
   if (cudaLaunchKernelEx(&config, kernel, Args(given)...) != cudaSuccess) {
     cudaGetLastError();
     return LCE_ERR_CUDA;
@@ -89,7 +97,7 @@ int launch_top(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
   const int parts = top_parts<T>(rows, vocab, k);
   const int v = allow_smem<&top_logits_kernel<T>>(sizeof(TopShared));
   if (v != LCE_OK) return v;
-  return launch_clusters(top_logits_kernel<T>, rows * parts, kTopThreads, sizeof(TopShared), parts, st,
+  return launch_clusters(top_logits_kernel<T>, rows * parts, kTopThreads, sizeof(TopShared), parts, false, st,
                          reinterpret_cast<const T*>(logits), (long long)ld, (uint32_t)vocab, k, parts, inv_t,
                          reinterpret_cast<T*>(values), reinterpret_cast<long long*>(indices), lse);
 }
@@ -118,7 +126,7 @@ int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, 
   p.weight_bits = kWeightBits;  // the sum over the row stays below 2^62
   while (vocab > (1ll << (62 - p.weight_bits))) --p.weight_bits;
   // top_k for all rows: one of the two kernels has them all, but for greedy rows, which the list has. A top_k for
-  // each row: both run, and a cluster whose row is the other's ends at once.
+  // each row: both run, side by side, and a cluster whose row is the other's ends at once.
   const bool each = p.top_k != nullptr;
   const int want = each ? 256 : (int)std::min<long long>(std::max<long long>(p.top_k_all, 1), kTopMax);
   const int list_parts = top_parts<T>(rows, vocab, want);
@@ -130,8 +138,8 @@ int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, 
   int v;
   if (lists) {
     if ((v = allow_smem<&sample_list_kernel<T>>(sizeof(TopShared))) != LCE_OK) return v;
-    if ((v = launch_clusters(sample_list_kernel<T>, rows * list_parts, kTopThreads, sizeof(TopShared), list_parts, st,
-                             logits, (long long)ld, (uint32_t)vocab, list_parts, p, tokens, logprobs)) != LCE_OK)
+    if ((v = launch_clusters(sample_list_kernel<T>, rows * list_parts, kTopThreads, sizeof(TopShared), list_parts, false,
+                             st, logits, (long long)ld, (uint32_t)vocab, list_parts, p, tokens, logprobs)) != LCE_OK)
       return v;
   }
   if (!others) return LCE_OK;
@@ -139,8 +147,8 @@ int launch_sample(const void* logits_, int64_t ld, int64_t rows, int64_t vocab, 
   row_layout(rows, vocab, (int)sizeof(T), &parts, &cache);
   const size_t fixed = (sizeof(RowShared) + 15) / 16 * 16;
   if ((v = allow_smem<&sample_row_kernel<T>>(fixed + kRowCacheMax)) != LCE_OK) return v;
-  return launch_clusters(sample_row_kernel<T>, rows * parts, kRowThreads, fixed + (size_t)cache * 16, parts, st, logits,
-                         (long long)ld, (uint32_t)vocab, parts, cache, p, tokens, logprobs);
+  return launch_clusters(sample_row_kernel<T>, rows * parts, kRowThreads, fixed + (size_t)cache * 16, parts, lists, st,
+                         logits, (long long)ld, (uint32_t)vocab, parts, cache, p, tokens, logprobs);
 }
 
 }  // namespace

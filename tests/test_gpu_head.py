@@ -417,3 +417,34 @@ def test_two_threads():
     for t in threads:
         t.join()
     assert wrong == []
+
+
+@pytest.mark.parametrize("k_list", [1, 40, 200])
+def test_what_follows_both_kernels_waits_for_both(k_list):
+    """Settings per row: two kernels side by side. All rows, or none, or half of them have a short list; what reads the
+    answers next in the stream has to find all of them."""
+    n, V = 30, 70001
+    logits = normal(n, V, torch.bfloat16, seed=k_list).cuda()
+    for share in (0, 1, 2):
+        ks = torch.full((n,), k_list)
+        if share != 0:
+            ks[::share] = 5000
+        ks = ks.cuda()
+        want = [sample_logits(logits, uniform(n, i), top_k=ks, top_p=0.9) for i in range(8)]
+        torch.cuda.synchronize()
+        tokens, logprobs = torch.zeros(8, n, dtype=torch.int64, device="cuda"), torch.zeros(8, n, device="cuda")
+        us = [uniform(n, i) for i in range(8)]
+        static, graph = us[0].clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = sample_logits(logits, static, top_k=ks, top_p=0.9)
+            copy = got.tokens.clone(), got.logprobs.clone()
+        for i in range(8):
+            got = sample_logits(logits, us[i], top_k=ks, top_p=0.9)
+            tokens[i], logprobs[i] = got.tokens, got.logprobs
+            del got
+            torch.full((n,), -7, device="cuda")  # may take the place of the answers
+        for i in range(8):
+            assert torch.equal(tokens[i], want[i].tokens) and torch.equal(logprobs[i], want[i].logprobs)
+            static.copy_(us[i])
+            graph.replay()
+            assert torch.equal(copy[0], want[i].tokens) and torch.equal(copy[1], want[i].logprobs)
