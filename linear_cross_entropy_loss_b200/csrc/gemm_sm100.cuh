@@ -94,6 +94,8 @@ struct GemmParams {
   void* out_sum;
   void* out_res;
   long long out_pair_ld;       // elements between rows of out_sum and of out_res
+  float out_res_scale;         // fp16: out_res holds the residual times this power of two (2^11 keeps it below out_sum and
+                               // out of the subnormal numbers, whose step of 2^-24 every launch would round to again)
   int out_pair_last;           // 1: last launch of the accumulation
   int out_rows;                // rows / columns of the output that exist; tiles may hang over both edges
   int out_cols;
@@ -597,6 +599,7 @@ __device__ __forceinline__ void epilogue_f32(const GemmParams& p, const CUtensor
   Elem* dst_sum = reinterpret_cast<Elem*>(p.out_sum) + row * p.out_pair_ld + (long long)n_blk * BLOCK_N;
   Elem* dst_res = reinterpret_cast<Elem*>(p.out_res) + row * p.out_pair_ld + (long long)n_blk * BLOCK_N;
   const bool write_res = pair && p.out_res != nullptr && !p.out_pair_last;
+  const float unscale = kKind == KIND_F16 && pair ? 1.f / p.out_res_scale : 1.f;
   float coef = (p.out_div != nullptr) ? p.out_scale / __ldg(p.out_div) : p.out_scale;
   if (p.row_coef != nullptr) coef *= p.row_coef[row];  // row_coef covers the padded rows too
 #pragma unroll 1
@@ -664,12 +667,15 @@ __device__ __forceinline__ void epilogue_f32(const GemmParams& p, const CUtensor
         for (int i = 0; i < 32; ++i) r[i] += t[i];
         load_elems32(dst_res + c * 32, t);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] += t[i];
+        for (int i = 0; i < 32; ++i) r[i] += kKind == KIND_F16 ? t[i] * unscale : t[i];
       }
       store_slab_chunk(dst_sum + c * 32, r);
       if (write_res) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] -= elem_to_float<Elem>(cast_elem<Elem>(r[i]));
+        for (int i = 0; i < 32; ++i) {
+          r[i] -= elem_to_float<Elem>(cast_elem<Elem>(r[i]));
+          if (kKind == KIND_F16) r[i] *= p.out_res_scale;
+        }
         store_slab_chunk(dst_res + c * 32, r);
       }
     } else if (pair) {
@@ -678,10 +684,16 @@ __device__ __forceinline__ void epilogue_f32(const GemmParams& p, const CUtensor
       for (int i = 0; i < 32; ++i) {
         if (i < lim) {
           float val = coef * __uint_as_float(v[i]);
-          if (p.accumulate) val += elem_to_float<Elem>(dst_sum[c * 32 + i]) + elem_to_float<Elem>(dst_res[c * 32 + i]);
+          if (p.accumulate) {
+            const float res = elem_to_float<Elem>(dst_res[c * 32 + i]);
+            val += elem_to_float<Elem>(dst_sum[c * 32 + i]) + (kKind == KIND_F16 ? res * unscale : res);
+          }
           const Elem hi = cast_elem<Elem>(val);
           dst_sum[c * 32 + i] = hi;
-          if (write_res) dst_res[c * 32 + i] = cast_elem<Elem>(val - elem_to_float<Elem>(hi));
+          if (write_res) {
+            const float res = val - elem_to_float<Elem>(hi);
+            dst_res[c * 32 + i] = cast_elem<Elem>(kKind == KIND_F16 ? res * p.out_res_scale : res);
+          }
         }
       }
     } else if (lim >= 32 && p.out_vector_ok) {

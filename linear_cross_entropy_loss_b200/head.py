@@ -187,7 +187,8 @@ def sample_logits(
     which is not: out-of-range entries are taken as the nearest value that means something. -inf and NaN logits are never
     drawn; +inf logits share all the mass. A row without any logit to draw gives token -1 and logprob -inf.
 
-    Weights and sums are kept in 64-bit integers, so the answer for a row depends on its inputs alone.
+    Weights and sums are kept in 64-bit integers (steps of 2^-44 of the largest weight for up to 2^18 columns), so the
+    answer for a row depends on its inputs alone; weights below half a step are none.
     """
     if torch.compiler.is_compiling():
         given = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]

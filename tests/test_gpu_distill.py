@@ -145,6 +145,13 @@ def test_types_and_layouts_of_the_lists():
     check(x, At, half, idx)
 
 
+@pytest.mark.parametrize("N,H,V,K,T,chunk", [(513, 8, 9000, 17, 0.5, 128), (513, 200, 9000, 1, 0.5, 1),
+                                             (300, 64, 9000, 300, 0.5, 256), (700, 70, 9001, 64, 1.0, 128)])
+def test_small_gradients_summed_over_chunks(N, H, V, K, T, chunk):
+    """dW below fp16's normal numbers: every chunk adds to it, only the last may round to a step of 2^-24."""
+    check(*problem(N, H, V, K, torch.float16, seed=N + K), T=T, chunk=chunk)
+
+
 @pytest.mark.parametrize("H,V", [(60, 777), (250, 1001), (64, 1003), (13, 256)])
 def test_sizes_that_need_copies(H, V):
     check(*problem(150, H, V, 11, torch.bfloat16, seed=H), chunk=128)
