@@ -16,8 +16,8 @@
 // What bounds it: for many long rows the stream (4096 x 131072 bf16, k = 64: 229 us, 4.7 TB/s; with the search left
 // out 167 us would be the rate of a copy). The log-sum-exp costs an exponential per logit and about a tenth of that
 // time; steps 2 to 4 are 17,000 of a block's 44,000 cycles, which the other two blocks of an SM hide in part. Four
-// blocks of 64 registers were slower (261 us: they spill), and so was a ring of asynchronous copies (290 us). Few or short rows are bound by the chain of barriers: 15
-// us for one row.
+// blocks of 64 registers were slower (261 us: they spill), and so was a ring of asynchronous copies (290 us). Few or
+// short rows are bound by the chain of barriers: 15 us for one row.
 //
 // A row with more groups than the shared array takes goes through 1 to 3 in segments. A row may also be split over
 // the blocks of a cluster, which share their first bounds and hand their lists to the first block.

@@ -909,8 +909,8 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
 }
 
 // It may run beside sample_list_kernel: the two read the same inputs and write different rows (256 x 131072 bf16, a
-// quarter of the rows here: 68.7 us against 72.5 one after the other; their registers leave little room for both). Its end is the end of
-// both, since its first block waits for the other kernel (and for nothing where that was not launched).
+// quarter of the rows here: 68.7 us against 72.5 one after the other; their registers leave little room for both). Its
+// end is the end of both, since its first block waits for the other kernel (and for nothing where that was not launched).
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 2)
 sample_row_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int parts, int cache_vectors,
