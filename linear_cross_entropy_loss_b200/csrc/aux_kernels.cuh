@@ -521,6 +521,41 @@ __device__ __forceinline__ float cast_to_float<__half>(__half v) { return __half
 template <>
 __device__ __forceinline__ float cast_to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// Row-reference mode. The factor of a row, f * exp(log_base), where it is below what the gradients' operands hold: x * C
+// has to stay a normal number of bf16 / TF32, and entries are divided by C. The window around the reference lets it go down
+// to exp(-72) / V, f (a mass, a regularizer's factor) and the other shards' logits further down without an end.
+// true factor = C * 2^-shift, C >= 2^-100: the row's entries are multiplied by 2^-shift, which is exact.
+constexpr float kLeastFactor = 1e-30f;  // from here on up C is the factor itself
+struct RowFactor {
+  float C;
+  int shift;
+};
+__device__ __forceinline__ RowFactor row_factor(float log_base, float f) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int kNothing = 300;  // 2^-300 times an entry of any type is zero
+  const float exponent = log_base * kLog2e;
+  const float whole = exponent + log2f(fabsf(f));
+  RowFactor r;
+  r.shift = whole > -100.f - float(kNothing) ? int(ceilf(-100.f - whole)) : kNothing;
+  r.C = r.shift < kNothing ? f * exp2f(exponent + float(r.shift)) : copysignf(kLeastFactor, f);
+  return r;
+}
+// The block's row times 2^-shift; behind it the whole block may read and write the row.
+template <typename T>
+__device__ __noinline__ void shift_row(T* row, long long columns, int shift) {
+  for (long long c = (long long)threadIdx.x * 8; c < columns; c += (long long)blockDim.x * 8) {  // columns % 8 == 0
+    Vec8<T> v;
+    v.load(row + c);
+    float e[8];
+    v.to_float(e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = ldexpf(e[k], -shift);
+    v.from_float(e);
+    v.store(row + c);
+  }
+  __syncthreads();
+}
+
 // Row-reference mode, after the log-sum-exp is known. One block per row:
 //   C_i = valid_i * exp(ref_i - lse_i) * (1 + 2 z_reg lse_i)        -> row_coef[i]   (factor of dx), moved to the
 //         nearest value whose reciprocal is a T number

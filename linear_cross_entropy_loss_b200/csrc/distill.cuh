@@ -213,6 +213,7 @@ __global__ void close_rescue_kernel(PassScalars* sc, int* rescue_groups, int n_g
 
 // Row-reference mode (see row_finish_kernel): one block per row,
 //   C = Q exp(ref - lse);  xs = C x;  slab[listed] = (Q softmax - q) / C, from the fp32 logit and rounded once.
+// Where C is too small for that (row_factor) the slab takes the powers of two that are missing.
 template <typename T>
 __global__ void __launch_bounds__(256)
 distill_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ xs, long long xs_ld, int hidden,
@@ -224,7 +225,11 @@ distill_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ x
   const float l = exists ? lse[r] : 0.f;
   const float Q = exists ? mass[r] : 0.f;
   float C = Q != 0.f ? Q * __expf(ref[r] - l) : 0.f;
-  if (Q != 0.f && fabsf(C) < 1e-30f) C = 1e-30f;  // keeps the entries finite
+  if (Q != 0.f && C < kLeastFactor) {  // (the whole block)
+    const RowFactor f = row_factor(ref[r] - l, Q);
+    shift_row(slab + (long long)r * slab_ld, slab_ld, f.shift);
+    C = f.C;
+  }
   if (threadIdx.x == 0) row_coef[r] = C;
   if (r == 0) close_rescue(sc, rescue_groups, n_groups, rows_valid);
   if (Q != 0.f) {
