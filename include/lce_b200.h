@@ -132,6 +132,8 @@ int lce_combine_chunk(const lce_problem* p, const float* row_parts_all, const in
  *                per-row factor c_i = exp(b_i - lse_i)(1 + 2 z_reg lse_i) minus the one-hot; only the label
  *                entry of each row is touched (slab[i, y_i] -= 1/c_i), c_i goes into the epilogue of dx and
  *                into a scaled copy c_i * x_i of the chunk's x rows that dW is computed from.
+ *                (Where c_i is below 1e-30 -- logits far above the base, another shard's far above this one's -- the
+ *                row of the slab is multiplied by the powers of two that keep c_i above it.)
  *                Needs lce_combine_chunk of the same rows.
  * lce_dx_chunk   dx rows = dZ W^T * logit_scale / n_valid (ops.py:317,332). dx: [n_rows_total, hidden]
  *                with row stride dx_ld and element type dx_dtype (LCE_DTYPE_*).

@@ -561,7 +561,8 @@ __device__ __noinline__ void shift_row(T* row, long long columns, int shift) {
 //         nearest value whose reciprocal is a T number
 //   xs[i, :] = C_i * x[i, :]                                        (A operand of dW = xs^T slab)
 //   slab[i, y_i] -= 1 / C_i   if this rank owns column y_i          (so that C_i * slab[i, :] = dZ[i, :])
-// ref_i is the base the row's partials were computed with (parts[0]).
+// ref_i is the base the row's partials were computed with (parts[0]). Where C_i is too small for that (row_factor) the slab
+// takes the powers of two that are missing.
 template <typename T>
 __global__ void __launch_bounds__(256)
 row_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ xs, long long xs_ld, int hidden,
@@ -576,7 +577,11 @@ row_finish_kernel(const T* __restrict__ x, long long x_ld, T* __restrict__ xs, l
   const bool valid = (yv != ignore_index);
   const float l = exists ? lse[r] : 0.f;
   float C = valid ? __expf(ref[r] - l) * (1.f + 2.f * z_regularization * l) : 0.f;
-  if (valid && fabsf(C) < 1e-30f) C = (C < 0.f) ? -1e-30f : 1e-30f;  // keeps 1 / C finite
+  if (valid && fabsf(C) < kLeastFactor) {  // (the whole block)
+    const RowFactor f = row_factor(ref[r] - l, 1.f + 2.f * z_regularization * l);
+    shift_row(slab + (long long)r * slab_ld, slab_ld, f.shift);
+    C = f.C;
+  }
   // The label entry carries the dominant term of the row's gradient (softmax - 1 is close to -1 there), so it is
   // kept exact: the factor is nudged (by at most half an ulp of T, the size of the rounding every softmax entry
   // gets anyway) to the nearest value whose reciprocal is representable in T. slab[i, y_i] - 1 / C then rounds
