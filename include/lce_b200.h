@@ -328,7 +328,8 @@ int lce_grad_scale_pair(void* a, int64_t a_ld, int64_t a_rows, int64_t a_cols, v
 /* out[r, j] = scale * sum_h x[r, h] W[h, j] in fp32: the logits themselves, for the operators below. No counterpart in
  * the reference. The contraction of the loss with its plain epilogue; x, weight as for lce_forward_chunk (hidden % 8 == 0,
  * rows on 16-byte boundaries, any rows and vocabulary); out: rows out_ld >= vocab elements apart, on 16-byte boundaries.
- * dev_status: one device int, 0 before the call; not 0 afterwards if a bounded wait in the kernel ran out. */
+ * dev_status: one device int, 0 before the call; not 0 afterwards if a bounded wait in the kernel ran out, and out is NaN
+ * in every place then (lce_top_logits answers NaN, lce_sample_logits token -1). */
 int lce_linear_logits(int32_t dtype, const void* x, int64_t x_ld, const void* weight, int64_t w_ld, int64_t rows,
                       int64_t hidden, int64_t vocab, float scale, float* out, int64_t out_ld, int32_t* dev_status,
                       void* stream);

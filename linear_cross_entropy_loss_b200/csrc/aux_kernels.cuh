@@ -670,4 +670,13 @@ scale_cast_kernel(const S* src, long long src_ld, D* dst, long long dst_ld, long
   }
 }
 
+// After a contraction whose result goes out as it is: NaN in every place of it if one of its bounded waits ran out, for some
+// tiles were not written then. (Otherwise every block ends at once.)
+__global__ void __launch_bounds__(256)
+fail_matrix_kernel(const int* __restrict__ status, float* __restrict__ m, long long ld, long long rows, long long cols) {
+  if (*status == 0) return;
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+    for (long long c = threadIdx.x; c < cols; c += blockDim.x) m[r * ld + c] = NAN;
+}
+
 }  // namespace lce

@@ -1599,7 +1599,10 @@ int lce_linear_logits(int32_t dtype, const void* x, int64_t x_ld, const void* we
   gp.out_scale = scale;
   gp.out_tma = 1;
   gp.status = dev_status;
-  return launch_gemm_dtype<false, true, EPI_F32, false>(dtype, ta, tb, tc, gp, sms, (cudaStream_t)stream, pair);
+  cudaStream_t st = (cudaStream_t)stream;
+  if ((v = launch_gemm_dtype<false, true, EPI_F32, false>(dtype, ta, tb, tc, gp, sms, st, pair)) != LCE_OK) return v;
+  fail_matrix_kernel<<<(unsigned)std::min<long long>(rows, sms), 256, 0, st>>>(dev_status, out, out_ld, rows, vocab);
+  return check_launch();
 }
 
 int lce_align_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype, int64_t rows,

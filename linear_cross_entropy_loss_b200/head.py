@@ -96,7 +96,8 @@ def _head_operands(x: torch.Tensor, At: torch.Tensor):
 
 
 def _logit_rows(x, At, scale: float) -> torch.Tensor:
-    """(rows, V) float32 logits, rows on 16-byte boundaries."""
+    """(rows, V) float32 logits, rows on 16-byte boundaries. NaN throughout if a wait inside the contraction ran out: the
+    status word is looked at on the device."""
     if torch.compiler.is_compiling():
         return linear_logits_op(x, At, float(scale))
     V = At.shape[1]
