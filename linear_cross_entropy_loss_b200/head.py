@@ -206,19 +206,22 @@ def sample_logits(
     if u.dim() != 1 or not u.is_contiguous():
         u = u.detach().reshape(-1).contiguous()
     s.u = u.data_ptr()
+    s.temperature_all = s.top_p_all = 1.0  # numbers that the library takes, where a tensor (or no row) stands for them
     alive = []  # what the pointers in `s` refer to, until the kernel has been enqueued
-    for name, dtype, value in (("temperature", torch.float32, temperature), ("top_k", torch.int32, top_k),
-                               ("top_p", torch.float32, top_p), ("min_p", torch.float32, min_p)):
+    for name, dtype, value, valid, rule in (
+        ("temperature", torch.float32, temperature, lambda v: v >= 0, "temperature must not be negative"),
+        ("top_k", torch.int32, top_k, lambda v: v >= 0, "top_k must not be negative"),
+        ("top_p", torch.float32, top_p, lambda v: 0 < v <= 1, "top_p must lie in (0, 1]"),
+        ("min_p", torch.float32, min_p, lambda v: 0 <= v <= 1, "min_p must lie in [0, 1]"),
+    ):
         number, tensor = _setting(value, name, dtype, n, dev)
         if tensor is None:
-            setattr(s, f"{name}_all", min(int(number), 2**62) if name == "top_k" else float(number))
+            number = min(int(number), 2**62) if name == "top_k" else float(number)
+            assert valid(number), rule
+            setattr(s, f"{name}_all", number)
         else:
             alive.append(tensor)
             setattr(s, name, tensor.data_ptr())
-    assert s.temperature or s.temperature_all >= 0, "temperature must not be negative"
-    assert s.top_k or s.top_k_all >= 0, "top_k must not be negative"
-    assert s.top_p or 0 < s.top_p_all <= 1, "top_p must lie in (0, 1]"
-    assert s.min_p or 0 <= s.min_p_all <= 1, "min_p must lie in [0, 1]"
     backend = get_backend()
     _require_cuda(backend, rows, u)
     tokens = torch.empty(n, dtype=torch.int64, device=dev)

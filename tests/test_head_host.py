@@ -1,0 +1,83 @@
+"""The operators of a head without a GPU, on a stand-in for the library: batches without rows."""
+import pytest
+import torch
+
+from linear_cross_entropy_loss_b200 import linear_sample, ops, sample_logits
+
+
+class Stub:
+    """Answers of the right shape for every call (and, of the logits and lists, the right ones)."""
+
+    requires_cuda = False
+
+    def linear_logits(self, x, At, scale, out, status):
+        out[:, :At.shape[1]] = scale * (x.float() @ At.float())
+
+    def top_logits(self, logits, k, temperature, values, indices, lse):
+        v, i = torch.topk(logits, k, dim=1)
+        values.copy_(v), indices.copy_(i), lse.copy_(torch.logsumexp(logits.float() / temperature, 1))
+
+    def sample_logits(self, logits, sampling, tokens, logprobs):
+        self.sampling = sampling
+        tokens.copy_(logits.argmax(1)), logprobs.zero_()
+
+    def distill_workspace_bytes(self, prob, k):
+        return 8
+
+    def distill_pass(self, prob, teacher, x, At, workspace, dx, dW, dW_res, loss):
+        loss.fill_(1.0)
+        for d in (dx, dW):
+            if d is not None:
+                d.fill_(0.5)
+
+    def align_rows(self, src, dst):
+        dst.copy_(src)
+
+    def grad_scale_pair(self, a, b, factor):
+        for m in (a, b):
+            m.copy_(m.float() * factor)
+
+    def grad_scale_cast(self, src, dst, factor):
+        dst.copy_(src.float() * factor)
+
+
+@pytest.fixture
+def stub():
+    backend = Stub()
+    ops.set_backend(backend)
+    yield backend
+    ops.set_backend(None)
+
+
+# ---------------------------------------------------------------------------------------------------- no rows
+SETTINGS = [dict(temperature=0.7), dict(top_k=4), dict(top_p=0.9), dict(min_p=0.1)]
+
+
+@pytest.mark.parametrize("kw", SETTINGS, ids=lambda kw: next(iter(kw)))
+@pytest.mark.parametrize("entries", [0, 1])
+@pytest.mark.parametrize("lead", [(0,), (0, 3), (2, 0)])
+def test_an_empty_batch_with_settings_per_row(stub, kw, entries, lead):
+    ((name, value),) = kw.items()
+    per_row = torch.full((entries,), value)
+    got = sample_logits(torch.zeros(*lead, 8), torch.zeros(lead), **{name: per_row})
+    assert got.tokens.shape == lead and got.tokens.dtype == torch.int64 and got.logprobs.shape == lead
+    head = linear_sample(torch.zeros(*lead, 16), torch.zeros(16, 8), torch.zeros(lead), **{name: per_row})
+    assert head.tokens.shape == lead and head.logprobs.shape == lead
+
+
+@pytest.mark.parametrize("kw", [dict(temperature=-1.0), dict(top_k=-1), dict(top_p=0.0), dict(min_p=2.0)])
+def test_an_empty_batch_is_refused_what_a_full_one_is(stub, kw):
+    for n in (0, 3):
+        with pytest.raises(AssertionError):
+            sample_logits(torch.zeros(n, 8), torch.zeros(n), **kw)
+
+
+def test_the_library_takes_an_empty_batch_as_the_python_layer_hands_it_over(stub):
+    """Pointers of empty tensors are null: the numbers that then count have to be ones that the C entry accepts."""
+    import ctypes
+
+    from linear_cross_entropy_loss_b200 import _native
+
+    none = torch.zeros(0)
+    sample_logits(torch.zeros(0, 8), none, temperature=none, top_k=none.int(), top_p=none, min_p=none)
+    assert _native.load().lce_sample_logits(_native.DTYPE_F32, None, 8, 0, 8, ctypes.byref(stub.sampling), None, None, None) == 0
