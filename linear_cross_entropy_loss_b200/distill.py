@@ -206,7 +206,8 @@ def linear_distillation(
         x, At = x.detach(), At.detach()
     if torch.compiler.is_compiling():
         want_grad = torch.is_grad_enabled() and (x.requires_grad or At.requires_grad)
-        return distillation_op(x, At, teacher_logits.detach(), teacher_indices, teacher_lse, float(temperature),
+        lse = None if teacher_lse is None else teacher_lse.reshape(rows)
+        return distillation_op(x, At, teacher_logits.detach(), teacher_indices, lse, float(temperature),
                                float(logit_scale), int(N_chunk_size), want_grad)[0]
     return LinearDistillationImplementation.apply(
         x, At, lists(teacher_logits), lists(teacher_indices), teacher_lse, temperature, logit_scale, N_chunk_size)

@@ -1,8 +1,8 @@
-"""The operators of a head without a GPU, on a stand-in for the library: batches without rows."""
+"""The operators of a head without a GPU, on a stand-in for the library: batches without rows, and traced calls."""
 import pytest
 import torch
 
-from linear_cross_entropy_loss_b200 import linear_sample, ops, sample_logits
+from linear_cross_entropy_loss_b200 import linear_distillation, linear_sample, ops, sample_logits
 
 
 class Stub:
@@ -49,6 +49,10 @@ def stub():
     ops.set_backend(None)
 
 
+def traced(call):
+    return torch.compile(call, fullgraph=True, backend="aot_eager")
+
+
 # ---------------------------------------------------------------------------------------------------- no rows
 SETTINGS = [dict(temperature=0.7), dict(top_k=4), dict(top_p=0.9), dict(min_p=0.1)]
 
@@ -81,3 +85,17 @@ def test_the_library_takes_an_empty_batch_as_the_python_layer_hands_it_over(stub
     none = torch.zeros(0)
     sample_logits(torch.zeros(0, 8), none, temperature=none, top_k=none.int(), top_p=none, min_p=none)
     assert _native.load().lce_sample_logits(_native.DTYPE_F32, None, 8, 0, 8, ctypes.byref(stub.sampling), None, None, None) == 0
+
+
+# ---------------------------------------------------------------------------------------------------- traced calls
+@pytest.mark.parametrize("lead", [(), (6,), (2, 3), (2, 1, 3)])
+@pytest.mark.parametrize("given", [False, True])
+def test_traced_distillation_takes_the_shapes_of_an_eager_one(stub, lead, given):
+    x, At = torch.randn(*lead, 8, requires_grad=True), torch.randn(8, 16, requires_grad=True)
+    t, idx = torch.randn(*lead, 4), torch.randint(0, 16, (*lead, 4))
+    lse = torch.logsumexp(t, -1) if given else None
+    want = linear_distillation(x, t, idx, At, lse)
+    loss = traced(lambda x, At: linear_distillation(x, t, idx, At, lse))(x, At)
+    assert loss.shape == want.shape == () and loss.item() == want.item()
+    loss.backward()
+    assert x.grad.shape == x.shape and At.grad.shape == At.shape
