@@ -56,7 +56,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     assert k <= _native.TOP_MAX, f"k must be at most {_native.TOP_MAX}"
     assert 2**-126 <= temperature < float("inf"), "temperature must be positive"
     if torch.compiler.is_compiling():
-        return TopLogits(*top_logits_op(logits, k, float(temperature)))
+        return TopLogits(*top_logits_op(logits.detach(), k, float(temperature)))
     backend = get_backend()
     _require_cuda(backend, rows)
     lead = logits.shape[:-1]
@@ -192,11 +192,11 @@ def sample_logits(
     answer for a row depends on its inputs alone; weights below half a step are none.
     """
     if torch.compiler.is_compiling():
-        given = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
+        given = [v.detach() if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
         numbers = [default if isinstance(v, torch.Tensor) else v
                    for v, default in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0))]
-        return Sampled(*sample_logits_op(logits, u, *given, float(numbers[0]), int(numbers[1]), float(numbers[2]),
-                                         float(numbers[3])))
+        return Sampled(*sample_logits_op(logits.detach(), u.detach(), *given, float(numbers[0]), int(numbers[1]),
+                                         float(numbers[2]), float(numbers[3])))
     rows = _rows_of(logits)
     n, dev = rows.shape[0], rows.device
     assert u.numel() == n, "u must have one entry per row of the logits"

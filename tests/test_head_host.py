@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from linear_cross_entropy_loss_b200 import linear_distillation, linear_sample, ops, sample_logits
+from linear_cross_entropy_loss_b200 import linear_distillation, linear_sample, ops, sample_logits, top_logits
 
 
 class Stub:
@@ -99,3 +99,19 @@ def test_traced_distillation_takes_the_shapes_of_an_eager_one(stub, lead, given)
     assert loss.shape == want.shape == () and loss.item() == want.item()
     loss.backward()
     assert x.grad.shape == x.shape and At.grad.shape == At.shape
+
+
+def test_traced_lists_and_draws_of_logits_that_require_a_gradient(stub):
+    """They are not differentiable, and do not stand in the way of what is."""
+    x, u = torch.randn(6, 9, requires_grad=True), torch.rand(6)
+
+    def call(x):
+        top, drawn = top_logits(2 * x, 3), sample_logits(2 * x, u, top_p=0.9)
+        return (x * x).sum() + top.values.sum() + top.lse.sum() + drawn.logprobs.sum(), top, drawn
+
+    for run in (call, traced(call)):
+        x.grad = None
+        loss, top, drawn = run(x)
+        assert not any(v.requires_grad for v in (*top, *drawn))
+        loss.backward()
+        assert torch.equal(x.grad, 2 * x.detach())
