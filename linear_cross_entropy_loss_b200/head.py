@@ -123,7 +123,9 @@ def linear_top_logits(x: torch.Tensor, At: torch.Tensor, k: int, temperature: fl
     assert logit_scale > 0 and int(N_chunk_size) >= 1
     rows, A = _head_operands(x, At)
     lead, k = x.shape[:-1], int(k)
-    parts = [top_logits(_logit_rows(c, A, logit_scale), k, temperature) for c in rows.split(int(N_chunk_size))]
+    # (a batch without rows is one chunk without rows; split() of one cannot be traced)
+    chunks = rows.split(int(N_chunk_size)) if rows.shape[0] > 0 else (rows,)
+    parts = [top_logits(_logit_rows(c, A, logit_scale), k, temperature) for c in chunks]
     values, indices, lse = parts[0] if len(parts) == 1 else (torch.cat(t) for t in zip(*parts))
     return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
 

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from linear_cross_entropy_loss_b200 import linear_distillation, linear_sample, ops, sample_logits, top_logits
+from linear_cross_entropy_loss_b200 import (linear_distillation, linear_sample, linear_top_logits, ops, sample_logits,
+                                            top_logits)
 
 
 class Stub:
@@ -115,3 +116,12 @@ def test_traced_lists_and_draws_of_logits_that_require_a_gradient(stub):
         assert not any(v.requires_grad for v in (*top, *drawn))
         loss.backward()
         assert torch.equal(x.grad, 2 * x.detach())
+
+
+def test_traced_head_without_rows(stub):
+    At = torch.randn(8, 16)
+    call = lambda x, u: (*linear_top_logits(x, At, 3), *linear_sample(x, At, u))  # noqa: E731
+    for lead in ((0,), (0, 2), (2, 0)):
+        want = call(torch.zeros(*lead, 8), torch.zeros(lead))
+        got = traced(call)(torch.zeros(*lead, 8), torch.zeros(lead))
+        assert [v.shape for v in got] == [v.shape for v in want]
