@@ -362,6 +362,21 @@ def test_traced_by_torch_compile_without_a_graph_break():
     assert torch.equal(xd.grad, 2 * want[1]) and torch.equal(Ad.grad, 2 * want[2])
 
 
+@pytest.mark.parametrize("factor", [65536.0, 0.3])
+def test_traced_fp16_gradients_are_scaled_like_eager_ones(factor):
+    """A GradScaler's factor is not a number of fp16, the gradients that it scales are."""
+    x, At, t, idx = problem(100, 64, 700, 6, torch.float16, seed=31)
+    td, id_ = t.cuda(), idx.cuda()
+
+    def grads(call):
+        xd, Ad = x.cuda().requires_grad_(), At.cuda().requires_grad_()
+        return torch.autograd.grad(factor * call(xd, Ad), (xd, Ad))
+
+    call = lambda a, b: linear_distillation(a, td, id_, b)  # noqa: E731
+    for got, want in zip(grads(torch.compile(call, fullgraph=True, backend="aot_eager")), grads(call)):
+        assert want.isfinite().all() and torch.equal(got, want)
+
+
 def test_a_head_traced_by_torch_compile_without_a_graph_break():
     head = LinearCrossEntropyLoss(64, 1001, device="cuda", dtype=torch.bfloat16, N_chunk_size=50)
     h, u = torch.randn(4, 30, 64, device="cuda", dtype=torch.bfloat16), torch.rand(4, 30, device="cuda")

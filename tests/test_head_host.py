@@ -125,3 +125,19 @@ def test_traced_head_without_rows(stub):
         want = call(torch.zeros(*lead, 8), torch.zeros(lead))
         got = traced(call)(torch.zeros(*lead, 8), torch.zeros(lead))
         assert [v.shape for v in got] == [v.shape for v in want]
+
+
+@pytest.mark.parametrize("factor", [65536.0, 0.3, 1.0, 2.0 ** -10])
+def test_traced_gradients_are_scaled_like_eager_ones(stub, factor):
+    """The factor of backward is a float: a loss scale that fp16 does not hold, and one that it rounds."""
+    x, At = torch.randn(6, 8).half().requires_grad_(), torch.randn(8, 16).half().requires_grad_()
+    t, idx = torch.randn(6, 4), torch.randint(0, 16, (6, 4))
+
+    def grads(call):
+        x.grad = At.grad = None
+        (call(x, At) * factor).backward()
+        return x.grad, At.grad
+
+    call = lambda x, At: linear_distillation(x, t, idx, At)  # noqa: E731
+    for got, want in zip(grads(traced(call)), grads(call)):
+        assert got.dtype == torch.float16 and torch.equal(got, want)
