@@ -750,7 +750,9 @@ def _fused_pass_backward(ctx, grad_out5, grad_dx, grad_dW):
     if not ctx.lce_want_grad:
         raise RuntimeError("the fused loss was traced without gradients")
     dx, dW = ctx.saved_tensors
-    g = grad_out5[0]  # only the loss is differentiable (reference ops.py:804-810)
+    # Only the loss is differentiable (reference ops.py:804-810). Its gradient keeps one dimension: without any it would be
+    # taken in the gradients' type, where a loss scale of 65536 is infinite (fp16).
+    g = grad_out5[:1]
     return (dx * g).to(dx.dtype), None, (dW * g).to(dW.dtype), None, None, None, None, None, None
 
 

@@ -327,6 +327,20 @@ def test_traced_by_torch_compile_without_a_graph_break():
     assert g_h is not None and g_w is not None
 
 
+@pytest.mark.parametrize("factor", [65536.0, 0.3])
+def test_traced_fp16_gradients_are_scaled_like_eager_ones(factor):
+    """A GradScaler's factor is not a number of fp16, the gradients that it scales are."""
+    x, y, W = (v.cuda() for v in random_problem(100, 64, 704, torch.float16, seed=3))
+
+    def grads(call):
+        xd, Wd = x.clone().requires_grad_(), W.clone().requires_grad_()
+        return torch.autograd.grad(factor * call(xd, Wd), (xd, Wd))
+
+    call = lambda a, b: linear_cross_entropy(a, y, b, ignore_index=-1)[0]  # noqa: E731
+    for got, want in zip(grads(torch.compile(call, fullgraph=True, backend="aot_eager")), grads(call)):
+        assert want.isfinite().all() and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_per_tile_slab_mode_for_bf16_and_fp32(dtype, monkeypatch):
     """LCE_SLAB_PER_TILE (exp(z - tile max) + one in-place slab pass) gives the same results as the default
