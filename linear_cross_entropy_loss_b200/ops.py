@@ -730,7 +730,7 @@ def fused_pass_op(x: torch.Tensor, y: torch.Tensor, At: torch.Tensor, ignore_ind
                                    monitoring, want_grad)
     if not want_grad:
         return out5, x.new_empty(0), At.new_empty(0)
-    return out5, dx.reshape(x.shape), dA
+    return out5, dx.reshape(x.shape).contiguous(), dA.contiguous()
 
 
 @fused_pass_op.register_fake

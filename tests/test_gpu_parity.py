@@ -341,6 +341,17 @@ def test_traced_fp16_gradients_are_scaled_like_eager_ones(factor):
         assert want.isfinite().all() and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("lead", [(40,), (4, 10), (1, 40), ()])
+@pytest.mark.parametrize("H,V", [(64, 704), (64, 701), (60, 704), (60, 701)])
+def test_the_traced_pass_is_what_its_shapes_promise(lead, H, V):
+    """Sizes and strides of the outputs, at sizes whose rows are padded inside."""
+    x, At = torch.randn(*lead, H, device="cuda").bfloat16(), torch.randn(H, V, device="cuda").bfloat16()
+    y = torch.randint(0, V, lead, device="cuda")
+    for want_grad in (True, False):
+        torch.library.opcheck(torch.ops.lce_b200.fused_pass.default, (x, y, At, -100, 0.0, 1.0, 4096, False, want_grad),
+                              test_utils=("test_schema", "test_faketensor"))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_per_tile_slab_mode_for_bf16_and_fp32(dtype, monkeypatch):
     """LCE_SLAB_PER_TILE (exp(z - tile max) + one in-place slab pass) gives the same results as the default
