@@ -142,7 +142,8 @@ int lce_combine_chunk(const lce_problem* p, const float* row_parts_all, const in
  *                x / W (row stride dw_ld elements), overwritten by the call with first != 0 and complete after
  *                the call with last != 0. For the 16-bit types the running sum is carried as the PAIR
  *                dweight + dweight_residual, both in the element type: each call rounds the new sum to dweight and
- *                the rounding error to dweight_residual (about 16 significant bits together; the reference
+ *                the rounding error (fp16: 2^11 times it, which keeps it out of the subnormal numbers) to
+ *                dweight_residual (about 16 significant bits together, fp16 22; the reference
  *                accumulates fp16 gradients in fp16 and bf16 gradients in an fp32 buffer the size of W, ops.py:
  *                440-444, 693). dweight_residual: scratch of the same shape and row stride (dwr_ld == dw_ld), only
  *                meaningful between the calls of one pass; may be null for a pass of a single call (first and

@@ -1069,7 +1069,7 @@ namespace {
 
 int dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0, int64_t rows, void* workspace,
              void* dweight, int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, int32_t first, int32_t last,
-             void* stream, float grad_scale, float res_scale) {
+             void* stream, float grad_scale) {
   int v = validate_problem(p);
   if (v != LCE_OK) return v;
   if ((v = check_chunk(p, row0, rows)) != LCE_OK) return v;
@@ -1129,7 +1129,7 @@ int dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0, in
     gp.out_res = need_res ? dweight_residual : nullptr;
     gp.out_pair_ld = dw_ld;
     gp.out_pair_last = last ? 1 : 0;
-    gp.out_res_scale = res_scale;
+    gp.out_res_scale = p->dtype == LCE_DTYPE_F16 ? 2048.f : 1.f;
   } else {
     gp.out = reinterpret_cast<float*>(dweight);
     gp.out_ld = dw_ld;
@@ -1159,7 +1159,7 @@ int lce_dw_chunk(const lce_problem* p, const void* x, int64_t x_ld, int64_t row0
   const int v = validate_problem(p);
   if (v != LCE_OK) return v;
   return dw_chunk(p, x, x_ld, row0, rows, workspace, dweight, dw_ld, dweight_residual, dwr_ld, first, last, stream,
-                  p->logit_scale, 1.f);
+                  p->logit_scale);
 }
 
 int lce_backward_chunk(const lce_problem* p, const void* x, int64_t x_ld, const void* weight, int64_t w_ld,
@@ -1555,7 +1555,7 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
     if (dx && (v = dx_chunk(p, weight, w_ld, row0, rows, workspace, dx, dx_ld, p->dtype, stream, d.grad_scale)) != LCE_OK)
       return v;
     if (dweight && (v = dw_chunk(p, x, x_ld, row0, rows, workspace, dweight, dw_ld, dweight_residual, dwr_ld, ci == 0,
-                                 ci == n_chunks - 1, stream, d.grad_scale, p->dtype == LCE_DTYPE_F16 ? 2048.f : 1.f)) != LCE_OK)
+                                 ci == n_chunks - 1, stream, d.grad_scale)) != LCE_OK)
       return v;
   }
   distill_finalize_kernel<<<1, 1024, 0, st>>>(w.pass.scalars, w.row_loss, (long long)p->n_rows_total, temperature, loss);

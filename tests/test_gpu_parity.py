@@ -451,3 +451,24 @@ def test_device_status_is_clean_after_a_pass():
     x, y, W = random_problem(256, 256, 512, torch.bfloat16, seed=15)
     out5, dx, dA, ws = ops.run_pass(x.cuda(), y.cuda(), W.cuda(), -1, 0.0, 1.0, 128, False, True)
     assert ops.get_backend().read_status(ws) == 0
+
+
+# ---------------------------------------------------------------------------------------------------- dW over chunks
+@pytest.mark.parametrize("H,V", [(64, 9000), (72, 9001)])
+def test_small_fp16_gradients_summed_over_chunks(H, V):
+    """dW below fp16's normal numbers, as value and residual over 16 chunks, against the sum of a single one. The same
+    entries of dZ are summed in fp32 and rounded once at the end, so the two differ where the sum lies within the residuals'
+    error of a midpoint: 15 residuals of half a step of 2^-35 each (the residual is kept 2^11 times as large) on both sides
+    of a midpoint every 2^-24, 15 * 2^-11 of all entries if they all point the same way, and the fp32 sums' own order."""
+    N = 2048
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(N, H, generator=g).half()
+    At = (torch.randn(H, V, generator=g).clamp(-2, 2) * H ** -0.5).half()
+    y = torch.randint(0, V, (N,), generator=g)
+    whole = run_gpu(x, y, At, chunk=4096, monitoring=False)
+    parts = run_gpu(x, y, At, chunk=128, monitoring=False)
+    a, b = whole[2].double(), parts[2].double()
+    assert (a.abs() < 2.0 ** -14).double().mean() > 0.5  # most of them are subnormal
+    step = torch.maximum(a.abs(), torch.full_like(a, 2.0 ** -14)).log2().floor().exp2() * 2.0 ** -10
+    assert ((a - b).abs() <= step).all()
+    assert (a != b).double().mean().item() <= 2.0 ** -6
