@@ -84,7 +84,7 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
       float l = -INFINITY;
       if (k < t.k) {
         col = teacher_column(t, row0 + r, k, vocab);
-        if (col != 0xffffffffu) l = teacher_logit(t, row0 + r, k) * t.inv_temperature;
+        if (col != 0xffffffffu) l = teacher_logit(t, row0 + r, k);
         if (!(l > -INFINITY) && l == l) col = 0xffffffffu;  // -inf: no weight
       }
       bad |= l != l || l == INFINITY;
@@ -94,14 +94,20 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     bad = __any_sync(0xffffffffu, bad);
-    float base = top;  // q = exp(l - base) / total
+    // q = exp(log_share) / total. Without a given log-sum-exp the largest logit comes off before the division by T: finite
+    // logits over a low T may be more than a float holds, their distances are what counts.
+    const bool given = t.lse != nullptr;
+    const float base = given ? t.lse[row0 + r] : 0.f;
+    auto log_share = [&](float l) {
+      if (!given) return (l - top) * t.inv_temperature;
+      const float scaled = l * t.inv_temperature;
+      return scaled > -INFINITY ? scaled - base : -INFINITY;
+    };
     float total = 1.f;
-    if (t.lse != nullptr) {
-      base = t.lse[row0 + r];
-    } else {
+    if (!given) {
       total = 0.f;
       for (int k = lane; k < padded; k += 32)
-        if (uint32_t(mine[k] >> 32) != 0xffffffffu) total += expf(__uint_as_float(uint32_t(mine[k])) - base);
+        if (uint32_t(mine[k] >> 32) != 0xffffffffu) total += expf(log_share(__uint_as_float(uint32_t(mine[k]))));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
@@ -111,7 +117,7 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
       uint32_t col = uint32_t(mine[k] >> 32);
       float q = 0.f;
       if (col != 0xffffffffu) {
-        const float log_q = __uint_as_float(uint32_t(mine[k])) - base - log_total;
+        const float log_q = log_share(__uint_as_float(uint32_t(mine[k]))) - log_total;
         q = bad ? __uint_as_float(0x7fc00000u) : expf(log_q);
         if (q == 0.f) col = 0xffffffffu;
         else ent += q * log_q;

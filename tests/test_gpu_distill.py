@@ -108,6 +108,20 @@ def test_entries_without_weight():
     check(x, At, t, idx)
 
 
+@pytest.mark.parametrize("dtype,T", [(torch.bfloat16, 0.5), (torch.float32, 0.25), (torch.float32, 0.9), (torch.float16, 0.5)])
+def test_lists_at_the_ends_of_a_type_at_low_temperatures(dtype, T):
+    """Finite logits have weight whatever they are: divided by the temperature they may be more than a float holds, their
+    distances from the largest one are what counts."""
+    x, At, t, idx = problem(64, 64, 700, 9, torch.bfloat16, seed=30, t_dtype=dtype)
+    lowest, largest = torch.finfo(dtype).min, torch.finfo(dtype).max
+    t[6], t[7] = lowest, largest         # nine equal ones
+    t[8], t[8, 3] = lowest, 1.0          # one far above the others
+    t[9], t[9, 3:5] = lowest, largest
+    t[10, 2:] = -math.inf
+    t[10, :2] = lowest
+    check(x, At, t, idx, T=T)
+
+
 def test_an_index_listed_twice_counts_twice():
     x, At, t, idx = problem(70, 64, 700, 10, torch.bfloat16, seed=10)
     idx[:, 3] = idx[:, 0]
