@@ -159,8 +159,8 @@ int lce_top_logits(int32_t dtype, const void* logits, int64_t ld, int64_t rows, 
                    float temperature, void* values, int64_t* indices, float* lse, void* stream) {
   const int v = check_rows(dtype, logits, ld, rows, vocab);
   if (v != LCE_OK) return v;
-  // (a temperature whose reciprocal is a number too)
-  if (k < 1 || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.f / temperature < INFINITY))
+  // (a temperature whose log2(e) / T, the scale of the exponents, is a number too)
+  if (k < 1 || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.f / temperature * kLog2e < INFINITY))
     return LCE_ERR_INVALID_ARGUMENT;
   if (k > vocab || k > LCE_TOP_MAX) return LCE_ERR_TOO_LARGE;
   if (rows == 0) return LCE_OK;

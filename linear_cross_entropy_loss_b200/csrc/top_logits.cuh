@@ -6,6 +6,8 @@
 
 namespace lce {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads, 3)
 top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, int k, int parts, float inv_temperature,
@@ -16,7 +18,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, uint32_t vocab, in
   const int part = int(blockIdx.x % parts);
   const RowGroups<T> row(logits + r * ld, vocab);
   const int v0 = int((long long)row.groups * part / parts), v1 = int((long long)row.groups * (part + 1) / parts);
-  const float log2_scale = inv_temperature * 1.4426950408889634f;
+  const float log2_scale = inv_temperature * kLog2e;
   float ref, sum;
   stream_top<T, true, Nan::kFirst>(s, row, v0, v1, parts, k, log2_scale, ref, sum);
   const float m = block_max(ref, s.scratch);

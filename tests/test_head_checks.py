@@ -265,3 +265,9 @@ def test_head_operators_refuse():
     for call in (lambda: linear_logits(x, At), lambda: linear_top_logits(x, At, 3), lambda: linear_sample(x, At, torch.zeros(4))):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
+
+
+@pytest.mark.parametrize("t", [4.2e-39, 3.2e-39, 2.0 ** -128])
+def test_top_logits_abi_refuses_temperatures_whose_scale_is_not_a_float(lib, t):
+    """1 / t is one down to just above 2^-128, log2(e) / t, which the exponentials use, is not."""
+    assert lib.lce_top_logits(1, 16, 100, 4, 100, 8, t, 16, 16, 16, None) == -1
