@@ -308,7 +308,7 @@ typedef struct lce_teacher {
   int32_t k;            /* 1 .. LCE_TEACHER_MAX */
   int32_t logits_dtype; /* LCE_DTYPE_* */
   int32_t indices_bits; /* 32 or 64 */
-  float temperature;    /* T > 0 */
+  float temperature;    /* T > 0; logit_scale / T and logit_scale * T have to be floats above 0 */
 } lce_teacher;
 int lce_distill_workspace_bytes(const lce_problem* p, int32_t k, size_t* bytes);
 int lce_distill_pass(const lce_problem* p, const lce_teacher* teacher, const void* x, int64_t x_ld,

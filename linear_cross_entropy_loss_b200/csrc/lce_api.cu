@@ -1490,14 +1490,18 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
   if (!x || !weight || !workspace || !loss) return LCE_ERR_INVALID_ARGUMENT;
   if (!p_in->want_grad && (dx || dweight)) return LCE_ERR_INVALID_ARGUMENT;
   if (p_in->want_grad && !dx && !dweight) return LCE_ERR_INVALID_ARGUMENT;
-  int sms = 0;
-  if ((v = ensure_device(&sms)) != LCE_OK) return v;
-
   lce_problem prob = *p_in;
   const lce_problem* p = &prob;
   prob.logit_scale = p_in->logit_scale / temperature;
   prob.ignore_index = kIgnoredRow;
-  if (!(prob.logit_scale > 0.f)) return LCE_ERR_INVALID_ARGUMENT;
+  Distill d;
+  d.boost = p->dtype == LCE_DTYPE_F16 ? 16384.f : 1.f;
+  d.grad_scale = p_in->logit_scale * temperature / d.boost;
+  for (const float scale : {prob.logit_scale, d.grad_scale})
+    if (!(scale > 0.f) || !(scale < INFINITY)) return LCE_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  if ((v = ensure_device(&sms)) != LCE_OK) return v;
+
   const DistillWorkspace w = layout_distill(p, teacher->k, workspace, sms);
   cudaStream_t st = (cudaStream_t)stream;
   TeacherInput in;
@@ -1511,9 +1515,6 @@ int lce_distill_pass(const lce_problem* p_in, const lce_teacher* teacher, const 
   in.indices_64 = teacher->indices_bits == 64;
   in.inv_temperature = 1.f / temperature;
 
-  Distill d;
-  d.boost = p->dtype == LCE_DTYPE_F16 ? 16384.f : 1.f;
-  d.grad_scale = p_in->logit_scale * temperature / d.boost;
   d.list_z = w.list_z;
   d.lists.idx = w.list_idx;
   d.lists.q = w.list_q;

@@ -178,6 +178,8 @@ def linear_distillation(
     assert teacher_indices.dtype in (torch.int64, torch.int32), "teacher_indices must be int64 or int32"
     assert 2**-126 <= temperature < float("inf"), "temperature must be positive"
     assert logit_scale > 0
+    for scale in (logit_scale / temperature, logit_scale * temperature):  # of the logits, of the gradients
+        assert 2**-126 <= scale < 2**128, "logit_scale and temperature scale the logits or their gradients out of range"
     assert int(N_chunk_size) >= 1
     assert x.numel() > 0 and At.shape[1] >= 1, "x must have at least one row"
     if teacher_lse is not None:

@@ -271,3 +271,13 @@ def test_head_operators_refuse():
 def test_top_logits_abi_refuses_temperatures_whose_scale_is_not_a_float(lib, t):
     """1 / t is one down to just above 2^-128, log2(e) / t, which the exponentials use, is not."""
     assert lib.lce_top_logits(1, 16, 100, 4, 100, 8, t, 16, 16, 16, None) == -1
+
+
+
+@pytest.mark.parametrize("scale,t", [(1e20, 1e-30), (1e-30, 1e20), (1e25, 1e20)])
+def test_a_scale_that_the_temperature_takes_out_of_range_is_refused(lib, scale, t):
+    """The logits are scaled by scale / t, the gradients by scale * t: both have to be floats above zero."""
+    assert call_distill(lib, distill_problem(logit_scale=scale), teacher(temperature=t)) == -1
+    a = distill_args()
+    with pytest.raises(AssertionError):
+        linear_distillation(**a, temperature=t, logit_scale=scale)
