@@ -316,8 +316,9 @@ int lce_distill_pass(const lce_problem* p, const lce_teacher* teacher, const voi
                      int64_t dw_ld, void* dweight_residual, int64_t dwr_ld, float* loss, void* stream);
 
 /* dst[r, c] = src[r, c] for src rows that start anywhere (src_ld elements apart) and dst rows on 16-byte boundaries:
- * what x and W need before a pass when their sizes are not multiples of 16 bytes. Whole vectors of 16 bytes are written, so dst_ld must
- * be at least cols rounded up to them; what lies behind column cols is unspecified. No counterpart in the reference. */
+ * what x and W need before a pass when their sizes are not multiples of 16 bytes. Whole vectors of 16 bytes are
+ * written, so dst_ld must be at least cols rounded up to them; what lies behind column cols is unspecified. No
+ * counterpart in the reference. */
 int lce_align_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype, int64_t rows,
                    int64_t cols, void* stream);
 

@@ -12,9 +12,9 @@
 //   distill_finish_kernel / distill_dz_kernel   dZ from the slab, with the listed entries written from their fp32 logits
 // then the dx and dW contractions as they are.
 //
-// What bounds it: the three contractions, 6 N H V operations. At N=4096 H=2048 V=32768 K=32 (bf16) they take 1,077 of
-// the 1,189 us of a step's kernels, everything that distillation adds (preparing the lists, copying the listed
-// logits, dZ) 35 us; at N=8192 H=2048 V=131072 K=64 a step takes 10.5 ms, 1,260 TFLOP/s.
+// What bounds it: the three contractions, 6 N H V operations. At N=4096 H=2048 V=32768 K=32 (bf16) they take 1,060 of
+// the 1,164 us of a step's kernels (one after the other, cold), preparing the lists 14, the listed entries of dZ and the
+// scaled rows of x 17; at N=8192 H=2048 V=131072 K=64 a step takes 10.5 to 11.1 ms, 1,190 to 1,260 TFLOP/s.
 //
 // Roundings to the element type. dZ is an operand of the tensor cores, so the slab has the type of x: one rounding of
 // each entry (listed entries once, from fp32). One base per row (bf16, fp32 slabs): the row's factor C goes into the
@@ -94,8 +94,8 @@ teacher_prepare_kernel(const TeacherInput t, long long row0, int rows, long long
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     bad = __any_sync(0xffffffffu, bad);
-    // q = exp(log_share) / total. Without a given log-sum-exp the largest logit comes off before the division by T: finite
-    // logits over a low T may be more than a float holds, their distances are what counts.
+    // q = exp(log_share) / total. Without a given log-sum-exp the largest logit comes off before the division by T:
+    // finite logits over a low T may be more than a float holds, their distances are what counts.
     const bool given = t.lse != nullptr;
     const float base = given ? t.lse[row0 + r] : 0.f;
     auto log_share = [&](float l) {

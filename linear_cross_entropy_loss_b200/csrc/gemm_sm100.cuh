@@ -87,15 +87,15 @@ struct GemmParams {
   float out_scale;             // coef = out_scale / (*out_div)   (out_div may be null: coef = out_scale)
   const float* out_div;
   // ---- EPI_F32, 16-bit element types: accumulation across launches as a pair of arrays in the ELEMENT type,
-  // sum = out_sum + out_res with out_sum = round(sum) and out_res = round(sum - out_sum) (about 16 significant
-  // bits, against the 8 or 11 of the result). out_sum is the result itself after the last launch: no fp32
+  // sum = out_sum + out_res with out_sum = round(sum) and out_res = round(sum - out_sum) (about 16 significant bits,
+  // 22 of fp16, against the 8 or 11 of the result). out_sum is the result itself after the last launch: no fp32
   // accumulator the size of the output, no conversion pass. `accumulate` = 0 for the first launch; out_res may be
   // null when nothing follows (last launch: the residual is not written) -- a single launch needs none at all.
   void* out_sum;
   void* out_res;
   long long out_pair_ld;       // elements between rows of out_sum and of out_res
-  float out_res_scale;         // fp16: out_res holds the residual times this power of two (2^11 keeps it below out_sum and
-                               // out of the subnormal numbers, whose step of 2^-24 every launch would round to again)
+  float out_res_scale;         // fp16: out_res holds the residual times this power of two (2^11 keeps it below out_sum
+                               // and out of the subnormal numbers, to whose step of 2^-24 every launch would round again)
   int out_pair_last;           // 1: last launch of the accumulation
   int out_rows;                // rows / columns of the output that exist; tiles may hang over both edges
   int out_cols;
@@ -368,8 +368,9 @@ __device__ __forceinline__ void slab_chunk_via_tma(const GemmParams& p, const CU
 }
 
 // The logits at the listed columns of this tile. A thread cannot index its registers by a column that differs from row
-// to row, but the accumulator is still in tensor memory: the warp walks the columns that any of its 32 rows lists, loads each once for all
-// rows, and the rows that list it keep it. 32 rows with 64 listed columns of 131072 have 4 such columns in a tile.
+// to row, but the accumulator is still in tensor memory: the warp walks the columns that any of its 32 rows lists,
+// loads each once for all rows, and the rows that list it keep it. 32 rows with 64 listed columns of 131072 have 4 such
+// columns in a tile.
 __device__ __forceinline__ void gather_listed(const GemmParams& p, uint32_t taddr, int n_blk, long long r, bool row_ok) {
   int at = 0, end = 0;
   if (row_ok) {

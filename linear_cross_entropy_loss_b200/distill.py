@@ -223,7 +223,8 @@ def distillation_op(x: torch.Tensor, At: torch.Tensor, t: torch.Tensor, idx: tor
     """(loss, dx, dAt); the gradients are empty without want_grad."""
     xd, Ad = x.detach(), At.detach()
     if not want_grad:
-        return linear_distillation(xd, t, idx, Ad, lse, temperature, logit_scale, N_chunk_size), x.new_empty(0), x.new_empty(0)
+        loss = linear_distillation(xd, t, idx, Ad, lse, temperature, logit_scale, N_chunk_size)
+        return loss, x.new_empty(0), x.new_empty(0)
     with torch.enable_grad():
         xd, Ad = xd.requires_grad_(), Ad.requires_grad_()
         loss = linear_distillation(xd, t, idx, Ad, lse, temperature, logit_scale, N_chunk_size)
@@ -248,8 +249,8 @@ def _distillation_backward(ctx, grad_loss, grad_dx, grad_dA):
     if not ctx.lce_want_grad:
         raise RuntimeError("the distillation loss was traced without gradients")
     dx, dA = ctx.saved_tensors
-    # As a tensor of one dimension the factor stays the float that it is (one without would be taken in the gradients' type:
-    # a loss scale of 65536 is infinite in fp16); each gradient is rounded once, as in the eager call.
+    # As a tensor of one dimension the factor stays the float that it is (one without would be taken in the gradients'
+    # type: a loss scale of 65536 is infinite in fp16); each gradient is rounded once, as in the eager call.
     factor = grad_loss.reshape(1)
     return (dx * factor).to(dx.dtype), (dA * factor).to(dA.dtype), None, None, None, None, None, None, None
 
