@@ -26,6 +26,7 @@ from .ops import (
     _scaled_grads,
     _tma_ready,
     get_backend,
+    scaled_op,
     slab_mode_policy,
 )
 
@@ -249,10 +250,7 @@ def _distillation_backward(ctx, grad_loss, grad_dx, grad_dA):
     if not ctx.lce_want_grad:
         raise RuntimeError("the distillation loss was traced without gradients")
     dx, dA = ctx.saved_tensors
-    # As a tensor of one dimension the factor stays the float that it is (one without would be taken in the gradients'
-    # type: a loss scale of 65536 is infinite in fp16); each gradient is rounded once, as in the eager call.
-    factor = grad_loss.reshape(1)
-    return (dx * factor).to(dx.dtype), (dA * factor).to(dA.dtype), None, None, None, None, None, None, None
+    return scaled_op(dx, grad_loss), scaled_op(dA, grad_loss), None, None, None, None, None, None, None
 
 
 distillation_op.register_autograd(_distillation_backward, setup_context=_distillation_setup)

@@ -741,6 +741,20 @@ def _fused_pass_fake(x, y, At, ignore_index, z_regularization, logit_scale, N_ch
     return out5, x.new_empty(x.shape), At.new_empty(At.shape)
 
 
+@torch.library.custom_op("lce_b200::scaled", mutates_args=())
+def scaled_op(grad: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
+    """grad * factor (one float) in fp32, rounded once to the type of grad: what the eager backward's kernels do in place. In
+    the gradient's own type a loss scale of 65536 would be infinite (fp16); as tensor expressions that a tracer records
+    one by one, the fp32 product would exist as a whole."""
+    out = torch.empty_like(grad)
+    return torch.mul(grad, factor.reshape(1), out=out)
+
+
+@scaled_op.register_fake
+def _scaled_fake(grad, factor):
+    return torch.empty_like(grad)
+
+
 def _fused_pass_setup(ctx, inputs, output):
     ctx.lce_want_grad = inputs[-1]
     ctx.save_for_backward(output[1], output[2])
@@ -750,10 +764,8 @@ def _fused_pass_backward(ctx, grad_out5, grad_dx, grad_dW):
     if not ctx.lce_want_grad:
         raise RuntimeError("the fused loss was traced without gradients")
     dx, dW = ctx.saved_tensors
-    # Only the loss is differentiable (reference ops.py:804-810). Its gradient keeps one dimension: without any it would be
-    # taken in the gradients' type, where a loss scale of 65536 is infinite (fp16).
-    g = grad_out5[:1]
-    return (dx * g).to(dx.dtype), None, (dW * g).to(dW.dtype), None, None, None, None, None, None
+    g = grad_out5[0]  # only the loss is differentiable (reference ops.py:804-810)
+    return scaled_op(dx, g), None, scaled_op(dW, g), None, None, None, None, None, None
 
 
 fused_pass_op.register_autograd(_fused_pass_backward, setup_context=_fused_pass_setup)

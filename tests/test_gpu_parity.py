@@ -352,6 +352,19 @@ def test_the_traced_pass_is_what_its_shapes_promise(lead, H, V):
                               test_utils=("test_schema", "test_faketensor"))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gradients_are_scaled_in_fp32_without_a_copy_in_it(dtype):
+    grad = torch.randn(512, 1001, generator=torch.Generator().manual_seed(0)).to(dtype).cuda()
+    for factor in (torch.tensor(0.3).cuda(), torch.tensor(65536.0).cuda()):
+        torch.library.opcheck(torch.ops.lce_b200.scaled.default, (grad, factor), test_utils=("test_schema", "test_faketensor"))
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.ops.lce_b200.scaled(grad, factor)
+        assert torch.cuda.max_memory_allocated() - before <= grad.nbytes + 1024
+        assert torch.equal(got, (grad.float() * factor).to(dtype))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_per_tile_slab_mode_for_bf16_and_fp32(dtype, monkeypatch):
     """LCE_SLAB_PER_TILE (exp(z - tile max) + one in-place slab pass) gives the same results as the default
